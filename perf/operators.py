@@ -117,7 +117,7 @@ def _quantise(x):
     """(codes, s, z) of x (..., D): codes as numbers (..., G, 32), s and z fp16 (..., G)."""
     x = x.float().unflatten(-1, (-1, GROUP)).clamp(-32768.0, 32768.0)
     lo, hi = x.amin(-1), x.amax(-1)
-    s, z = ((hi - lo) / 15.0).half(), lo.half()
+    s, z = ((hi - lo) / torch.full_like(lo, 15.0)).half(), lo.half()  # a quotient: by a number torch multiplies by its inverse
     sf, zf = s.float().unsqueeze(-1), z.float().unsqueeze(-1)
     c = torch.where(sf > 0, ((x - zf) / sf).round().clamp(0.0, 15.0), torch.zeros_like(x))
     return c, s, z
