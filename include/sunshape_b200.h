@@ -368,6 +368,104 @@ int ss_lse_merge(const float* parts, int n_parts, int64_t rows, int d, const flo
  * of the output: part_out f32 [b*hq*tq][d + 2]. */
 int ss_decode_attn_partial(const ss_decode_args* a, float* part_out, void* stream);
 
+/* --------------------------------------------------------------------------
+ * Serving over paged 4-bit KV caches (no counterpart in the reference, whose
+ * caches hold equally long sequences).
+ *
+ * A pool holds n_pages pages of n_heads kv-heads; a page of one head is
+ * page_size / 16 blocks of 16 tokens, each 20 * d bytes (byte layout:
+ * csrc/int4_pages.cuh). Groups of 32 dims share an fp16 scale s and zero z,
+ * value = code * s + z. Slot page * page_size + i is the i-th token of a page.
+ * pages and both strides (bytes) are multiples of 16; d is 64, 128 or 256;
+ * page_size is a multiple of 16.
+ * -------------------------------------------------------------------------- */
+
+/* Block tables and slot maps of one step, from n requests' lengths (n <= 16384).
+ * Request b holds seq_lens[b] tokens and brings q_lens[b] (negative: 0). New
+ * pages are popped from the stack free_pages[0 .. n_free[0]) in request order
+ * and entered into block_table (rows of table_stride ints, width used). Writes
+ *   cu_q[n + 1]      first token of each request
+ *   positions, requests, slots [n_tokens]   of each token; 0, -1, -1 past the last
+ *   new_lens[n], new_free[1]                lengths and free pages after the step
+ *   status[1]        0, or: 1 the pool has too few pages, 2 a table row is too
+ *                    narrow, 4 more new tokens than n_tokens. Then nothing is
+ *                    allocated, every slot is -1, cu_q is 0, lengths stay.
+ * seq_lens and n_free are not changed, so a repeated call repeats its result. */
+int ss_plan_step(const int32_t* seq_lens, const int32_t* q_lens, int n, int32_t* block_table,
+                 int64_t table_stride, int width, const int32_t* free_pages, int n_pages,
+                 const int32_t* n_free, int page_size, int64_t n_tokens, int32_t* cu_q,
+                 int32_t* positions, int32_t* requests, int64_t* slots, int32_t* new_lens,
+                 int32_t* new_free, int32_t* status, void* stream);
+
+/* Pushes the pages of every request with done[b] != 0 back onto the stack and
+ * clears its table row (-1); its new length is 0. status 8: more pages than
+ * are out would come back; nothing is changed then. */
+int ss_release_pages(const int32_t* seq_lens, const uint8_t* done, int n, int32_t* block_table,
+                     int64_t table_stride, int width, int32_t* free_pages, int n_pages,
+                     const int32_t* n_free, int page_size, int32_t* new_lens, int32_t* new_free,
+                     int32_t* status, void* stream);
+
+/* Quantises rows k, v (n tokens, n_heads, d; element strides, dims contiguous)
+ * into the pages at slots[n]; a slot outside the pool (-1: padding) is skipped.
+ * Two tokens of one call must not share a slot. Magnitudes above 2^15
+ * saturate; a NaN marks its group: the group reads as NaN. */
+int ss_int4_append(const void* k, const void* v, int dtype, int64_t k_token_stride,
+                   int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                   const int64_t* slots, int64_t n, int n_heads, int d, void* pages,
+                   int64_t n_pages, int64_t page_stride, int64_t head_stride, int page_size,
+                   void* stream);
+
+/* Reads the rows at slots[n] back into dense (n, n_heads, d) outputs
+ * (16-byte aligned); a slot outside the pool reads as 0. */
+int ss_int4_fetch(const int64_t* slots, int64_t n, int n_heads, int d, const void* pages,
+                  int64_t n_pages, int64_t page_stride, int64_t head_stride, int page_size,
+                  void* k_out, void* v_out, int dtype, void* stream);
+
+/* Attention of ragged requests over the pages. Tokens cu_q[b] .. cu_q[b+1] of
+ * q belong to request b, whose keys are the first seq_lens[b] tokens of its
+ * table row (the new ones included); query row i of q_b stands at position
+ * seq_lens[b] - q_b + i. causal: keys after the position are hidden; window
+ * > 0: so are keys at position - window and before. A row that sees no key
+ * gives 0 and lse -inf; so does a token outside cu_q. Keys on a table entry
+ * outside the pool are hidden. Bits of a page past a request's length are
+ * never used. */
+typedef struct ss_int4_attn_args {
+  const void* q;                  /* (n_tokens, hq, d), dims contiguous */
+  int dtype;                      /* SS_F16 or SS_BF16, of q and out */
+  int64_t q_token_stride, q_head_stride; /* elements */
+  int64_t n_tokens;
+  int hq, hkv, d;
+  const void* pages;
+  int n_pages;
+  int64_t page_stride, head_stride; /* bytes */
+  int page_size;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int width;
+  const int32_t* seq_lens;
+  const int32_t* cu_q;
+  int n_requests;
+  int max_q;                      /* most query rows of a request (a hint for the launch) */
+  float scale;
+  int causal, window;
+  void* out;                      /* (n_tokens, hq, d) dense, 16-byte aligned */
+  float* lse;                     /* (n_tokens, hq) natural logarithm, or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} ss_int4_attn_args;
+
+int ss_int4_attention(const ss_int4_attn_args* a, void* stream);
+
+/* Log probability of targets[r] (int64; < 0: 0, >= vocab: NaN; NULL: all 0),
+ * entropy (nats) and the `top` <= 32 largest logits of each row, by (value
+ * descending, index ascending), with their log probabilities; -1 and -inf
+ * past the vocabulary. logits: rows of row_stride elements, any alignment of
+ * the element type. A row of -inf alone: log probabilities -inf, entropy 0. A
+ * row holding NaN or +inf: NaN everywhere, ids -1. */
+int ss_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t row_stride,
+                      int vocab, const int64_t* targets, int top, float* logprobs,
+                      float* entropy, int32_t* top_ids, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

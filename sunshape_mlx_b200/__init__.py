@@ -38,6 +38,18 @@ from .kernels import (
     reset_kernel_stats,
     unpack_indices,
 )
+from .logprobs import TokenLogprobs, token_logprobs
+from .paged import (
+    Int4PagedKVCache,
+    PageTables,
+    StepPlan,
+    int4_append,
+    int4_attention,
+    int4_fetch,
+    int4_pool,
+    plan_step,
+    release_pages,
+)
 from .value_codecs import GroupedValueCodec, TurboQuantValueCodec
 
 __version__ = "0.3.0+b200"
@@ -52,5 +64,7 @@ __all__ = [
     "fused_attention_causal_metal", "fused_attention_dequant_metal",
     "fused_attention_dequant_causal_metal", "block_vq_quantize_metal", "GroupedValueCodec",
     "TurboQuantValueCodec", "create_kv_cache", "get_kernel_stats", "reset_kernel_stats",
-    "save_cache", "load_cache",
+    "save_cache", "load_cache", "PageTables", "Int4PagedKVCache", "StepPlan", "plan_step",
+    "release_pages", "int4_pool", "int4_append", "int4_fetch", "int4_attention", "token_logprobs",
+    "TokenLogprobs",
 ]

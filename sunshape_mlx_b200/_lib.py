@@ -95,6 +95,22 @@ class AppendArgs(C.Structure):
     ]
 
 
+class Int4AttnArgs(C.Structure):
+    """Mirror of ss_int4_attn_args."""
+
+    _fields_ = [
+        ("q", vp), ("dtype", i32), ("q_token_stride", i64), ("q_head_stride", i64),
+        ("n_tokens", i64), ("hq", i32), ("hkv", i32), ("d", i32),
+        ("pages", vp), ("n_pages", i32), ("page_stride", i64), ("head_stride", i64),
+        ("page_size", i32),
+        ("block_table", vp), ("table_stride", i64), ("width", i32),
+        ("seq_lens", vp), ("cu_q", vp), ("n_requests", i32), ("max_q", i32),
+        ("scale", f32), ("causal", i32), ("window", i32),
+        ("out", vp), ("lse", vp),
+        ("workspace", vp), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _SIGS = {
     "ss_abi_version": ([], i32),
     "ss_last_error": ([], C.c_char_p),
@@ -131,6 +147,14 @@ _SIGS = {
     "ss_set_assign_wait": ([i64, i64], i32),
     "ss_query_centroid_dots": ([vp, i64, i32, vp, i32, i32, vp, vp], i32),
     "ss_rotate_rows": ([vp, i64, i32, i64, vp, vp, i32, i64, vp], i32),
+    "ss_plan_step": ([vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, i64, vp, vp, vp, vp, vp, vp,
+                      vp, vp], i32),
+    "ss_release_pages": ([vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp], i32),
+    "ss_int4_append": ([vp, vp, i32, i64, i64, i64, i64, vp, i64, i32, i32, vp, i64, i64, i64,
+                        i32, vp], i32),
+    "ss_int4_fetch": ([vp, i64, i32, i32, vp, i64, i64, i64, i32, vp, vp, i32, vp], i32),
+    "ss_int4_attention": ([C.POINTER(Int4AttnArgs), vp], i32),
+    "ss_token_logprobs": ([vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp, vp], i32),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -229,6 +253,24 @@ def ptr(t: torch.Tensor | None):
 
 def stream_ptr(device: torch.device | None = None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+class _Here:
+    """A context that does nothing: the tensors are on the current device."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_CTX = _Here()
+
+
+def on_device(device: torch.device):
+    """Makes `device` current for a launch (free where it is already)."""
+    return _HERE_CTX if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -28,6 +28,16 @@ int* error_sink();
     if (!(cond)) return ::ss::fail(SS_ERR_BAD_ARG, (msg));     \
   } while (0)
 
+// Runs the body of a C entry point; no C++ exception leaves it.
+template <class F>
+int c_entry(F&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return SS_ERR_CUDA;
+  }
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // Creates (or returns a cached) 3-D tiled tensor map over fp16 data laid out

@@ -1,0 +1,277 @@
+// Writing rows into 4-bit KV pages by slot, and reading them back.
+//
+// A group of 32 dims of one token and head is stored as
+//   x' = clamp(x, +-2^15), lo = min x', hi = max x'
+//   s = fp16((hi - lo) / 15), z = fp16(lo)
+//   c = clamp(rint((x' - z) / s), 0, 15), 0 where s = 0;   value = c * s + z
+// (fp32 arithmetic, IEEE division, ties to even). A NaN makes its group's s
+// and z NaN, so readers see NaN for the group and nothing else.
+// Bound by HBM: a row is read once and 5 bits per value are written.
+#include "int4_pages.cuh"
+
+namespace ss {
+namespace {
+
+struct RowsParams {
+  const void *k, *v;   // append: inputs; fetch: unused
+  void *ko, *vo;       // fetch: outputs (N, H, D) contiguous
+  int dtype;
+  int64_t k_st, k_sh, v_st, v_sh;  // token and head strides of the inputs (elements)
+  const int64_t* slots;
+  int64_t n;
+  int h;
+  uint8_t* pages;
+  int64_t page_stride, head_stride;  // bytes
+  int page;
+  int64_t n_slots;
+};
+
+// 8 consecutive elements as fp32.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8]) {
+  if constexpr (DT == SS_F32) {
+    const float* p = reinterpret_cast<const float*>(base) + at;
+    if constexpr (VEC) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
+    uint32_t u[4];
+    if constexpr (VEC) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+      u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = DT == SS_F16 ? h2f(u[i] & 0xffff) : bf2f(u[i] & 0xffff);
+      x[2 * i + 1] = DT == SS_F16 ? h2f(u[i] >> 16) : bf2f(u[i] >> 16);
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void* base, int64_t at, const float (&x)[8]) {
+  if constexpr (DT == SS_F32) {
+    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + at);
+    p[0] = make_float4(x[0], x[1], x[2], x[3]);
+    p[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == SS_F16) {
+        u[i] = pack_h2(x[2 * i], x[2 * i + 1]);
+      } else {
+        __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        u[i] = *reinterpret_cast<uint32_t*>(&b);
+      }
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// The 4 lanes of a group hold 8 values each: this lane's code word and the group's (s, z).
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], uint32_t& sz) {
+  float lo = x[0], hi = x[0];
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    nan |= x[i] != x[i];
+    x[i] = fminf(fmaxf(x[i], -kInt4Max), kInt4Max);
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+  }
+  lo = fminf(fmaxf(lo, -kInt4Max), kInt4Max);
+  hi = fminf(fmaxf(hi, -kInt4Max), kInt4Max);
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+  }
+  const uint16_t sh = nan ? 0x7fff : f2h(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  const uint16_t zh = nan ? 0x7fff : f2h(lo);
+  sz = sh | (uint32_t)zh << 16;
+  const float s = h2f(sh), z = h2f(zh);
+  uint32_t w = 0;
+  if (s > 0.f) {  // false for NaN
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
+      w |= (uint32_t)c << (4 * i);
+    }
+  }
+  return w;
+}
+
+template <int D, int DT, bool VEC>
+__global__ void __launch_bounds__(256) append_kernel(RowsParams p) {
+  using B = Int4Blk<D>;
+  constexpr int X = D / 8;  // words of a row
+  const int64_t total = p.n * p.h * X;
+  for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t i = i0 + threadIdx.x;  // whole groups of 4 lanes are in or out: X is a multiple of 8
+    const bool in = i < total;
+    const int x = (int)(i % X);
+    const int64_t row = i / X;
+    const int64_t t = row / p.h;
+    const int hd = (int)(row - t * p.h);
+    const int64_t slot = in ? p.slots[t] : -1;
+    const bool live = slot >= 0 && slot < p.n_slots;
+    float a[8] = {}, b[8] = {};
+    if (live) {
+      load8<DT, VEC>(p.k, t * p.k_st + hd * p.k_sh + x * 8, a);
+      load8<DT, VEC>(p.v, t * p.v_st + hd * p.v_sh + x * 8, b);
+    }
+    uint32_t ksz, vsz;
+    const uint32_t kw = quantise8(a, ksz), vw = quantise8(b, vsz);
+    if (!live) continue;
+    const int64_t page = slot / p.page;
+    const int in_page = (int)(slot - page * p.page);
+    uint8_t* blk = p.pages + page * p.page_stride + hd * p.head_stride + (int64_t)(in_page >> 4) * B::kBytes;
+    const int tok = in_page & 15;
+    *reinterpret_cast<uint32_t*>(blk + B::key_word(tok, x >> 2, x & 3)) = kw;
+    *reinterpret_cast<uint32_t*>(blk + B::value_word(tok, x)) = vw;
+    if ((x & 3) == 0) {
+      *reinterpret_cast<uint32_t*>(blk + B::key_sz(tok, x >> 2)) = ksz;
+      *reinterpret_cast<uint32_t*>(blk + B::value_sz(tok, x >> 2)) = vsz;
+    }
+  }
+}
+
+__device__ __forceinline__ void dequant8(uint32_t w, uint32_t sz, float (&x)[8]) {
+  const float s = h2f(sz & 0xffff), z = h2f(sz >> 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15), s, z);
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(256) fetch_kernel(RowsParams p) {
+  using B = Int4Blk<D>;
+  constexpr int X = D / 8;
+  const int64_t total = p.n * p.h * X;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int x = (int)(i % X);
+    const int64_t row = i / X;
+    const int64_t t = row / p.h;
+    const int hd = (int)(row - t * p.h);
+    const int64_t slot = p.slots[t];
+    float a[8] = {}, b[8] = {};
+    if (slot >= 0 && slot < p.n_slots) {
+      const int64_t page = slot / p.page;
+      const int in_page = (int)(slot - page * p.page);
+      const uint8_t* blk = p.pages + page * p.page_stride + hd * p.head_stride + (int64_t)(in_page >> 4) * B::kBytes;
+      const int tok = in_page & 15;
+      dequant8(*reinterpret_cast<const uint32_t*>(blk + B::key_word(tok, x >> 2, x & 3)),
+               *reinterpret_cast<const uint32_t*>(blk + B::key_sz(tok, x >> 2)), a);
+      dequant8(*reinterpret_cast<const uint32_t*>(blk + B::value_word(tok, x)),
+               *reinterpret_cast<const uint32_t*>(blk + B::value_sz(tok, x >> 2)), b);
+    }
+    store8<DT>(p.ko, i * 8, a);
+    store8<DT>(p.vo, i * 8, b);
+  }
+}
+
+int rows_grid(int64_t total) {
+  const int64_t want = (total + 255) / 256, cap = 8LL * sm_count();
+  return (int)(want < cap ? want : cap);
+}
+
+template <int D>
+int launch_append(const RowsParams& p, bool vec, cudaStream_t st) {
+  const int g = rows_grid(p.n * p.h * (D / 8));
+#define SS_APPEND(DT)                                                     \
+  if (vec) append_kernel<D, DT, true><<<g, 256, 0, st>>>(p);              \
+  else append_kernel<D, DT, false><<<g, 256, 0, st>>>(p)
+  if (p.dtype == SS_F32) { SS_APPEND(SS_F32); }
+  else if (p.dtype == SS_F16) { SS_APPEND(SS_F16); }
+  else { SS_APPEND(SS_BF16); }
+#undef SS_APPEND
+  return check_launch("ss_int4_append");
+}
+
+template <int D>
+int launch_fetch(const RowsParams& p, cudaStream_t st) {
+  const int g = rows_grid(p.n * p.h * (D / 8));
+  if (p.dtype == SS_F32) fetch_kernel<D, SS_F32><<<g, 256, 0, st>>>(p);
+  else if (p.dtype == SS_F16) fetch_kernel<D, SS_F16><<<g, 256, 0, st>>>(p);
+  else fetch_kernel<D, SS_BF16><<<g, 256, 0, st>>>(p);
+  return check_launch("ss_int4_fetch");
+}
+
+int check_pool(const void* pages, int64_t n_pages, int64_t page_stride, int64_t head_stride, int h,
+               int page_size, int d) {
+  SS_REQUIRE(pages, "int4 pages: null pointer");
+  SS_REQUIRE(int4_head_dim_ok(d), "int4 pages: head_dim must be 64, 128 or 256");
+  SS_REQUIRE(page_size >= 16 && page_size % 16 == 0, "int4 pages: page_size must be a multiple of 16");
+  SS_REQUIRE(n_pages >= 1 && h >= 1, "int4 pages: empty pool");
+  SS_REQUIRE(((reinterpret_cast<uintptr_t>(pages) | (uintptr_t)page_stride | (uintptr_t)head_stride) & 15) == 0,
+             "int4 pages: the pool and its strides must be multiples of 16 bytes");
+  return SS_OK;
+}
+
+}  // namespace
+}  // namespace ss
+
+using namespace ss;
+
+extern "C" {
+
+int ss_int4_append(const void* k, const void* v, int dtype, int64_t k_token_stride,
+                   int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                   const int64_t* slots, int64_t n, int n_heads, int d, void* pages,
+                   int64_t n_pages, int64_t page_stride, int64_t head_stride, int page_size,
+                   void* stream) {
+  return c_entry([&]() -> int {
+    if (n == 0) return SS_OK;
+    SS_REQUIRE(k && v && slots && n > 0, "ss_int4_append: null pointer or negative count");
+    SS_REQUIRE(dtype >= SS_F32 && dtype <= SS_BF16, "ss_int4_append: bad dtype");
+    if (int rc = check_pool(pages, n_pages, page_stride, head_stride, n_heads, page_size, d)) return rc;
+    count_dispatch("ss_int4_append");
+    RowsParams p{};
+    p.k = k; p.v = v; p.dtype = dtype;
+    p.k_st = k_token_stride; p.k_sh = k_head_stride; p.v_st = v_token_stride; p.v_sh = v_head_stride;
+    p.slots = slots; p.n = n; p.h = n_heads;
+    p.pages = static_cast<uint8_t*>(pages);
+    p.page_stride = page_stride; p.head_stride = head_stride; p.page = page_size;
+    p.n_slots = n_pages * page_size;
+    const int es = dtype == SS_F32 ? 4 : 2;
+    const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                       (uintptr_t)((k_token_stride | k_head_stride | v_token_stride | v_head_stride) * es)) & 15) == 0;
+    cudaStream_t st = as_stream(stream);
+    return d == 64 ? launch_append<64>(p, vec, st) : d == 128 ? launch_append<128>(p, vec, st)
+                                                              : launch_append<256>(p, vec, st);
+  });
+}
+
+int ss_int4_fetch(const int64_t* slots, int64_t n, int n_heads, int d, const void* pages,
+                  int64_t n_pages, int64_t page_stride, int64_t head_stride, int page_size,
+                  void* k_out, void* v_out, int dtype, void* stream) {
+  return c_entry([&]() -> int {
+    if (n == 0) return SS_OK;
+    SS_REQUIRE(k_out && v_out && slots && n > 0, "ss_int4_fetch: null pointer or negative count");
+    SS_REQUIRE(dtype >= SS_F32 && dtype <= SS_BF16, "ss_int4_fetch: bad dtype");
+    SS_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0,
+               "ss_int4_fetch: outputs must be 16-byte aligned");
+    if (int rc = check_pool(pages, n_pages, page_stride, head_stride, n_heads, page_size, d)) return rc;
+    count_dispatch("ss_int4_fetch");
+    RowsParams p{};
+    p.ko = k_out; p.vo = v_out; p.dtype = dtype;
+    p.slots = slots; p.n = n; p.h = n_heads;
+    p.pages = static_cast<uint8_t*>(const_cast<void*>(pages));
+    p.page_stride = page_stride; p.head_stride = head_stride; p.page = page_size;
+    p.n_slots = n_pages * page_size;
+    cudaStream_t st = as_stream(stream);
+    return d == 64 ? launch_fetch<64>(p, st) : d == 128 ? launch_fetch<128>(p, st) : launch_fetch<256>(p, st);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,57 @@
+"""Log probabilities of given tokens, with entropy and top alternatives: what
+a server returns beside its tokens, and what compressed caches are compared
+with uncompressed ones by."""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+
+__all__ = ["TokenLogprobs", "token_logprobs"]
+
+_MAX_TOP = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """logprobs, entropy (rows,) fp32; top_ids (rows, top_k) int32 and
+    top_logprobs (rows, top_k) fp32."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0) -> TokenLogprobs:
+    """Natural log probabilities under softmax(logits).
+
+    logits (rows, vocab) fp32, fp16 or bf16, contiguous in vocab; targets
+    (rows,) int64: a negative one (padding) gives 0, one past the vocabulary
+    NaN. ``top_k`` <= 32 alternatives by value, equal ones by index; -1 and
+    -inf past the vocabulary. Logits of -inf are impossible tokens; a row of
+    nothing else gives -inf and entropy 0. A row with NaN or +inf gives NaN
+    everywhere and ids of -1.
+    """
+    L.require_cuda(logits, targets)
+    if logits.dim() != 2 or not logits.shape[1]:
+        raise ValueError("logits must be (rows, vocab)")
+    n, vocab = logits.shape
+    if logits.stride(1) != 1 and vocab > 1:
+        raise ValueError("logits must be contiguous in vocab")
+    dev = logits.device
+    if targets.dtype != torch.int64 or targets.shape != (n,) or targets.device != dev or not targets.is_contiguous():
+        raise ValueError("targets must be a contiguous int64 tensor with one element per row, on the logits' device")
+    if not 0 <= top_k <= _MAX_TOP:
+        raise ValueError(f"top_k must be in [0, {_MAX_TOP}], got {top_k}")
+    dt = L.dtype_code(logits.dtype)
+    out = torch.empty((2 + top_k) * n, dtype=torch.float32, device=dev)
+    lp, ent, top = out.split((n, n, top_k * n))
+    ids = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+    with L.on_device(dev):
+        L.call("ss_token_logprobs", logits.data_ptr(), dt, n, logits.stride(0), vocab,
+               targets.data_ptr(), top_k, lp.data_ptr(), ent.data_ptr(), ids.data_ptr(),
+               top.data_ptr(), L.stream_ptr(dev))
+    return TokenLogprobs(lp, ent, ids, top.view(n, top_k))
