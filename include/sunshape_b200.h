@@ -450,10 +450,14 @@ typedef struct ss_int4_attn_args {
   int causal, window;
   void* out;                      /* (n_tokens, hq, d) dense, 16-byte aligned */
   float* lse;                     /* (n_tokens, hq) natural logarithm, or NULL */
-  void* workspace;
+  void* workspace;                /* ss_int4_attention_workspace(d) bytes, zeroed once */
   size_t workspace_bytes;
 } ss_int4_attn_args;
 
+/* Bytes of scratch on the current device. The caller zeroes it once and keeps
+ * it: every launch leaves its counters at zero. Launches that may overlap on
+ * the GPU must not share it. */
+size_t ss_int4_attention_workspace(int d);
 int ss_int4_attention(const ss_int4_attn_args* a, void* stream);
 
 /* Log probability of targets[r] (int64; < 0: 0, >= vocab: NaN; NULL: all 0),

@@ -153,6 +153,7 @@ _SIGS = {
     "ss_int4_append": ([vp, vp, i32, i64, i64, i64, i64, vp, i64, i32, i32, vp, i64, i64, i64,
                         i32, vp], i32),
     "ss_int4_fetch": ([vp, i64, i32, i32, vp, i64, i64, i64, i32, vp, vp, i32, vp], i32),
+    "ss_int4_attention_workspace": ([i32], C.c_size_t),
     "ss_int4_attention": ([C.POINTER(Int4AttnArgs), vp], i32),
     "ss_token_logprobs": ([vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp, vp], i32),
 }

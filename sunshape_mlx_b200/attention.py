@@ -24,11 +24,12 @@ __all__ = ["sunshape_sdpa", "decode_partials", "workspace_for", "PreparedDecode"
 _WS: dict[tuple, torch.Tensor] = {}
 
 
-def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Zero-initialised decode workspace, one per (device, stream), grown on
-    demand. The kernel leaves its arrival counters at zero on exit, so the
-    buffer is reused without clearing; calls sharing it are stream-ordered."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+def workspace_for(device: torch.device, nbytes: int, kind: str = "decode") -> torch.Tensor:
+    """Zero-initialised workspace, one per (device, stream, kind of kernel),
+    grown on demand. The kernels leave their arrival counters at zero on exit,
+    so the buffer is reused without clearing; calls sharing it are
+    stream-ordered."""
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream, kind)
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)

@@ -6,7 +6,33 @@
 //   out = sum p_t v_t / sum p_t,   lse = max z + ln sum p_t;
 // a row that sees no key gives out = 0, lse = -inf.
 //
-// One warp per (query token, query head), one key at a time, in fp32.
+// Split. A unit is (request, kv-head, up to R query rows): the rows share its
+// keys, so a block is read once for all of them. The blocks of all units in a
+// row are cut into ranges of equal cost, one per CTA (persistent, one CTA per
+// SM); a unit cut by a range boundary leaves partial (o, m, l) rows in the
+// workspace and the last CTA to arrive joins them in the order of the ranges,
+// so results do not depend on timing. Lengths are read on the GPU: nothing
+// waits for the host.
+//
+// One warp takes a 16-token block at a time, with its own ring of cp.async
+// copies (20 D contiguous bytes a block) and its own softmax state; the warps
+// meet at the end of a unit only.
+//   S^T (16 tokens x 8 rows) by warp MMAs. With code c, scale s and zero z of
+//   a (token, group): q . k = sum_g s_g (sum_d q_d c_d) + sum_g z_g (sum_d q_d).
+//   The codes enter the MMA as 64 + c (a nibble ORed into the bits of 64.0 is
+//   exactly 64 + c), the accumulators start at -64 sum_d q_d, and s_g is
+//   applied to the fp32 result, so keys are never rounded. The zeros take one
+//   MMA more, with the row's group sums split into two fp16 terms.
+//   Queries enter as fp16 after a power of two per row that puts the row's
+//   largest magnitude in [128, 256): exact for fp16 and bf16 down to 2^-31 of
+//   that magnitude.
+//   O^T (D x 8 rows) += V^T P^T: two tokens' words are interleaved by byte
+//   permutes so that a register holds a dim of two tokens; v = fp16(c s + z),
+//   the one rounding of the values. Probabilities are fp16 pairs hi + lo
+//   where the output is fp16 (their rounding would otherwise be as large as
+//   the output's); for up to 4 rows lo uses the columns that are free anyway.
+// The softmax reference of a row moves only when a logit exceeds it by 2^8:
+// the usual block needs one vote and no shuffles.
 #include "int4_pages.cuh"
 
 namespace ss {
@@ -17,7 +43,7 @@ struct AttnParams {
   int dtype;
   int64_t q_st, q_sh;
   int64_t n_tokens;
-  int hq, hkv;
+  int hq, hkv, grp;
   const uint8_t* pages;
   int n_pages;
   int64_t page_stride, head_stride;
@@ -31,56 +57,675 @@ struct AttnParams {
   int causal, window;
   void* out;
   float* lse;
+  uint8_t* ws;
+  int n_slots;  // CTAs the workspace was sized for
 };
 
-template <int D>
-__global__ void __launch_bounds__(256) attn_rows_kernel(AttnParams p) {
-  using B = Int4Blk<D>;
-  constexpr int E = D / 32;  // dims of a lane: lane * E ..
-  const int lane = threadIdx.x & 31;
-  const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (row >= p.n_tokens * p.hq) return;
-  const int64_t t = row / p.hq;
-  const int hq = (int)(row - t * p.hq), h = hq / (p.hq / p.hkv);
-  float o[E] = {}, m = -INFINITY, l = 0.f;
-  int lo = 0, hi = p.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid] <= t) lo = mid; else hi = mid;
-  }
-  if (t >= p.cu_q[lo] && t < p.cu_q[lo + 1]) {
-    const int len = min(max(p.seq_lens[lo], 0), p.width * p.page);
-    const int pos = len - (p.cu_q[lo + 1] - p.cu_q[lo]) + (int)(t - p.cu_q[lo]);
-    float q[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = load_as_f32(p.q, p.dtype, t * p.q_st + hq * p.q_sh + lane * E + e) * p.scale;
-    const int last = p.causal ? min(len - 1, pos) : len - 1;
-    const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-    const int x = lane * E / 8, g = lane * E / 32, n0 = lane * E % 8;
-    for (int k = first; k <= last; ++k) {
-      const int page = p.table[lo * p.table_stride + k / p.page];
-      if (page < 0 || page >= p.n_pages) continue;
-      const int in_page = k % p.page, tok = in_page & 15;
-      const uint8_t* blk = p.pages + page * p.page_stride + h * p.head_stride + (int64_t)(in_page >> 4) * B::kBytes;
-      const uint32_t kw = *reinterpret_cast<const uint32_t*>(blk + B::key_word(tok, x >> 2, x & 3));
-      const uint32_t ks = *reinterpret_cast<const uint32_t*>(blk + B::key_sz(tok, g));
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(blk + B::value_word(tok, x));
-      const uint32_t vs = *reinterpret_cast<const uint32_t*>(blk + B::value_sz(tok, g));
-      float z = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) z += q[e] * fmaf((float)((kw >> (4 * (n0 + e))) & 15), h2f(ks & 0xffff), h2f(ks >> 16));
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
-      const float mn = fmaxf(m, z), a = m == mn ? 1.f : expf(m - mn), w = z == mn ? 1.f : expf(z - mn);
-      m = mn;
-      l = l * a + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * fmaf((float)((vw >> (4 * (n0 + e))) & 15), h2f(vs & 0xffff), h2f(vs >> 16));
+constexpr int kSegCost = 24;     // blocks' worth of time that the ends of a unit take
+constexpr int kMinCost = 96;     // a range is not cut below this many blocks' worth
+constexpr float kLow = -1e30f;   // softmax reference before any key
+constexpr float kSlack = 8.f;    // a logit may exceed the reference by this (base 2)
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Modes: query rows of a unit, and whether probabilities are hi + lo.
+enum { kRows4, kRows8, kRows8Lo, kRows16, kRows16Lo };
+__host__ __device__ constexpr int mode_rows(int m) { return m == kRows4 ? 4 : m <= kRows8Lo ? 8 : 16; }
+
+template <int D, int MODE>
+struct Shape {
+  static constexpr int R = mode_rows(MODE);
+  static constexpr int NR = R == 16 ? 2 : 1;       // 8-column tiles
+  static constexpr bool LO = MODE == kRows8Lo || MODE == kRows16Lo;  // a second MMA for lo
+  static constexpr int W = D == 256 || NR == 2 ? 8 : 12;  // warps
+  static constexpr int S = D == 256 ? 3 : 4;       // ring stages of a warp
+  static constexpr int kRing = W * S * Int4Blk<D>::kBytes;
+  static constexpr int kMerge = W * R * (D + 4) * 4;  // rows padded by 4 floats
+  static constexpr int kSmem = kRing + kMerge + (2 * W * R + 3 * R) * 4 + (W * 32 + 2) * 8;
+};
+
+// What a request contributes to the schedule.
+struct Req {
+  int nq, len, rbs, blk0, nblk;  // query rows' tokens, keys, row blocks, first key block, key blocks (>= 1)
+};
+
+template <int R>
+__device__ __forceinline__ Req load_req(const AttnParams& p, int b) {
+  Req r;
+  const int c0 = max(p.cu_q[b], 0);
+  r.nq = max(p.cu_q[b + 1] - c0, 0);
+  r.len = min(max(p.seq_lens[b], 0), p.width * p.page);
+  r.rbs = (int)(((int64_t)r.nq * p.grp + R - 1) / R);
+  r.blk0 = p.window > 0 ? max(0, r.len - r.nq - p.window + 1) / kBlkTokens : 0;
+  r.nblk = max(1, (r.len + kBlkTokens - 1) / kBlkTokens - r.blk0);
+  return r;
+}
+
+// One CTA's walk over its range: unit after unit.
+template <int R>
+struct Walk {
+  int b = 0, h = 0, rb = 0;  // unit
+  int64_t at = 0;            // cost position of the unit's start
+  Req r{};
+
+  __device__ __forceinline__ int64_t cost() const { return r.nblk + kSegCost; }
+  __device__ void skip_empty(const AttnParams& p) {
+    while (b < p.n) {
+      r = load_req<R>(p, b);
+      if (r.rbs > 0) break;
+      ++b;
     }
   }
+  __device__ void next(const AttnParams& p) {
+    at += cost();
+    if (++rb < r.rbs) return;
+    rb = 0;
+    if (++h < p.hkv) return;
+    h = 0;
+    ++b;
+    skip_empty(p);
+  }
+};
+
+__device__ __forceinline__ uint32_t lop_or(uint32_t x, uint32_t mask, uint32_t magic) {
+  uint32_t r;  // (x & mask) | magic
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(magic));
+  return r;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float lo_h(uint32_t x) { return __low2float(*reinterpret_cast<__half2*>(&x)); }
+__device__ __forceinline__ float hi_h(uint32_t x) { return __high2float(*reinterpret_cast<__half2*>(&x)); }
+
+template <int N>
+__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&v)[N]) {
+  if constexpr (N == 2) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    v[0] = a.x; v[1] = a.y;
+  } else {
 #pragma unroll
-  for (int e = 0; e < E; ++e) store_from_f32(p.out, p.dtype, row * D + lane * E + e, l == 0.f ? 0.f : o[e] / l);
-  if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : m + logf(l);
+    for (int i = 0; i < N; i += 4) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p + 4 * i);
+      v[i] = a.x; v[i + 1] = a.y; v[i + 2] = a.z; v[i + 3] = a.w;
+    }
+  }
+}
+
+template <int D, int MODE>
+__global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(const __grid_constant__ AttnParams p) {
+  using B = Int4Blk<D>;
+  using Sh = Shape<D, MODE>;
+  constexpr int R = Sh::R, NR = Sh::NR, W = Sh::W, S = Sh::S, G = B::G, N = B::N, T = W * 32;
+  constexpr int MT = D / 16;  // 16-dim tiles of O
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem + Sh::kRing);            // [W][R][D + 4]
+  float* s_m = s_o + W * R * (D + 4);                                 // [W][R]
+  float* s_l = s_m + W * R;                                           // [W][R]
+  float* s_rm = s_l + W * R;                                          // [R] joined reference
+  float* s_rl = s_rm + R;                                             // [R] joined sum
+  float* s_flag = s_rl + R;                                           // [R] (only [0]: last to arrive)
+  int64_t* s_cum = reinterpret_cast<int64_t*>(s_flag + R);            // [T] + 2
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gi = lane >> 2, gj = lane & 3;
+  uint8_t* ring = smem + warp * S * B::kBytes;
+
+  // tokens outside cu_q: zero rows
+  {
+    const int64_t first = min((int64_t)max(p.cu_q[0], 0), p.n_tokens), last = min((int64_t)max(p.cu_q[p.n], 0), p.n_tokens);
+    const int64_t none = first + p.n_tokens - last, row = (int64_t)p.hq * D / 8;
+    for (int64_t i = (int64_t)blockIdx.x * T + tid; i < none * row; i += (int64_t)gridDim.x * T) {
+      int64_t t = i / row;
+      t = t < first ? t : last + t - first;
+      reinterpret_cast<uint4*>(p.out)[t * row + i % row] = make_uint4(0, 0, 0, 0);
+      if (p.lse && i % row < p.hq) p.lse[t * p.hq + i % row] = -INFINITY;
+    }
+  }
+
+  // ---- schedule: costs of the requests, thread by thread, then a scan -------
+  const int per = (p.n + T - 1) / T;
+  const int rb0 = min(p.n, tid * per), rb1 = min(p.n, rb0 + per);
+  int64_t cost = 0, units = 0;
+  for (int b = rb0; b < rb1; ++b) {
+    const Req r = load_req<R>(p, b);
+    cost += (int64_t)r.rbs * p.hkv * (r.nblk + kSegCost);
+    units += (int64_t)r.rbs * p.hkv;
+  }
+  int64_t inc = cost;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+    units += __shfl_xor_sync(0xffffffffu, units, o);
+  }
+  int64_t* s_w = reinterpret_cast<int64_t*>(s_o);  // [W] costs, [W] units
+  if (lane == 31) s_w[warp] = inc;
+  if (lane == 0) s_w[W + warp] = units;
+  __syncthreads();
+  int64_t total = 0, before = 0;
+  units = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w == warp) before = total;
+    total += s_w[w];
+    units += s_w[W + w];
+  }
+  s_cum[tid] = before + inc - cost;  // cost of the requests before this thread's
+  __syncthreads();
+  // as many ranges as SMs, but none smaller than a unit or kMinCost
+  int64_t want = (total + kMinCost + kSegCost - 1) / (kMinCost + kSegCost);
+  want = want < units ? units : want;
+  const int nc = (int)(want < gridDim.x ? want : (int64_t)gridDim.x);
+  if ((int)blockIdx.x >= nc) return;
+  auto range_start = [&](int64_t i) { return i * total / nc; };
+  auto cta_of = [&](int64_t c) { return (int)(((c + 1) * nc - 1) / total); };  // the range that holds c
+  const int64_t lo = range_start(blockIdx.x), hi = range_start(blockIdx.x + 1);
+
+  Walk<R> walk;
+  {
+    int a = 0, e = T;  // the last thread whose requests start at or before lo
+    while (e - a > 1) {
+      const int mid = (a + e) >> 1;
+      if (s_cum[mid] <= lo) a = mid; else e = mid;
+    }
+    walk.b = min(p.n, a * per);
+    walk.at = s_cum[a];
+    walk.skip_empty(p);
+    for (;;) {
+      const int64_t one = walk.cost(), all = one * walk.r.rbs * p.hkv;
+      if (walk.at + all > lo) {
+        const int64_t u = (lo - walk.at) / one;
+        walk.h = (int)(u / walk.r.rbs);
+        walk.rb = (int)(u - (int64_t)walk.h * walk.r.rbs);
+        walk.at += u * one;
+        break;
+      }
+      walk.at += all;
+      ++walk.b;
+      walk.skip_empty(p);
+    }
+  }
+
+  // key blocks [k0, k1) of the walk's unit that this CTA's range covers
+  auto blocks = [&](const Walk<R>& w, int& k0, int& k1) {
+    const int64_t body = w.at + kSegCost;
+    const int64_t a = (lo > body ? lo : body) - body, e = (hi < body + w.r.nblk ? hi : body + w.r.nblk) - body;
+    k0 = w.r.blk0 + (int)a;
+    k1 = e > a ? w.r.blk0 + (int)e : k0;
+    if (p.causal) {  // nothing after the last row of the unit
+      const int last_row = (int)min((int64_t)w.r.nq * p.grp, (int64_t)(w.rb + 1) * R) - 1;
+      const int end = min(w.r.len, w.r.len - w.r.nq + last_row / p.grp + 1);
+      k1 = max(k0, min(k1, (max(end, 0) + kBlkTokens - 1) / kBlkTokens));
+    }
+    if (w.r.len == 0) k1 = k0;
+    return e > a;  // this CTA takes part in the unit
+  };
+
+  // ---- copies: this warp's blocks in the order it will use them -------------
+  Walk<R> pw = walk;
+  int pk = 0, pk1 = 0, pid = 0, pn = 0;
+  bool more = true, fresh = true;
+  auto issue = [&](int stage) {
+    while (more && (fresh || pk >= pk1)) {
+      if (!fresh) pw.next(p);
+      fresh = false;
+      if (pw.b >= p.n || pw.at >= hi) { more = false; break; }
+      blocks(pw, pk, pk1);
+      pk += warp;
+      pn = 32;
+    }
+    if (more) {
+      if (pn == 32) {  // page ids of the next 32 blocks, one a lane
+        const int k = pk + lane * W;
+        pid = k < pk1 ? p.table[pw.b * p.table_stride + (int64_t)k * kBlkTokens / p.page] : -1;
+        pn = 0;
+      }
+      const int id = __shfl_sync(0xffffffffu, pid, pn++);
+      const bool ok = id >= 0 && id < p.n_pages;
+      const uint8_t* src = p.pages;
+      if (ok) src += id * p.page_stride + pw.h * p.head_stride + (int64_t)((int64_t)pk * kBlkTokens % p.page / kBlkTokens) * B::kBytes;
+      const uint32_t dst = smem_u32(ring + stage * B::kBytes);
+#pragma unroll
+      for (int i = lane; i < B::kBytes / 16; i += 32) cp_async16(dst + i * 16, src + (ok ? i * 16 : 0), ok ? 16 : 0);
+      pk += W;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue(s);
+  int stage = 0;
+
+  // ---- unit after unit --------------------------------------------------------
+  for (; walk.b < p.n && walk.at < hi; walk.next(p)) {
+    int k0, k1;
+    const bool part = blocks(walk, k0, k1);
+    const Req r = walk.r;
+    const int b = walk.b, tok0 = max(p.cu_q[b], 0);
+    const int row0 = walk.rb * R, rows = min(R, (int)((int64_t)r.nq * p.grp - row0));
+    if (!part) continue;  // uniform over the CTA: the range ends inside the unit's fixed cost
+
+    // queries as B fragments: lane (i, j) holds dims 32 g + 8 j .. + 7 of row i
+    uint32_t qf[NR][G][4];
+    float bias[NR][G][2], fac[NR][2];
+    uint32_t qz[NR][2];
+    int kend[NR][2], kbeg[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int col = nr * 8 + gi, row = MODE == kRows4 ? (col & 3) : col;
+      float x[G][8], big = 0.f;
+      const int tt = (row0 + row) / p.grp, hd = walk.h * p.grp + (row0 + row) % p.grp;
+      const bool live = row < rows && tok0 + (int64_t)tt < p.n_tokens;
+      const int64_t at = (tok0 + (int64_t)tt) * p.q_st + hd * p.q_sh + gj * 8;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[g][e] = live ? load_as_f32(p.q, p.dtype, at + g * 32 + e) : 0.f;
+          big = fmaxf(big, fabsf(x[g][e]));
+        }
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // 2^e with big * 2^e in [128, 256); 1 for rows of zeros or infinities
+      int ex = 0;
+      if (big > 0.f && big < INFINITY) ex = 134 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
+      const float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
+      float sum[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        sum[g] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // a register: dims e and e + 4, as the key words' nibbles come
+          qf[nr][g][e] = pack_h2(x[g][e] * up, x[g][e + 4] * up);
+          sum[g] += lo_h(qf[nr][g][e]) + hi_h(qf[nr][g][e]);
+        }
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+      }
+      // group sums as the B fragment of the zeros' MMA: k = group hi, k + 8 = group lo
+      float z0 = 0.f, z1 = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; g += 2) {
+        if (gj == g / 2) { z0 = sum[g]; z1 = sum[g + 1]; }
+      }
+      qz[nr][0] = pack_h2(z0, z1);
+      qz[nr][1] = pack_h2(z0 - lo_h(qz[nr][0]), z1 - hi_h(qz[nr][0]));
+      const float back = p.scale * kLog2e / up;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // the columns of this lane's accumulators
+        const int cc = 2 * gj + c, from = cc * 4;
+        fac[nr][c] = __shfl_sync(0xffffffffu, back, from);
+#pragma unroll
+        for (int g = 0; g < G; ++g) bias[nr][g][c] = -64.f * __shfl_sync(0xffffffffu, sum[g], from);
+        const int rr = MODE == kRows4 ? (cc & 3) : nr * 8 + cc;
+        const int pos = r.len - r.nq + (row0 + rr) / p.grp;
+        kend[nr][c] = rr >= rows ? 0 : p.causal ? min(r.len, pos + 1) : r.len;
+        kbeg[nr][c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      }
+    }
+    // blocks in [all0, all1) are seen whole by every row of the unit
+    int all0 = 0, all1 = 0x7fffffff;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int rr = MODE == kRows4 ? ((2 * gj + c) & 3) : nr * 8 + 2 * gj + c;
+        if (rr < rows) {
+          all0 = max(all0, kbeg[nr][c]);
+          all1 = min(all1, kend[nr][c]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      all0 = max(all0, __shfl_xor_sync(0xffffffffu, all0, o));
+      all1 = min(all1, __shfl_xor_sync(0xffffffffu, all1, o));
+    }
+
+    float o[NR][MT][4], m[NR][2], l[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nr][t][e] = 0.f;
+      }
+      m[nr][0] = m[nr][1] = kLow;
+      l[nr][0] = l[nr][1] = 0.f;
+    }
+
+    // page ids of this warp's blocks, to hide keys of table entries outside the pool
+    int cid = 0, cn = 32;
+    for (int k = k0 + warp; k < k1; k += W) {
+      if (cn == 32) {
+        const int kk = k + lane * W;
+        cid = kk < k1 ? p.table[b * p.table_stride + (int64_t)kk * kBlkTokens / p.page] : 0;
+        cn = 0;
+      }
+      const int id = __shfl_sync(0xffffffffu, cid, cn++);
+      const bool there = id >= 0 && id < p.n_pages;
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+      __syncwarp();
+      issue(stage == 0 ? S - 1 : stage - 1);
+      const uint8_t* blk = ring + stage * B::kBytes;
+      stage = stage == S - 1 ? 0 : stage + 1;
+      const int t0 = k * kBlkTokens;
+
+      // ---- logits: S^T = K Q^T ----
+      float s[NR][4];
+      {
+        uint32_t z[4] = {0u, 0u, 0u, 0u};  // zeros of tokens i, i + 8: groups 2j, 2j + 1
+        if (2 * gj < G) {
+          uint32_t a[2], c[2];
+          lds(blk + B::key_sz(gi, 2 * gj), a);
+          lds(blk + B::key_sz(gi + 8, 2 * gj), c);
+          z[0] = z[2] = __byte_perm(a[0], a[1], 0x7632);
+          z[1] = z[3] = __byte_perm(c[0], c[1], 0x7632);
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+          s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.f;
+          mma_16816(s[nr], z[0], z[1], z[2], z[3], qz[nr][0], qz[nr][1]);
+        }
+#pragma unroll
+        for (int c = 0; c < G / N; ++c) {
+          uint32_t w0[N], w1[N], z0[N], z1[N];
+          lds(blk + B::key_word(gi, c * N, gj), w0);
+          lds(blk + B::key_word(gi + 8, c * N, gj), w1);
+          lds(blk + B::key_sz(gi, c * N), z0);
+          lds(blk + B::key_sz(gi + 8, c * N), z1);
+#pragma unroll
+          for (int g = 0; g < N; ++g) {
+            uint32_t h0[4], h1[4];  // 64 + code of dims (e, e + 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x0 = e == 0 ? w0[g] << 4 : w0[g] >> (4 * (e - 1)), x1 = e == 0 ? w1[g] << 4 : w1[g] >> (4 * (e - 1));
+              h0[e] = lop_or(x0, 0x00f000f0u, 0x54005400u);
+              h1[e] = lop_or(x1, 0x00f000f0u, 0x54005400u);
+            }
+            const float s0 = lo_h(z0[g]), s1 = lo_h(z1[g]);
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+              float a[4] = {bias[nr][c * N + g][0], bias[nr][c * N + g][1], bias[nr][c * N + g][0], bias[nr][c * N + g][1]};
+              mma_16816(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
+              mma_16816(a, h0[2], h1[2], h0[3], h1[3], qf[nr][c * N + g][2], qf[nr][c * N + g][3]);
+              s[nr][0] = fmaf(s0, a[0], s[nr][0]);
+              s[nr][1] = fmaf(s0, a[1], s[nr][1]);
+              s[nr][2] = fmaf(s1, a[2], s[nr][2]);
+              s[nr][3] = fmaf(s1, a[3], s[nr][3]);
+            }
+          }
+        }
+      }
+
+      // ---- probabilities ----
+      const bool edge = !there || t0 < all0 || t0 + kBlkTokens > all1;
+      uint32_t ph[NR][2], pl[NR][2];
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = s[nr][e] * fac[nr][e & 1];
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + gi + (e >> 1) * 8;
+            if (!there || t >= kend[nr][e & 1] || t < kbeg[nr][e & 1]) y[e] = -INFINITY;
+          }
+        }
+        const bool over = fmaxf(y[0], y[2]) > m[nr][0] + kSlack || fmaxf(y[1], y[3]) > m[nr][1] + kSlack;
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(y[c], y[c + 2]);
+#pragma unroll
+            for (int sft = 4; sft < 32; sft <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sft));
+            const float mn = fmaxf(m[nr][c], top), f = ex2(m[nr][c] - mn);
+            m[nr][c] = mn;
+            l[nr][c] *= f;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              o[nr][t][c] *= f;
+              o[nr][t][c + 2] *= f;
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e] - m[nr][e & 1]);
+        l[nr][0] += y[0] + y[2];
+        l[nr][1] += y[1] + y[3];
+        uint32_t a = pack_h2(y[0], y[1]), c = pack_h2(y[2], y[3]);
+        if constexpr (MODE == kRows4) {  // columns 4-7 repeat rows 0-3: they take lo
+          const uint32_t al = pack_h2(y[0] - lo_h(a), y[1] - hi_h(a)), cl = pack_h2(y[2] - lo_h(c), y[3] - hi_h(c));
+          a = gj < 2 ? a : al;
+          c = gj < 2 ? c : cl;
+        }
+        ph[nr][0] = transpose8x8(a);
+        ph[nr][1] = transpose8x8(c);
+        if constexpr (Sh::LO) {
+          pl[nr][0] = transpose8x8(pack_h2(y[0] - lo_h(a), y[1] - hi_h(a)));
+          pl[nr][1] = transpose8x8(pack_h2(y[2] - lo_h(c), y[3] - hi_h(c)));
+        }
+      }
+
+      // ---- O^T += V^T P^T ----
+      {
+        uint32_t vz[4], vw[4 * B::W];
+        lds(blk + B::value_sz(2 * gj, gi * B::W / 4), vz);
+#pragma unroll
+        for (int c = 0; c < B::W; ++c) {
+          uint32_t t4[4];
+          lds(blk + B::kV + c * 512 + lane * 16, t4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vw[4 * c + e] = t4[e];
+        }
+        if (t0 + kBlkTokens > r.len) {  // places that hold no token yet: whatever bits they have
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t0 + 2 * gj + (e >> 1) * 8 + (e & 1) >= r.len) vz[e] = 0u;
+        }
+        uint32_t sc[2], zr[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          sc[hh] = __byte_perm(vz[2 * hh], vz[2 * hh + 1], 0x5410);
+          zr[hh] = __byte_perm(vz[2 * hh], vz[2 * hh + 1], 0x7632);
+        }
+#pragma unroll
+        for (int wi = 0; wi < B::W; ++wi) {
+          uint32_t x[2][2];  // [hi][dims 0-3 | 4-7]: two tokens' nibbles side by side
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const uint32_t u = vw[(hh * 2) * B::W + wi], v = vw[(hh * 2 + 1) * B::W + wi];
+            x[hh][0] = __byte_perm(u, v, 0x5410);
+            x[hh][1] = __byte_perm(u, v, 0x7632);
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint32_t a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // a0: hi 0, dim n; a1: dim n + 4; a2, a3: hi 1
+              const uint32_t u = x[e >> 1][e & 1] >> (8 * (n >> 1));
+              const uint32_t c = n & 1 ? hsub2(lop_or(u, 0x00f000f0u, 0x54005400u), 0x54005400u)
+                                       : hsub2(lop_or(u, 0x000f000fu, 0x64006400u), 0x64006400u);
+              a[e] = hfma2(c, sc[e >> 1], zr[e >> 1]);
+            }
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+              mma_16816(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], ph[nr][0], ph[nr][1]);
+              if constexpr (Sh::LO) mma_16816(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], pl[nr][0], pl[nr][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+
+    // ---- join the warps -------------------------------------------------------
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int sft = 4; sft < 32; sft <<= 1) l[nr][c] += __shfl_xor_sync(0xffffffffu, l[nr][c], sft);
+        const int row = nr * 8 + 2 * gj + c;
+        const bool mine = MODE != kRows4 || gj < 2;
+        if (MODE == kRows4) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            o[nr][t][c] += __shfl_xor_sync(0xffffffffu, o[nr][t][c], 2);
+            o[nr][t][c + 2] += __shfl_xor_sync(0xffffffffu, o[nr][t][c + 2], 2);
+          }
+        }
+        if (mine) {
+          float* dst = s_o + (warp * R + row) * (D + 4);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {  // tile t = (word wi, nibble n): dims 8 (i W + wi) + n, + 4
+            const int dim = (gi * B::W + t / 4) * 8 + t % 4;
+            dst[dim] = o[nr][t][c];
+            dst[dim + 4] = o[nr][t][c + 2];
+          }
+          if (gi == 0) {
+            s_m[warp * R + row] = m[nr][c];
+            s_l[warp * R + row] = l[nr][c];
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (tid < R) {
+      float mm = kLow, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_m[w * R + tid]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = ex2(s_m[w * R + tid] - mm);
+        ll += f * s_l[w * R + tid];
+        s_m[w * R + tid] = f;
+      }
+      s_rm[tid] = mm;
+      s_rl[tid] = ll;
+    }
+    __syncthreads();
+    const int64_t body = walk.at + kSegCost;
+    const int c_first = cta_of(body), c_last = cta_of(body + r.nblk - 1);
+    const bool whole = c_first == c_last;
+    constexpr int kPart = R * (D + 2);
+    float* parts = reinterpret_cast<float*>(p.ws + ((size_t)p.n_slots * 4 + 15) / 16 * 16);
+    // a CTA leaves at most two parts: of the unit it starts in, and of the one it ends in
+    auto slot_of = [&](int c) {
+      const int64_t st = range_start(c);
+      return parts + (size_t)(2 * c + (st >= walk.at ? 0 : 1)) * kPart;
+    };
+    float* mine = whole ? nullptr : slot_of(blockIdx.x);
+    auto finish = [&](int row, int dim, float4 v, float mm, float ll) {  // 4 dims of a row
+      const int rr = row0 + row, hd = walk.h * p.grp + rr % p.grp;
+      const int64_t t = tok0 + (int64_t)(rr / p.grp);
+      if (t >= p.n_tokens) return;
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      const int64_t at = (t * p.hq + hd) * D + dim;
+      uint2 u;
+      if (p.dtype == SS_F16) {
+        u = make_uint2(pack_h2(v.x * inv, v.y * inv), pack_h2(v.z * inv, v.w * inv));
+      } else {
+        __nv_bfloat162 a = __floats2bfloat162_rn(v.x * inv, v.y * inv), c = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+        u = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&c));
+      }
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = u;
+      if (p.lse && dim == 0) p.lse[t * p.hq + hd] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
+    };
+    for (int e = tid; e < rows * (D / 4); e += T) {
+      const int row = e / (D / 4), dim = e % (D / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = s_m[w * R + row];
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * R + row) * (D + 4) + dim);
+        v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+      }
+      if (whole) {
+        finish(row, dim, v, s_rm[row], s_rl[row]);
+      } else {
+        __stcg(reinterpret_cast<float4*>(mine + row * D + dim), v);
+      }
+    }
+    if (!whole) {
+      if (tid < rows) {
+        __stcg(mine + R * D + tid, s_rm[tid]);
+        __stcg(mine + R * D + R + tid, s_rl[tid]);
+      }
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        uint32_t* cnt = reinterpret_cast<uint32_t*>(p.ws) + c_first;
+        const uint32_t parts_n = c_last - c_first + 1;
+        const uint32_t seen = atomicAdd(cnt, 1u);
+        if (seen == parts_n - 1) *cnt = 0u;  // every part is in: the counter is ready for the next launch
+        __threadfence();
+        s_flag[0] = seen == parts_n - 1 ? 1.f : 0.f;
+      }
+      __syncthreads();
+      if (s_flag[0] != 0.f) {
+        for (int e = tid; e < rows * (D / 4); e += T) {
+          const int row = e / (D / 4), dim = e % (D / 4) * 4;
+          float mm = kLow, ll = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = c_first; c <= c_last; ++c) {
+            const float* src = slot_of(c);
+            const float m2 = __ldcg(src + R * D + row), l2 = __ldcg(src + R * D + R + row);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src + row * D + dim));
+            const float mn = fmaxf(mm, m2), f1 = ex2(mm - mn), f2 = ex2(m2 - mn);
+            mm = mn;
+            ll = f1 * ll + f2 * l2;
+            v.x = f1 * v.x + f2 * x.x; v.y = f1 * v.y + f2 * x.y; v.z = f1 * v.z + f2 * x.z; v.w = f1 * v.w + f2 * x.w;
+          }
+          finish(row, dim, v, mm, ll);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Workspace: a counter per CTA, then two parts per CTA (up to 16 rows of D + 2 floats).
+size_t attn_ws_bytes(int d, int ctas) {
+  return ((size_t)ctas * 4 + 15) / 16 * 16 + (size_t)ctas * 2 * 16 * (d + 2) * 4;
+}
+
+template <int D, int MODE>
+int launch_decode(AttnParams& p, cudaStream_t st) {
+  constexpr int smem = Shape<D, MODE>::kSmem;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(SS_ERR_CUDA, std::string("ss_int4_attention: ") + cudaGetErrorString(e));
+  attn_decode_kernel<D, MODE><<<p.n_slots, Shape<D, MODE>::W * 32, smem, st>>>(p);
+  return check_launch("ss_int4_attention");
+}
+
+template <int D>
+int launch_mode(AttnParams& p, int rows, cudaStream_t st) {
+  const bool lo = p.dtype == SS_F16;
+  if (rows <= 4) return launch_decode<D, kRows4>(p, st);
+  if (rows <= 8 || D == 256) return lo ? launch_decode<D, kRows8Lo>(p, st) : launch_decode<D, kRows8>(p, st);
+  if constexpr (D != 256) return lo ? launch_decode<D, kRows16Lo>(p, st) : launch_decode<D, kRows16>(p, st);
+  return SS_OK;
 }
 
 }  // namespace
@@ -88,7 +733,11 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnParams p) {
 
 using namespace ss;
 
-extern "C" int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
+extern "C" {
+
+size_t ss_int4_attention_workspace(int d) { return attn_ws_bytes(d, sm_count()); }
+
+int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
   return c_entry([&]() -> int {
     SS_REQUIRE(a, "ss_int4_attention: null pointer");
     if (a->n_tokens == 0) return SS_OK;
@@ -102,25 +751,31 @@ extern "C" int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
                "ss_int4_attention: empty batch, pool or table");
     SS_REQUIRE(a->page_size >= 16 && a->page_size % 16 == 0,
                "ss_int4_attention: page_size must be a multiple of 16");
+    SS_REQUIRE((int64_t)a->width * a->page_size <= 0x7fffffff - 256,
+               "ss_int4_attention: a table row must hold fewer than 2^31 tokens");
     SS_REQUIRE(((reinterpret_cast<uintptr_t>(a->pages) | (uintptr_t)a->page_stride | (uintptr_t)a->head_stride) & 15) == 0,
                "ss_int4_attention: the pool and its strides must be multiples of 16 bytes");
-    SS_REQUIRE(a->window >= 0, "ss_int4_attention: window must not be negative");
+    SS_REQUIRE((reinterpret_cast<uintptr_t>(a->out) & 15) == 0, "ss_int4_attention: out must be 16-byte aligned");
+    SS_REQUIRE(a->window >= 0 && a->max_q >= 1, "ss_int4_attention: window must not be negative, max_q positive");
+    const int ctas = sm_count();
+    if (!a->workspace || a->workspace_bytes < attn_ws_bytes(a->d, ctas) || (reinterpret_cast<uintptr_t>(a->workspace) & 15))
+      return fail(SS_ERR_WORKSPACE, "ss_int4_attention: workspace null, too small or not 16-byte aligned");
     count_dispatch("ss_int4_attention");
     AttnParams p{};
     p.q = a->q; p.dtype = a->dtype; p.q_st = a->q_token_stride; p.q_sh = a->q_head_stride;
-    p.n_tokens = a->n_tokens; p.hq = a->hq; p.hkv = a->hkv;
+    p.n_tokens = a->n_tokens; p.hq = a->hq; p.hkv = a->hkv; p.grp = a->hq / a->hkv;
     p.pages = static_cast<const uint8_t*>(a->pages); p.n_pages = a->n_pages;
     p.page_stride = a->page_stride; p.head_stride = a->head_stride; p.page = a->page_size;
     p.table = a->block_table; p.table_stride = a->table_stride; p.width = a->width;
     p.seq_lens = a->seq_lens; p.cu_q = a->cu_q; p.n = a->n_requests;
     p.scale = a->scale; p.causal = a->causal; p.window = a->window;
     p.out = a->out; p.lse = a->lse;
-    const int64_t warps = a->n_tokens * a->hq;
-    const unsigned grid = (unsigned)((warps + 7) / 8);
+    p.ws = static_cast<uint8_t*>(a->workspace); p.n_slots = ctas;
+    const int64_t most = (int64_t)a->max_q * p.grp;
+    const int rows = most > 16 ? 16 : (int)most;
     cudaStream_t st = as_stream(stream);
-    if (a->d == 64) attn_rows_kernel<64><<<grid, 256, 0, st>>>(p);
-    else if (a->d == 128) attn_rows_kernel<128><<<grid, 256, 0, st>>>(p);
-    else attn_rows_kernel<256><<<grid, 256, 0, st>>>(p);
-    return check_launch("ss_int4_attention");
+    return a->d == 64 ? launch_mode<64>(p, rows, st) : a->d == 128 ? launch_mode<128>(p, rows, st) : launch_mode<256>(p, rows, st);
   });
 }
+
+}  // extern "C"

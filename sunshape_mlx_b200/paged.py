@@ -23,6 +23,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib as L
+from .attention import workspace_for
 
 __all__ = ["StepPlan", "plan_step", "release_pages", "int4_append", "int4_fetch",
            "int4_attention", "int4_pool", "PageTables", "Int4PagedKVCache"]
@@ -234,12 +235,13 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     out = torch.empty((n, hq, d), dtype=queries.dtype, device=dev)
     lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if return_lse else None
     if n:
+        ws = workspace_for(dev, L.load().ss_int4_attention_workspace(d), "int4")
         a = L.Int4AttnArgs(queries.data_ptr(), L.dtype_code(queries.dtype), queries.stride(0),
                            queries.stride(1), n, hq, hkv, d, pages.data_ptr(), pages.shape[0],
                            pages.stride(0), pages.stride(1), page, block_table.data_ptr(),
                            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
                            cu_q.data_ptr(), b, max_q, scale, 1 if causal else 0, window,
-                           out.data_ptr(), lse.data_ptr() if return_lse else None, None, 0)
+                           out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel())
         with L.on_device(dev):
             L.call("ss_int4_attention", C.byref(a), L.stream_ptr(dev))
     return (out, lse) if return_lse else out

@@ -343,7 +343,8 @@ def test_attention_large_and_special_values(ss):
     o = ss.int4_attention(big, pool, table, lens, cu, 1.0, max_q=1)
     for b, (k, v) in enumerate(kv):
         z = torch.einsum("hd,td->ht", big[b].double(), k[:, 0].double())
-        assert torch.equal(o[b], v[z.argmax(-1), 0].to(o.dtype))
+        want = v[z.argmax(-1), 0].double()  # values may pass through fp16 on their way to bf16: the bound above with dz = 0
+        assert ((o[b].double() - want).abs() <= (2.0 ** -8 + 4 * 2.0 ** -11) * want.abs()).all()
     # tiny ones: the mean of the values
     o = ss.int4_attention((q.float() * 1e-30).to(torch.bfloat16), pool, table, lens, cu, 1.0, max_q=1)
     for b, (k, v) in enumerate(kv):
