@@ -20,12 +20,13 @@
 //   S^T (16 tokens x 8 rows) by warp MMAs. With code c, scale s and zero z of
 //   a (token, group): q . k = sum_g s_g (sum_d q_d c_d) + sum_g z_g (sum_d q_d).
 //   The codes enter the MMA as 64 + c (a nibble ORed into the bits of 64.0 is
-//   exactly 64 + c), the accumulators start at -64 sum_d q_d, and s_g is
-//   applied to the fp32 result, so keys are never rounded. The zeros take one
-//   MMA more, with the row's group sums split into two fp16 terms.
+//   exactly 64 + c) and s_g is applied to the fp32 result, so keys are never
+//   rounded. The zeros, less the 64 s_g that this adds, take two MMAs more:
+//   z_g and s_g are the operand as they are stored, the row's group sums are
+//   split into two fp16 terms.
 //   Queries enter as fp16 after a power of two per row that puts the row's
-//   largest magnitude in [128, 256): exact for fp16 and bf16 down to 2^-31 of
-//   that magnitude.
+//   largest magnitude in [2, 4): exact for fp16 and bf16 down to 2^-25 of that
+//   magnitude.
 //   O^T (D x 8 rows) += V^T P^T: two tokens' words are interleaved by byte
 //   permutes so that a register holds a dim of two tokens; v = fp16(c s + z),
 //   the one rounding of the values. Probabilities are fp16 pairs hi + lo
@@ -47,7 +48,8 @@ struct AttnParams {
   const uint8_t* pages;
   int n_pages;
   int64_t page_stride, head_stride;
-  int page;
+  int page, page_blocks;  // tokens and blocks of a page
+  uint32_t page_inv;      // 2^32 / page_blocks, rounded up
   const int32_t* table;
   int64_t table_stride;
   int width;
@@ -153,6 +155,19 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 __device__ __forceinline__ float lo_h(uint32_t x) { return __low2float(*reinterpret_cast<__half2*>(&x)); }
 __device__ __forceinline__ float hi_h(uint32_t x) { return __high2float(*reinterpret_cast<__half2*>(&x)); }
+
+// Page of a request's block k, and the block's place in it.
+__device__ __forceinline__ int page_of(const AttnParams& p, int k, int& in_page) {
+  if (p.page_blocks == 1) {
+    in_page = 0;
+    return k;
+  }
+  int q = (int)__umulhi((uint32_t)k, p.page_inv);  // k / page_blocks, or one more
+  int r = k - q * p.page_blocks;
+  if (r < 0) { --q; r += p.page_blocks; }
+  in_page = r;
+  return q;
+}
 
 template <int N>
 __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&v)[N]) {
@@ -280,7 +295,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 
   // ---- copies: this warp's blocks in the order it will use them -------------
   Walk<R> pw = walk;
-  int pk = 0, pk1 = 0, pid = 0, pn = 0;
+  int pk = 0, pk1 = 0, pid = 0, pin = 0, pn = 0;
+  uint32_t hidden = 0;  // a bit per issued block: its table entry is outside the pool
   bool more = true, fresh = true;
   auto issue = [&](int stage) {
     while (more && (fresh || pk >= pk1)) {
@@ -294,17 +310,21 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
     if (more) {
       if (pn == 32) {  // page ids of the next 32 blocks, one a lane
         const int k = pk + lane * W;
-        pid = k < pk1 ? p.table[pw.b * p.table_stride + (int64_t)k * kBlkTokens / p.page] : -1;
+        pid = k < pk1 ? p.table[pw.b * p.table_stride + page_of(p, k, pin)] : -1;
         pn = 0;
       }
-      const int id = __shfl_sync(0xffffffffu, pid, pn++);
+      const int id = __shfl_sync(0xffffffffu, pid, pn), in_page = __shfl_sync(0xffffffffu, pin, pn);
+      ++pn;
       const bool ok = id >= 0 && id < p.n_pages;
+      hidden = hidden << 1 | (ok ? 0u : 1u);
       const uint8_t* src = p.pages;
-      if (ok) src += id * p.page_stride + pw.h * p.head_stride + (int64_t)((int64_t)pk * kBlkTokens % p.page / kBlkTokens) * B::kBytes;
+      if (ok) src += id * p.page_stride + pw.h * p.head_stride + in_page * B::kBytes;
       const uint32_t dst = smem_u32(ring + stage * B::kBytes);
 #pragma unroll
       for (int i = lane; i < B::kBytes / 16; i += 32) cp_async16(dst + i * 16, src + (ok ? i * 16 : 0), ok ? 16 : 0);
       pk += W;
+    } else {
+      hidden <<= 1;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -323,8 +343,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 
     // queries as B fragments: lane (i, j) holds dims 32 g + 8 j .. + 7 of row i
     uint32_t qf[NR][G][4];
-    float bias[NR][G][2], fac[NR][2];
-    uint32_t qz[NR][2];
+    float fac[NR][2];
+    uint32_t qz[NR][2], qb[NR][2];
     int kend[NR][2], kbeg[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -343,9 +363,9 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // 2^e with big * 2^e in [128, 256); 1 for rows of zeros or infinities
+      // 2^e with big * 2^e in [2, 4); 1 for rows of zeros or infinities
       int ex = 0;
-      if (big > 0.f && big < INFINITY) ex = 134 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
+      if (big > 0.f && big < INFINITY) ex = 128 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
       const float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
       float sum[G];
 #pragma unroll
@@ -359,7 +379,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
       }
-      // group sums as the B fragment of the zeros' MMA: k = group hi, k + 8 = group lo
+      // B fragments of the zeros' MMAs: k = group against z, k + 8 = group against s; hi and lo
       float z0 = 0.f, z1 = 0.f;
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
@@ -367,13 +387,13 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
       qz[nr][0] = pack_h2(z0, z1);
       qz[nr][1] = pack_h2(z0 - lo_h(qz[nr][0]), z1 - hi_h(qz[nr][0]));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qb[nr][e] = pack_h2(-64.f * lo_h(qz[nr][e]), -64.f * hi_h(qz[nr][e]));
       const float back = p.scale * kLog2e / up;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {  // the columns of this lane's accumulators
         const int cc = 2 * gj + c, from = cc * 4;
         fac[nr][c] = __shfl_sync(0xffffffffu, back, from);
-#pragma unroll
-        for (int g = 0; g < G; ++g) bias[nr][g][c] = -64.f * __shfl_sync(0xffffffffu, sum[g], from);
         const int rr = MODE == kRows4 ? (cc & 3) : nr * 8 + cc;
         const int pos = r.len - r.nq + (row0 + rr) / p.grp;
         kend[nr][c] = rr >= rows ? 0 : p.causal ? min(r.len, pos + 1) : r.len;
@@ -411,16 +431,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       l[nr][0] = l[nr][1] = 0.f;
     }
 
-    // page ids of this warp's blocks, to hide keys of table entries outside the pool
-    int cid = 0, cn = 32;
     for (int k = k0 + warp; k < k1; k += W) {
-      if (cn == 32) {
-        const int kk = k + lane * W;
-        cid = kk < k1 ? p.table[b * p.table_stride + (int64_t)kk * kBlkTokens / p.page] : 0;
-        cn = 0;
-      }
-      const int id = __shfl_sync(0xffffffffu, cid, cn++);
-      const bool there = id >= 0 && id < p.n_pages;
+      const bool there = (hidden >> (S - 2) & 1) == 0;
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
       __syncwarp();
       issue(stage == 0 ? S - 1 : stage - 1);
@@ -431,18 +443,21 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       // ---- logits: S^T = K Q^T ----
       float s[NR][4];
       {
-        uint32_t z[4] = {0u, 0u, 0u, 0u};  // zeros of tokens i, i + 8: groups 2j, 2j + 1
+        uint32_t z[4] = {0u, 0u, 0u, 0u};  // zeros, then scales, of tokens i, i + 8: groups 2j, 2j + 1
         if (2 * gj < G) {
           uint32_t a[2], c[2];
           lds(blk + B::key_sz(gi, 2 * gj), a);
           lds(blk + B::key_sz(gi + 8, 2 * gj), c);
-          z[0] = z[2] = __byte_perm(a[0], a[1], 0x7632);
-          z[1] = z[3] = __byte_perm(c[0], c[1], 0x7632);
+          z[0] = __byte_perm(a[0], a[1], 0x7632);
+          z[1] = __byte_perm(c[0], c[1], 0x7632);
+          z[2] = __byte_perm(a[0], a[1], 0x5410);
+          z[3] = __byte_perm(c[0], c[1], 0x5410);
         }
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.f;
-          mma_16816(s[nr], z[0], z[1], z[2], z[3], qz[nr][0], qz[nr][1]);
+          mma_16816(s[nr], z[0], z[1], z[2], z[3], qz[nr][0], qb[nr][0]);
+          mma_16816(s[nr], z[0], z[1], z[2], z[3], qz[nr][1], qb[nr][1]);
         }
 #pragma unroll
         for (int c = 0; c < G / N; ++c) {
@@ -463,7 +478,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
             const float s0 = lo_h(z0[g]), s1 = lo_h(z1[g]);
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-              float a[4] = {bias[nr][c * N + g][0], bias[nr][c * N + g][1], bias[nr][c * N + g][0], bias[nr][c * N + g][1]};
+              float a[4] = {0.f, 0.f, 0.f, 0.f};
               mma_16816(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
               mma_16816(a, h0[2], h1[2], h0[3], h1[3], qf[nr][c * N + g][2], qf[nr][c * N + g][3]);
               s[nr][0] = fmaf(s0, a[0], s[nr][0]);
@@ -482,7 +497,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       for (int nr = 0; nr < NR; ++nr) {
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = s[nr][e] * fac[nr][e & 1];
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(s[nr][e], fac[nr][e & 1], -m[nr][e & 1]);
         if (edge) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -490,8 +505,9 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
             if (!there || t >= kend[nr][e & 1] || t < kbeg[nr][e & 1]) y[e] = -INFINITY;
           }
         }
-        const bool over = fmaxf(y[0], y[2]) > m[nr][0] + kSlack || fmaxf(y[1], y[3]) > m[nr][1] + kSlack;
-        if (__any_sync(0xffffffffu, over)) {
+        if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[2]), fmaxf(y[1], y[3])) > kSlack)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = y[e] == -INFINITY ? y[e] : s[nr][e] * fac[nr][e & 1];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float top = fmaxf(y[c], y[c + 2]);
@@ -500,6 +516,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
             const float mn = fmaxf(m[nr][c], top), f = ex2(m[nr][c] - mn);
             m[nr][c] = mn;
             l[nr][c] *= f;
+            y[c] -= mn;
+            y[c + 2] -= mn;
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
               o[nr][t][c] *= f;
@@ -508,7 +526,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e] - m[nr][e & 1]);
+        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
         l[nr][0] += y[0] + y[2];
         l[nr][1] += y[1] + y[3];
         uint32_t a = pack_h2(y[0], y[1]), c = pack_h2(y[2], y[3]);
@@ -766,6 +784,8 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.n_tokens = a->n_tokens; p.hq = a->hq; p.hkv = a->hkv; p.grp = a->hq / a->hkv;
     p.pages = static_cast<const uint8_t*>(a->pages); p.n_pages = a->n_pages;
     p.page_stride = a->page_stride; p.head_stride = a->head_stride; p.page = a->page_size;
+    p.page_blocks = a->page_size / kBlkTokens;
+    p.page_inv = p.page_blocks == 1 ? 0u : (uint32_t)(((1ull << 32) + p.page_blocks - 1) / p.page_blocks);
     p.table = a->block_table; p.table_stride = a->table_stride; p.width = a->width;
     p.seq_lens = a->seq_lens; p.cu_q = a->cu_q; p.n = a->n_requests;
     p.scale = a->scale; p.causal = a->causal; p.window = a->window;
