@@ -41,7 +41,7 @@ namespace {
 
 struct AttnParams {
   const void* q;
-  int dtype;
+  int dtype, q_vec;  // q_vec: rows of q are 16-byte aligned
   int64_t q_st, q_sh;
   int64_t n_tokens;
   int hq, hkv, grp;
@@ -82,7 +82,7 @@ struct Shape {
   static constexpr int S = D == 256 ? 3 : 4;       // ring stages of a warp
   static constexpr int kRing = W * S * Int4Blk<D>::kBytes;
   static constexpr int kMerge = W * R * (D + 4) * 4;  // rows padded by 4 floats
-  static constexpr int kSmem = kRing + kMerge + (2 * W * R + 3 * R) * 4 + (W * 32 + 2) * 8;
+  static constexpr int kSmem = kRing + kMerge + 2 * W * R * 4 + (W * 32 + 1) * 8;
 };
 
 // What a request contributes to the schedule.
@@ -148,9 +148,15 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// D(16x8) += A(16x16) B(16x8) as mma_16816, free to be scheduled among independent ones.
+__device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ float lo_h(uint32_t x) { return __low2float(*reinterpret_cast<__half2*>(&x)); }
@@ -193,10 +199,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
   float* s_o = reinterpret_cast<float*>(smem + Sh::kRing);            // [W][R][D + 4]
   float* s_m = s_o + W * R * (D + 4);                                 // [W][R]
   float* s_l = s_m + W * R;                                           // [W][R]
-  float* s_rm = s_l + W * R;                                          // [R] joined reference
-  float* s_rl = s_rm + R;                                             // [R] joined sum
-  float* s_flag = s_rl + R;                                           // [R] (only [0]: last to arrive)
-  int64_t* s_cum = reinterpret_cast<int64_t*>(s_flag + R);            // [T] + 2
+  int64_t* s_cum = reinterpret_cast<int64_t*>(s_l + W * R);           // [T]
+  int* s_last = reinterpret_cast<int*>(s_cum + T);                    // this CTA joins the unit's parts
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gi = lane >> 2, gj = lane & 3;
@@ -353,12 +357,24 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       const int tt = (row0 + row) / p.grp, hd = walk.h * p.grp + (row0 + row) % p.grp;
       const bool live = row < rows && tok0 + (int64_t)tt < p.n_tokens;
       const int64_t at = (tok0 + (int64_t)tt) * p.q_st + hd * p.q_sh + gj * 8;
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + at;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+        if (live) {
+          if (p.q_vec) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(qp + g * 32));
+            u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+          } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[g][e] = live ? load_as_f32(p.q, p.dtype, at + g * 32 + e) : 0.f;
-          big = fmaxf(big, fabsf(x[g][e]));
+            for (int e = 0; e < 4; ++e) u[e] = qp[g * 32 + 2 * e] | (uint32_t)qp[g * 32 + 2 * e + 1] << 16;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[g][2 * e] = p.dtype == SS_F16 ? lo_h(u[e]) : __uint_as_float(u[e] << 16);
+          x[g][2 * e + 1] = p.dtype == SS_F16 ? hi_h(u[e]) : __uint_as_float(u[e] & 0xffff0000u);
+          big = fmaxf(big, fmaxf(fabsf(x[g][2 * e]), fabsf(x[g][2 * e + 1])));
         }
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
@@ -456,8 +472,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.f;
-          mma_16816(s[nr], z[0], z[1], z[2], z[3], qz[nr][0], qb[nr][0]);
-          mma_16816(s[nr], z[0], z[1], z[2], z[3], qz[nr][1], qb[nr][1]);
+          mma(s[nr], z[0], z[1], z[2], z[3], qz[nr][0], qb[nr][0]);
+          mma(s[nr], z[0], z[1], z[2], z[3], qz[nr][1], qb[nr][1]);
         }
 #pragma unroll
         for (int c = 0; c < G / N; ++c) {
@@ -479,8 +495,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
               float a[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_16816(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
-              mma_16816(a, h0[2], h1[2], h0[3], h1[3], qf[nr][c * N + g][2], qf[nr][c * N + g][3]);
+              mma(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
+              mma(a, h0[2], h1[2], h0[3], h1[3], qf[nr][c * N + g][2], qf[nr][c * N + g][3]);
               s[nr][0] = fmaf(s0, a[0], s[nr][0]);
               s[nr][1] = fmaf(s0, a[1], s[nr][1]);
               s[nr][2] = fmaf(s1, a[2], s[nr][2]);
@@ -586,8 +602,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
             }
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-              mma_16816(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], ph[nr][0], ph[nr][1]);
-              if constexpr (Sh::LO) mma_16816(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], pl[nr][0], pl[nr][1]);
+              mma(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], ph[nr][0], ph[nr][1]);
+              if constexpr (Sh::LO) mma(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], pl[nr][0], pl[nr][1]);
             }
           }
         }
@@ -614,10 +630,9 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         if (mine) {
           float* dst = s_o + (warp * R + row) * (D + 4);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {  // tile t = (word wi, nibble n): dims 8 (i W + wi) + n, + 4
-            const int dim = (gi * B::W + t / 4) * 8 + t % 4;
-            dst[dim] = o[nr][t][c];
-            dst[dim + 4] = o[nr][t][c + 2];
+          for (int t = 0; t < MT; ++t) {  // place 16 t + 8 h + i: a warp's stores go to 32 banks
+            dst[16 * t + gi] = o[nr][t][c];
+            dst[16 * t + 8 + gi] = o[nr][t][c + 2];
           }
           if (gi == 0) {
             s_m[warp * R + row] = m[nr][c];
@@ -627,30 +642,15 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
     }
     __syncthreads();
-    if (tid < R) {
-      float mm = kLow, ll = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_m[w * R + tid]);
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float f = ex2(s_m[w * R + tid] - mm);
-        ll += f * s_l[w * R + tid];
-        s_m[w * R + tid] = f;
-      }
-      s_rm[tid] = mm;
-      s_rl[tid] = ll;
-    }
-    __syncthreads();
     const int64_t body = walk.at + kSegCost;
     const int c_first = cta_of(body), c_last = cta_of(body + r.nblk - 1);
     const bool whole = c_first == c_last;
     constexpr int kPart = R * (D + 2);
     float* parts = reinterpret_cast<float*>(p.ws + ((size_t)p.n_slots * 4 + 15) / 16 * 16);
-    // a CTA leaves at most two parts: of the unit it starts in, and of the one it ends in
-    auto slot_of = [&](int c) {
-      const int64_t st = range_start(c);
-      return parts + (size_t)(2 * c + (st >= walk.at ? 0 : 1)) * kPart;
-    };
+    // a CTA leaves at most two parts: of the unit it starts in (the first slot), and of the one it
+    // ends in; only a unit's first CTA can have started in another one
+    const int first_slot = range_start(c_first) >= walk.at ? 0 : 1;
+    auto slot_of = [&](int c) { return parts + (size_t)(2 * c + (c == c_first ? first_slot : 0)) * kPart; };
     float* mine = whole ? nullptr : slot_of(blockIdx.x);
     auto finish = [&](int row, int dim, float4 v, float mm, float ll) {  // 4 dims of a row
       const int rr = row0 + row, hd = walk.h * p.grp + rr % p.grp;
@@ -670,24 +670,31 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
     };
     for (int e = tid; e < rows * (D / 4); e += T) {
       const int row = e / (D / 4), dim = e % (D / 4) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float mm = kLow, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_m[w * R + row]);
+      // dims 8 (i W + wi) + 4 h + n are in tile 4 wi + n
+      const int x = dim / 8, at = x % B::W * 64 + dim / 4 % 2 * 8 + x / B::W;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float f = s_m[w * R + row];
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * R + row) * (D + 4) + dim);
-        v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+        const float f = ex2(s_m[w * R + row] - mm);
+        ll = fmaf(f, s_l[w * R + row], ll);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) v[n] = fmaf(f, s_o[(w * R + row) * (D + 4) + at + 16 * n], v[n]);
       }
+      const float4 v4 = make_float4(v[0], v[1], v[2], v[3]);
       if (whole) {
-        finish(row, dim, v, s_rm[row], s_rl[row]);
+        finish(row, dim, v4, mm, ll);
       } else {
-        __stcg(reinterpret_cast<float4*>(mine + row * D + dim), v);
+        __stcg(reinterpret_cast<float4*>(mine + row * D + dim), v4);
+        if (dim == 0) {
+          __stcg(mine + R * D + row, mm);
+          __stcg(mine + R * D + R + row, ll);
+        }
       }
     }
     if (!whole) {
-      if (tid < rows) {
-        __stcg(mine + R * D + tid, s_rm[tid]);
-        __stcg(mine + R * D + R + tid, s_rl[tid]);
-      }
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -696,14 +703,15 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         const uint32_t seen = atomicAdd(cnt, 1u);
         if (seen == parts_n - 1) *cnt = 0u;  // every part is in: the counter is ready for the next launch
         __threadfence();
-        s_flag[0] = seen == parts_n - 1 ? 1.f : 0.f;
+        *s_last = seen == parts_n - 1;
       }
       __syncthreads();
-      if (s_flag[0] != 0.f) {
+      if (*s_last) {
         for (int e = tid; e < rows * (D / 4); e += T) {
           const int row = e / (D / 4), dim = e % (D / 4) * 4;
           float mm = kLow, ll = 0.f;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
           for (int c = c_first; c <= c_last; ++c) {
             const float* src = slot_of(c);
             const float m2 = __ldcg(src + R * D + row), l2 = __ldcg(src + R * D + R + row);
@@ -781,6 +789,7 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     count_dispatch("ss_int4_attention");
     AttnParams p{};
     p.q = a->q; p.dtype = a->dtype; p.q_st = a->q_token_stride; p.q_sh = a->q_head_stride;
+    p.q_vec = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(a->q_token_stride * 2) | (uintptr_t)(a->q_head_stride * 2)) & 15) == 0;
     p.n_tokens = a->n_tokens; p.hq = a->hq; p.hkv = a->hkv; p.grp = a->hq / a->hkv;
     p.pages = static_cast<const uint8_t*>(a->pages); p.n_pages = a->n_pages;
     p.page_stride = a->page_stride; p.head_stride = a->head_stride; p.page = a->page_size;
