@@ -19,14 +19,14 @@
 // meet at the end of a unit only.
 //   S^T (16 tokens x 8 rows) by warp MMAs. With code c, scale s and zero z of
 //   a (token, group): q . k = sum_g s_g (sum_d q_d c_d) + sum_g z_g (sum_d q_d).
-//   The codes enter the MMA as 64 + c (a nibble ORed into the bits of 64.0 is
-//   exactly 64 + c) and s_g is applied to the fp32 result, so keys are never
-//   rounded. The zeros, less the 64 s_g that this adds, take two MMAs more:
-//   z_g and s_g are the operand as they are stored, the row's group sums are
-//   split into two fp16 terms.
+//   A nibble masked out of its word is, read as fp16, the subnormal c 2^-24 or
+//   c 2^-20: it enters the MMA as it is, the other power of two is in the
+//   query's dims, and s_g 2^24 is applied to the fp32 result, so keys are never
+//   rounded. The zeros take one MMA more: z_g as stored against the row's group
+//   sums in two fp16 terms.
 //   Queries enter as fp16 after a power of two per row that puts the row's
-//   largest magnitude in [2, 4): exact for fp16 and bf16 down to 2^-25 of that
-//   magnitude.
+//   largest magnitude in [256, 512): exact for fp16 and bf16 down to 2^-28 of
+//   that magnitude.
 //   O^T (D x 8 rows) += V^T P^T: two tokens' words are interleaved by byte
 //   permutes so that a register holds a dim of two tokens; v = fp16(c s + z),
 //   the one rounding of the values. Probabilities are fp16 pairs hi + lo
@@ -153,6 +153,17 @@ __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// D = A B
+__device__ __forceinline__ void mma0(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -299,36 +310,52 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 
   // ---- copies: this warp's blocks in the order it will use them -------------
   Walk<R> pw = walk;
-  int pk = 0, pk1 = 0, pid = 0, pin = 0, pn = 0;
-  uint32_t hidden = 0;  // a bit per issued block: its table entry is outside the pool
-  bool more = true, fresh = true;
-  auto issue = [&](int stage) {
-    while (more && (fresh || pk >= pk1)) {
-      if (!fresh) pw.next(p);
-      fresh = false;
-      if (pw.b >= p.n || pw.at >= hi) { more = false; break; }
+  int pk = 0, pk1 = 0, pn = 32;
+  int64_t poff = 0;      // a lane's block among the next 32: its offset in the pool, -1 if it has none
+  uint32_t hidden = 0;   // a bit per issued block: its table entry is outside the pool
+  bool more = true;
+  auto open = [&]() {  // the next unit in which this warp has a block
+    while (true) {
+      if (pw.b >= p.n || pw.at >= hi) { more = false; return; }
       blocks(pw, pk, pk1);
       pk += warp;
       pn = 32;
+      if (pk < pk1) return;
+      pw.next(p);
     }
+  };
+  open();
+  const uint32_t ring_at = smem_u32(ring) + lane * 16;
+  auto issue = [&](int stage) {
+    hidden <<= 1;
     if (more) {
-      if (pn == 32) {  // page ids of the next 32 blocks, one a lane
+      if (pn == 32) {
         const int k = pk + lane * W;
-        pid = k < pk1 ? p.table[pw.b * p.table_stride + page_of(p, k, pin)] : -1;
+        int in_page;
+        poff = -1;
+        if (k < pk1) {
+          const int id = p.table[pw.b * p.table_stride + page_of(p, k, in_page)];
+          if (id >= 0 && id < p.n_pages) poff = id * p.page_stride + pw.h * p.head_stride + in_page * B::kBytes;
+        }
         pn = 0;
       }
-      const int id = __shfl_sync(0xffffffffu, pid, pn), in_page = __shfl_sync(0xffffffffu, pin, pn);
-      ++pn;
-      const bool ok = id >= 0 && id < p.n_pages;
-      hidden = hidden << 1 | (ok ? 0u : 1u);
-      const uint8_t* src = p.pages;
-      if (ok) src += id * p.page_stride + pw.h * p.head_stride + in_page * B::kBytes;
-      const uint32_t dst = smem_u32(ring + stage * B::kBytes);
+      const int64_t off = __shfl_sync(0xffffffffu, poff, pn++);
+      const uint8_t* src = p.pages + off + lane * 16;
+      const uint32_t dst = ring_at + stage * B::kBytes;
+      if (off >= 0) {
 #pragma unroll
-      for (int i = lane; i < B::kBytes / 16; i += 32) cp_async16(dst + i * 16, src + (ok ? i * 16 : 0), ok ? 16 : 0);
+        for (int i = 0; i < B::kBytes / 512; ++i) cp_async16(dst + i * 512, src + i * 512, 16);
+        if (B::kBytes % 512 && lane < B::kBytes % 512 / 16) cp_async16(dst + B::kBytes / 512 * 512, src + B::kBytes / 512 * 512, 16);
+      } else {
+        hidden |= 1u;
+#pragma unroll
+        for (int i = lane; i < B::kBytes / 16; i += 32) cp_async16(dst + (i - lane) * 16, p.pages, 0);
+      }
       pk += W;
-    } else {
-      hidden <<= 1;
+      if (pk >= pk1) {
+        pw.next(p);
+        open();
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -348,7 +375,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
     // queries as B fragments: lane (i, j) holds dims 32 g + 8 j .. + 7 of row i
     uint32_t qf[NR][G][4];
     float fac[NR][2];
-    uint32_t qz[NR][2], qb[NR][2];
+    uint32_t qz[NR][2];
     int kend[NR][2], kbeg[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -379,9 +406,9 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // 2^e with big * 2^e in [2, 4); 1 for rows of zeros or infinities
+      // 2^e with big * 2^e in [256, 512); 1 for rows of zeros or infinities
       int ex = 0;
-      if (big > 0.f && big < INFINITY) ex = 128 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
+      if (big > 0.f && big < INFINITY) ex = 135 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
       const float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
       float sum[G];
 #pragma unroll
@@ -391,11 +418,12 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         for (int e = 0; e < 4; ++e) {  // a register: dims e and e + 4, as the key words' nibbles come
           qf[nr][g][e] = pack_h2(x[g][e] * up, x[g][e + 4] * up);
           sum[g] += lo_h(qf[nr][g][e]) + hi_h(qf[nr][g][e]);
+          if (e & 1) qf[nr][g][e] = hmul2(qf[nr][g][e], 0x2c002c00u);  // 2^-4: those codes come as 2^-20
         }
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
       }
-      // B fragments of the zeros' MMAs: k = group against z, k + 8 = group against s; hi and lo
+      // group sums as the B fragment of the zeros' MMA: k = group hi, k + 8 = group lo
       float z0 = 0.f, z1 = 0.f;
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
@@ -403,8 +431,6 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
       qz[nr][0] = pack_h2(z0, z1);
       qz[nr][1] = pack_h2(z0 - lo_h(qz[nr][0]), z1 - hi_h(qz[nr][0]));
-#pragma unroll
-      for (int e = 0; e < 2; ++e) qb[nr][e] = pack_h2(-64.f * lo_h(qz[nr][e]), -64.f * hi_h(qz[nr][e]));
       const float back = p.scale * kLog2e / up;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {  // the columns of this lane's accumulators
@@ -435,6 +461,8 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       all1 = min(all1, __shfl_xor_sync(0xffffffffu, all1, o));
     }
 
+    const int full0 = (all0 + kBlkTokens - 1) / kBlkTokens, full_n = max(0, all1 / kBlkTokens - full0);
+
     float o[NR][MT][4], m[NR][2], l[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -449,6 +477,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 
     for (int k = k0 + warp; k < k1; k += W) {
       const bool there = (hidden >> (S - 2) & 1) == 0;
+      const bool edge = (uint32_t)(k - full0) >= (uint32_t)full_n || !there;
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
       __syncwarp();
       issue(stage == 0 ? S - 1 : stage - 1);
@@ -459,21 +488,17 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       // ---- logits: S^T = K Q^T ----
       float s[NR][4];
       {
-        uint32_t z[4] = {0u, 0u, 0u, 0u};  // zeros, then scales, of tokens i, i + 8: groups 2j, 2j + 1
+        uint32_t z[2] = {0u, 0u};  // zeros of tokens i, i + 8: groups 2j, 2j + 1
         if (2 * gj < G) {
           uint32_t a[2], c[2];
           lds(blk + B::key_sz(gi, 2 * gj), a);
           lds(blk + B::key_sz(gi + 8, 2 * gj), c);
           z[0] = __byte_perm(a[0], a[1], 0x7632);
           z[1] = __byte_perm(c[0], c[1], 0x7632);
-          z[2] = __byte_perm(a[0], a[1], 0x5410);
-          z[3] = __byte_perm(c[0], c[1], 0x5410);
         }
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
-          s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.f;
-          mma(s[nr], z[0], z[1], z[2], z[3], qz[nr][0], qb[nr][0]);
-          mma(s[nr], z[0], z[1], z[2], z[3], qz[nr][1], qb[nr][1]);
+          mma0(s[nr], z[0], z[1], z[0], z[1], qz[nr][0], qz[nr][1]);
         }
 #pragma unroll
         for (int c = 0; c < G / N; ++c) {
@@ -484,18 +509,17 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
           lds(blk + B::key_sz(gi + 8, c * N), z1);
 #pragma unroll
           for (int g = 0; g < N; ++g) {
-            uint32_t h0[4], h1[4];  // 64 + code of dims (e, e + 4)
+            uint32_t h0[4], h1[4];  // codes of dims (e, e + 4) times 2^-24 (even e) or 2^-20
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t x0 = e == 0 ? w0[g] << 4 : w0[g] >> (4 * (e - 1)), x1 = e == 0 ? w1[g] << 4 : w1[g] >> (4 * (e - 1));
-              h0[e] = lop_or(x0, 0x00f000f0u, 0x54005400u);
-              h1[e] = lop_or(x1, 0x00f000f0u, 0x54005400u);
+              h0[e] = (e < 2 ? w0[g] : w0[g] >> 8) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
+              h1[e] = (e < 2 ? w1[g] : w1[g] >> 8) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
             }
-            const float s0 = lo_h(z0[g]), s1 = lo_h(z1[g]);
+            const float s0 = lo_h(z0[g]) * 16777216.f, s1 = lo_h(z1[g]) * 16777216.f;
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-              float a[4] = {0.f, 0.f, 0.f, 0.f};
-              mma(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
+              float a[4];
+              mma0(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
               mma(a, h0[2], h1[2], h0[3], h1[3], qf[nr][c * N + g][2], qf[nr][c * N + g][3]);
               s[nr][0] = fmaf(s0, a[0], s[nr][0]);
               s[nr][1] = fmaf(s0, a[1], s[nr][1]);
@@ -507,7 +531,6 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
 
       // ---- probabilities ----
-      const bool edge = !there || t0 < all0 || t0 + kBlkTokens > all1;
       uint32_t ph[NR][2], pl[NR][2];
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
@@ -570,7 +593,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 #pragma unroll
           for (int e = 0; e < 4; ++e) vw[4 * c + e] = t4[e];
         }
-        if (t0 + kBlkTokens > r.len) {  // places that hold no token yet: whatever bits they have
+        if (edge) {  // places that hold no token yet: whatever bits they have
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (t0 + 2 * gj + (e >> 1) * 8 + (e & 1) >= r.len) vz[e] = 0u;
