@@ -21,7 +21,7 @@
 //   a (token, group): q . k = sum_g s_g (sum_d q_d c_d) + sum_g z_g (sum_d q_d).
 //   A nibble masked out of its word is, read as fp16, the subnormal c 2^-24 or
 //   c 2^-20: it enters the MMA as it is, the other power of two is in the
-//   query's dims, and s_g 2^24 is applied to the fp32 result, so keys are never
+//   query's dims, and s_g is applied to the fp32 result, so keys are never
 //   rounded. The zeros take one MMA more: z_g as stored against the row's group
 //   sums in two fp16 terms.
 //   Queries enter as fp16 after a power of two per row that puts the row's
@@ -63,7 +63,7 @@ struct AttnParams {
   int n_slots;  // CTAs the workspace was sized for
 };
 
-constexpr int kSegCost = 24;     // blocks' worth of time that the ends of a unit take
+constexpr int kSegCost = 48;     // blocks' worth of time that the ends of a unit take
 constexpr int kMinCost = 96;     // a range is not cut below this many blocks' worth
 constexpr float kLow = -1e30f;   // softmax reference before any key
 constexpr float kSlack = 8.f;    // a logit may exceed the reference by this (base 2)
@@ -78,9 +78,11 @@ struct Shape {
   static constexpr int R = mode_rows(MODE);
   static constexpr int NR = R == 16 ? 2 : 1;       // 8-column tiles
   static constexpr bool LO = MODE == kRows8Lo || MODE == kRows16Lo;  // a second MMA for lo
-  static constexpr int W = D == 256 || NR == 2 ? 8 : 12;  // warps
-  static constexpr int S = D == 256 ? 3 : 4;       // ring stages of a warp
-  static constexpr int kRing = W * S * Int4Blk<D>::kBytes;
+  static constexpr int U = D == 256 || NR == 2 ? 1 : 2;  // blocks a warp takes at a time
+  static constexpr int kCtas = U == 2 ? 2 : 1;     // CTAs on an SM: one joins its warps while the other streams
+  static constexpr int W = kCtas == 2 ? 6 : 8;     // warps
+  static constexpr int S = D == 64 ? 4 : D == 256 ? 3 : U == 2 ? 2 : 4;  // ring stages of a warp
+  static constexpr int kRing = W * S * U * Int4Blk<D>::kBytes;
   static constexpr int kMerge = W * R * (D + 4) * 4;  // rows padded by 4 floats
   static constexpr int kSmem = kRing + kMerge + 2 * W * R * 4 + (W * 32 + 1) * 8;
 };
@@ -201,10 +203,10 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&v)[N]) {
 }
 
 template <int D, int MODE>
-__global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas) attn_decode_kernel(const __grid_constant__ AttnParams p) {
   using B = Int4Blk<D>;
   using Sh = Shape<D, MODE>;
-  constexpr int R = Sh::R, NR = Sh::NR, W = Sh::W, S = Sh::S, G = B::G, N = B::N, T = W * 32;
+  constexpr int R = Sh::R, NR = Sh::NR, W = Sh::W, S = Sh::S, U = Sh::U, G = B::G, N = B::N, T = W * 32;
   constexpr int MT = D / 16;  // 16-dim tiles of O
   extern __shared__ __align__(16) uint8_t smem[];
   float* s_o = reinterpret_cast<float*>(smem + Sh::kRing);            // [W][R][D + 4]
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gi = lane >> 2, gj = lane & 3;
-  uint8_t* ring = smem + warp * S * B::kBytes;
+  uint8_t* ring = smem + warp * S * U * B::kBytes;
 
   // tokens outside cu_q: zero rows
   {
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
     while (true) {
       if (pw.b >= p.n || pw.at >= hi) { more = false; return; }
       blocks(pw, pk, pk1);
-      pk += warp;
+      pk += warp * U;
       pn = 32;
       if (pk < pk1) return;
       pw.next(p);
@@ -327,10 +329,9 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
   open();
   const uint32_t ring_at = smem_u32(ring) + lane * 16;
   auto issue = [&](int stage) {
-    hidden <<= 1;
     if (more) {
       if (pn == 32) {
-        const int k = pk + lane * W;
+        const int k = pk + lane / U * (W * U) + lane % U;
         int in_page;
         poff = -1;
         if (k < pk1) {
@@ -339,23 +340,29 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         }
         pn = 0;
       }
-      const int64_t off = __shfl_sync(0xffffffffu, poff, pn++);
-      const uint8_t* src = p.pages + off + lane * 16;
-      const uint32_t dst = ring_at + stage * B::kBytes;
-      if (off >= 0) {
 #pragma unroll
-        for (int i = 0; i < B::kBytes / 512; ++i) cp_async16(dst + i * 512, src + i * 512, 16);
-        if (B::kBytes % 512 && lane < B::kBytes % 512 / 16) cp_async16(dst + B::kBytes / 512 * 512, src + B::kBytes / 512 * 512, 16);
-      } else {
-        hidden |= 1u;
+      for (int u = 0; u < U; ++u) {
+        const int64_t off = __shfl_sync(0xffffffffu, poff, pn++);
+        const uint8_t* src = p.pages + off + lane * 16;
+        const uint32_t dst = ring_at + (stage * U + u) * B::kBytes;
+        hidden <<= 1;
+        if (off >= 0) {
 #pragma unroll
-        for (int i = lane; i < B::kBytes / 16; i += 32) cp_async16(dst + (i - lane) * 16, p.pages, 0);
+          for (int i = 0; i < B::kBytes / 512; ++i) cp_async16(dst + i * 512, src + i * 512, 16);
+          if (B::kBytes % 512 && lane < B::kBytes % 512 / 16) cp_async16(dst + B::kBytes / 512 * 512, src + B::kBytes / 512 * 512, 16);
+        } else {  // no such block: zeros
+          hidden |= 1u;
+#pragma unroll
+          for (int i = lane; i < B::kBytes / 16; i += 32) cp_async16(dst + (i - lane) * 16, p.pages, 0);
+        }
       }
-      pk += W;
+      pk += W * U;
       if (pk >= pk1) {
         pw.next(p);
         open();
       }
+    } else {
+      hidden <<= U;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -376,7 +383,6 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
     uint32_t qf[NR][G][4];
     float fac[NR][2];
     uint32_t qz[NR][2];
-    int kend[NR][2], kbeg[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       const int col = nr * 8 + gi, row = MODE == kRows4 ? (col & 3) : col;
@@ -431,27 +437,31 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       }
       qz[nr][0] = pack_h2(z0, z1);
       qz[nr][1] = pack_h2(z0 - lo_h(qz[nr][0]), z1 - hi_h(qz[nr][0]));
-      const float back = p.scale * kLog2e / up;
+      const float back = p.scale * (kLog2e * 0x1p24f) / up;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {  // the columns of this lane's accumulators
         const int cc = 2 * gj + c, from = cc * 4;
         fac[nr][c] = __shfl_sync(0xffffffffu, back, from);
-        const int rr = MODE == kRows4 ? (cc & 3) : nr * 8 + cc;
-        const int pos = r.len - r.nq + (row0 + rr) / p.grp;
-        kend[nr][c] = rr >= rows ? 0 : p.causal ? min(r.len, pos + 1) : r.len;
-        kbeg[nr][c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
       }
     }
+    // keys [beg, end) that a column's row sees
+    auto sees = [&](int nr, int c, int& beg, int& end) {
+      const int cc = 2 * gj + c, rr = MODE == kRows4 ? (cc & 3) : nr * 8 + cc;
+      const int pos = r.len - r.nq + (row0 + rr) / p.grp;
+      end = rr >= rows ? 0 : p.causal ? min(r.len, pos + 1) : r.len;
+      beg = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      return rr < rows;
+    };
     // blocks in [all0, all1) are seen whole by every row of the unit
     int all0 = 0, all1 = 0x7fffffff;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int rr = MODE == kRows4 ? ((2 * gj + c) & 3) : nr * 8 + 2 * gj + c;
-        if (rr < rows) {
-          all0 = max(all0, kbeg[nr][c]);
-          all1 = min(all1, kend[nr][c]);
+        int beg, end;
+        if (sees(nr, c, beg, end)) {
+          all0 = max(all0, beg);
+          all1 = min(all1, end);
         }
       }
     }
@@ -475,19 +485,21 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
       l[nr][0] = l[nr][1] = 0.f;
     }
 
-    for (int k = k0 + warp; k < k1; k += W) {
-      const bool there = (hidden >> (S - 2) & 1) == 0;
-      const bool edge = (uint32_t)(k - full0) >= (uint32_t)full_n || !there;
+    for (int k = k0 + warp * U; k < k1; k += W * U) {
+      const uint32_t gone = hidden >> ((S - 2) * U);  // bit U - 1 - u: block u is not there
+      const bool edge = (uint32_t)(k - full0) >= (uint32_t)full_n || k + U > full0 + full_n || (gone & ((1u << U) - 1)) != 0;
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
       __syncwarp();
       issue(stage == 0 ? S - 1 : stage - 1);
-      const uint8_t* blk = ring + stage * B::kBytes;
+      const uint8_t* blk0 = ring + stage * U * B::kBytes;
       stage = stage == S - 1 ? 0 : stage + 1;
       const int t0 = k * kBlkTokens;
 
       // ---- logits: S^T = K Q^T ----
-      float s[NR][4];
-      {
+      float s[U][NR][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint8_t* blk = blk0 + u * B::kBytes;
         uint32_t z[2] = {0u, 0u};  // zeros of tokens i, i + 8: groups 2j, 2j + 1
         if (2 * gj < G) {
           uint32_t a[2], c[2];
@@ -498,7 +510,9 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         }
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
-          mma0(s[nr], z[0], z[1], z[0], z[1], qz[nr][0], qz[nr][1]);
+          mma0(s[u][nr], z[0], z[1], z[0], z[1], qz[nr][0], qz[nr][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][nr][e] *= 0x1p-24f;  // the codes' power of two
         }
 #pragma unroll
         for (int c = 0; c < G / N; ++c) {
@@ -515,48 +529,70 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
               h0[e] = (e < 2 ? w0[g] : w0[g] >> 8) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
               h1[e] = (e < 2 ? w1[g] : w1[g] >> 8) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
             }
-            const float s0 = lo_h(z0[g]) * 16777216.f, s1 = lo_h(z1[g]) * 16777216.f;
+            const float s0 = lo_h(z0[g]), s1 = lo_h(z1[g]);
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
               float a[4];
               mma0(a, h0[0], h1[0], h0[1], h1[1], qf[nr][c * N + g][0], qf[nr][c * N + g][1]);
               mma(a, h0[2], h1[2], h0[3], h1[3], qf[nr][c * N + g][2], qf[nr][c * N + g][3]);
-              s[nr][0] = fmaf(s0, a[0], s[nr][0]);
-              s[nr][1] = fmaf(s0, a[1], s[nr][1]);
-              s[nr][2] = fmaf(s1, a[2], s[nr][2]);
-              s[nr][3] = fmaf(s1, a[3], s[nr][3]);
+              s[u][nr][0] = fmaf(s0, a[0], s[u][nr][0]);
+              s[u][nr][1] = fmaf(s0, a[1], s[u][nr][1]);
+              s[u][nr][2] = fmaf(s1, a[2], s[u][nr][2]);
+              s[u][nr][3] = fmaf(s1, a[3], s[u][nr][3]);
             }
           }
         }
       }
 
       // ---- probabilities ----
-      uint32_t ph[NR][2], pl[NR][2];
+      uint32_t ph[U][NR][2], pl[U][NR][2];
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
-        float y[4];
+        float y[U][4], over = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = fmaf(s[nr][e], fac[nr][e & 1], -m[nr][e & 1]);
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[u][e] = fmaf(s[u][nr][e], fac[nr][e & 1], -m[nr][e & 1]);
+        }
         if (edge) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int t = t0 + gi + (e >> 1) * 8;
-            if (!there || t >= kend[nr][e & 1] || t < kbeg[nr][e & 1]) y[e] = -INFINITY;
+          for (int c = 0; c < 2; ++c) {
+            int beg, end;
+            sees(nr, c, beg, end);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+              for (int e = c; e < 4; e += 2) {
+                const int t = t0 + u * kBlkTokens + gi + (e >> 1) * 8;
+                if ((gone >> (U - 1 - u) & 1) || t >= end || t < beg) y[u][e] = -INFINITY;
+              }
+            }
           }
         }
-        if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[2]), fmaxf(y[1], y[3])) > kSlack)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = y[e] == -INFINITY ? y[e] : s[nr][e] * fac[nr][e & 1];
+        for (int u = 0; u < U; ++u) over = fmaxf(over, fmaxf(fmaxf(y[u][0], y[u][2]), fmaxf(y[u][1], y[u][3])));
+        if (__any_sync(0xffffffffu, over > kSlack)) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(y[c], y[c + 2]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+              for (int e = c; e < 4; e += 2) {
+                y[u][e] = y[u][e] == -INFINITY ? y[u][e] : s[u][nr][e] * fac[nr][c];
+                top = fmaxf(top, y[u][e]);
+              }
+            }
 #pragma unroll
             for (int sft = 4; sft < 32; sft <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sft));
             const float mn = fmaxf(m[nr][c], top), f = ex2(m[nr][c] - mn);
             m[nr][c] = mn;
             l[nr][c] *= f;
-            y[c] -= mn;
-            y[c + 2] -= mn;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              y[u][c] -= mn;
+              y[u][c + 2] -= mn;
+            }
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
               o[nr][t][c] *= f;
@@ -565,25 +601,30 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
-        l[nr][0] += y[0] + y[2];
-        l[nr][1] += y[1] + y[3];
-        uint32_t a = pack_h2(y[0], y[1]), c = pack_h2(y[2], y[3]);
-        if constexpr (MODE == kRows4) {  // columns 4-7 repeat rows 0-3: they take lo
-          const uint32_t al = pack_h2(y[0] - lo_h(a), y[1] - hi_h(a)), cl = pack_h2(y[2] - lo_h(c), y[3] - hi_h(c));
-          a = gj < 2 ? a : al;
-          c = gj < 2 ? c : cl;
-        }
-        ph[nr][0] = transpose8x8(a);
-        ph[nr][1] = transpose8x8(c);
-        if constexpr (Sh::LO) {
-          pl[nr][0] = transpose8x8(pack_h2(y[0] - lo_h(a), y[1] - hi_h(a)));
-          pl[nr][1] = transpose8x8(pack_h2(y[2] - lo_h(c), y[3] - hi_h(c)));
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[u][e] = ex2(y[u][e]);
+          l[nr][0] += y[u][0] + y[u][2];
+          l[nr][1] += y[u][1] + y[u][3];
+          uint32_t a = pack_h2(y[u][0], y[u][1]), c = pack_h2(y[u][2], y[u][3]);
+          if constexpr (MODE == kRows4) {  // columns 4-7 repeat rows 0-3: they take lo
+            const uint32_t al = pack_h2(y[u][0] - lo_h(a), y[u][1] - hi_h(a)), cl = pack_h2(y[u][2] - lo_h(c), y[u][3] - hi_h(c));
+            a = gj < 2 ? a : al;
+            c = gj < 2 ? c : cl;
+          }
+          ph[u][nr][0] = transpose8x8(a);
+          ph[u][nr][1] = transpose8x8(c);
+          if constexpr (Sh::LO) {
+            pl[u][nr][0] = transpose8x8(pack_h2(y[u][0] - lo_h(a), y[u][1] - hi_h(a)));
+            pl[u][nr][1] = transpose8x8(pack_h2(y[u][2] - lo_h(c), y[u][3] - hi_h(c)));
+          }
         }
       }
 
       // ---- O^T += V^T P^T ----
-      {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint8_t* blk = blk0 + u * B::kBytes;
         uint32_t vz[4], vw[4 * B::W];
         lds(blk + B::value_sz(2 * gj, gi * B::W / 4), vz);
 #pragma unroll
@@ -596,7 +637,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
         if (edge) {  // places that hold no token yet: whatever bits they have
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t0 + 2 * gj + (e >> 1) * 8 + (e & 1) >= r.len) vz[e] = 0u;
+            if (t0 + u * kBlkTokens + 2 * gj + (e >> 1) * 8 + (e & 1) >= r.len) vz[e] = 0u;
         }
         uint32_t sc[2], zr[2];
 #pragma unroll
@@ -609,24 +650,24 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
           uint32_t x[2][2];  // [hi][dims 0-3 | 4-7]: two tokens' nibbles side by side
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            const uint32_t u = vw[(hh * 2) * B::W + wi], v = vw[(hh * 2 + 1) * B::W + wi];
-            x[hh][0] = __byte_perm(u, v, 0x5410);
-            x[hh][1] = __byte_perm(u, v, 0x7632);
+            const uint32_t a = vw[(hh * 2) * B::W + wi], c = vw[(hh * 2 + 1) * B::W + wi];
+            x[hh][0] = __byte_perm(a, c, 0x5410);
+            x[hh][1] = __byte_perm(a, c, 0x7632);
           }
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             uint32_t a[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // a0: hi 0, dim n; a1: dim n + 4; a2, a3: hi 1
-              const uint32_t u = x[e >> 1][e & 1] >> (8 * (n >> 1));
-              const uint32_t c = n & 1 ? hsub2(lop_or(u, 0x00f000f0u, 0x54005400u), 0x54005400u)
-                                       : hsub2(lop_or(u, 0x000f000fu, 0x64006400u), 0x64006400u);
+              const uint32_t xx = x[e >> 1][e & 1] >> (8 * (n >> 1));
+              const uint32_t c = n & 1 ? hsub2(lop_or(xx, 0x00f000f0u, 0x54005400u), 0x54005400u)
+                                       : hsub2(lop_or(xx, 0x000f000fu, 0x64006400u), 0x64006400u);
               a[e] = hfma2(c, sc[e >> 1], zr[e >> 1]);
             }
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-              mma(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], ph[nr][0], ph[nr][1]);
-              if constexpr (Sh::LO) mma(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], pl[nr][0], pl[nr][1]);
+              mma(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], ph[u][nr][0], ph[u][nr][1]);
+              if constexpr (Sh::LO) mma(o[nr][wi * 4 + n], a[0], a[1], a[2], a[3], pl[u][nr][0], pl[u][nr][1]);
             }
           }
         }
@@ -753,9 +794,10 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, 1) attn_decode_kernel(
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Workspace: a counter per CTA, then two parts per CTA (up to 16 rows of D + 2 floats).
-size_t attn_ws_bytes(int d, int ctas) {
-  return ((size_t)ctas * 4 + 15) / 16 * 16 + (size_t)ctas * 2 * 16 * (d + 2) * 4;
+// Workspace: a counter per CTA, then two parts per CTA of R rows of D + 2 floats
+// (up to 16 rows for one CTA on an SM, up to 8 for two).
+size_t attn_ws_bytes(int d, int sms) {
+  return ((size_t)sms * 2 * 4 + 15) / 16 * 16 + (size_t)sms * 2 * 16 * (d + 2) * 4;
 }
 
 template <int D, int MODE>
@@ -764,6 +806,7 @@ int launch_decode(AttnParams& p, cudaStream_t st) {
   static_assert(smem <= 227 * 1024, "shared memory");
   const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(SS_ERR_CUDA, std::string("ss_int4_attention: ") + cudaGetErrorString(e));
+  p.n_slots = sm_count() * Shape<D, MODE>::kCtas;
   attn_decode_kernel<D, MODE><<<p.n_slots, Shape<D, MODE>::W * 32, smem, st>>>(p);
   return check_launch("ss_int4_attention");
 }
@@ -822,7 +865,7 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.seq_lens = a->seq_lens; p.cu_q = a->cu_q; p.n = a->n_requests;
     p.scale = a->scale; p.causal = a->causal; p.window = a->window;
     p.out = a->out; p.lse = a->lse;
-    p.ws = static_cast<uint8_t*>(a->workspace); p.n_slots = ctas;
+    p.ws = static_cast<uint8_t*>(a->workspace); p.n_slots = 0;
     const int64_t most = (int64_t)a->max_q * p.grp;
     const int rows = most > 16 ? 16 : (int)most;
     cudaStream_t st = as_stream(stream);
