@@ -11,18 +11,30 @@
 // entropy 0. A row that holds NaN or +inf gives NaN, and ids -1.
 // A target < 0 gives 0 (padding), one >= vocab NaN.
 //
-// One CTA per row: one pass for the sums, then k passes that each take the
-// next one in order.
+// One pass over a row, by a CTA or, for few rows, by a cluster whose first
+// CTA joins the others' results out of their shared memory. A thread keeps
+// (M, l, A) of its own elements in fp32 and rescales only when 32 new ones
+// raise its maximum. The k-th largest of the threads' maxima bounds the k-th
+// largest element from below, so only the few threads whose maximum reaches it
+// hold candidates: their elements alone are read again (3 % of a row at k =
+// 20), by all threads together, and ranked against each other.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace ss {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
+constexpr int kLpMaxSplit = 8;
+constexpr int kLpCap = 1024;     // candidates of a CTA; more (many equal logits) take the ordered path
+constexpr int kLpVecs = 4;       // 16-byte loads of a thread in flight
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFar = -1e30f;  // stands for -inf in differences: its exponential is 0, times it is 0
+constexpr float kFar = -1e30f;   // stands for -inf in differences: its exponential is 0, times it is 0
 
 struct LpParams {
   const void* x;
@@ -34,90 +46,391 @@ struct LpParams {
   int32_t* top_ids;
 };
 
-__device__ __forceinline__ bool before(float v, int i, float w, int j) {  // (v, i) ranks before (w, j)
-  return v > w || (v == w && i < j);
+struct Sums {
+  float m, l, a;
+};
+
+__device__ __forceinline__ float lp_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ Sums merge(const Sums& x, const Sums& y) {
+  Sums r;
+  r.m = fmaxf(x.m, y.m);
+  const float d1 = fmaxf(x.m - r.m, kFar), d2 = fmaxf(y.m - r.m, kFar);
+  const float e1 = lp_ex2(d1 * kLog2e), e2 = lp_ex2(d2 * kLog2e);
+  r.l = e1 * x.l + e2 * y.l;
+  r.a = e1 * (x.a + d1 * x.l) + e2 * (y.a + d2 * y.l);
+  return r;
+}
+// max that keeps NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Unsigned integers in the order of the floats (-0 and +0 alike).
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ bool before(uint32_t k, int i, uint32_t k2, int i2) {  // ranks first
+  return k > k2 || (k == k2 && i < i2);
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LpParams p) {
-  __shared__ float s_m[kLpWarps], s_l[kLpWarps], s_a[kLpWarps], s_v[kLpWarps];
-  __shared__ int s_i[kLpWarps], s_bad;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
-  const char* base = reinterpret_cast<const char*>(p.x) + row * p.row_stride * (DT == SS_F32 ? 4 : 2);
-  if (tid == 0) s_bad = 0;
-  float m = -INFINITY, l = 0.f, a = 0.f;
-  bool bad = false;
-  for (int i = tid; i < p.vocab; i += kLpThreads) {
-    const float y = load_as_f32(base, DT, i);
-    bad |= !(y < INFINITY);
-    if (y > m) {
-      const float d = fmaxf(m - y, kFar), e = exp2f(d * kLog2e);
-      a = e * (a + d * l);
-      l *= e;
-      m = y;
-    }
-    const float d = fmaxf(y - m, kFar), e = exp2f(d * kLog2e);  // kFar too for -inf - -inf
-    l += e;
-    a += e * d;
-  }
-  if (bad) s_bad = 1;
-  auto merge = [](float& m, float& l, float& a, float m2, float l2, float a2) {
-    const float n = fmaxf(m, m2);
-    const float d1 = fmaxf(m - n, kFar), d2 = fmaxf(m2 - n, kFar);
-    const float e1 = exp2f(d1 * kLog2e), e2 = exp2f(d2 * kLog2e);
-    a = e1 * (a + d1 * l) + e2 * (a2 + d2 * l2);
-    l = e1 * l + e2 * l2;
-    m = n;
-  };
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o),
-                a2 = __shfl_xor_sync(0xffffffffu, a, o);
-    merge(m, l, a, m2, l2, a2);
-  }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; s_a[warp] = a; }
-  __syncthreads();
-  m = s_m[0]; l = s_l[0]; a = s_a[0];
-  for (int w = 1; w < kLpWarps; ++w) merge(m, l, a, s_m[w], s_l[w], s_a[w]);
-  bad = s_bad;
-  const float nan = __int_as_float(0x7fffffff);
-  const float ll = logf(l);
-  auto lp = [&](float x) { return bad ? nan : l > 0.f ? (x - m) - ll : -INFINITY; };
-  if (tid == 0) {
-    const int64_t t = p.targets ? p.targets[row] : -1;
-    p.logprobs[row] = t < 0 ? 0.f : t >= p.vocab ? nan : lp(load_as_f32(base, DT, t));
-    p.entropy[row] = bad ? nan : l > 0.f ? ll - a / l : 0.f;
-  }
-  float pv = INFINITY;
-  int pi = -1;
-  for (int k = 0; k < p.top; ++k) {
-    float v = -INFINITY;
-    int at = 0x7fffffff;
-    if (!bad) {
-      for (int i = tid; i < p.vocab; i += kLpThreads) {
-        const float x = load_as_f32(base, DT, i);
-        if (before(pv, pi, x, i) && before(x, i, v, at)) { v = x; at = i; }
+struct Vec {
+  static constexpr int E = DT == SS_F32 ? 4 : 8;  // elements of 16 bytes
+  static __device__ __forceinline__ void get(const uint4& u, float (&x)[E]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == SS_F32) {
+        x[i] = __uint_as_float(w[i]);
+      } else if constexpr (DT == SS_BF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
       }
     }
-    for (int o = 16; o > 0; o >>= 1) {
-      const float v2 = __shfl_xor_sync(0xffffffffu, v, o);
-      const int i2 = __shfl_xor_sync(0xffffffffu, at, o);
-      if (before(v2, i2, v, at)) { v = v2; at = i2; }
-    }
-    __syncthreads();
-    if (lane == 0) { s_v[warp] = v; s_i[warp] = at; }
-    __syncthreads();
-    v = s_v[0]; at = s_i[0];
-    for (int w = 1; w < kLpWarps; ++w)
-      if (before(s_v[w], s_i[w], v, at)) { v = s_v[w]; at = s_i[w]; }
-    pv = v;
-    pi = at;
-    if (tid == 0) {
-      const bool none = at == 0x7fffffff;
-      p.top_ids[row * p.top + k] = none ? -1 : at;
-      p.top_lp[row * p.top + k] = bad ? nan : none ? -INFINITY : lp(v);
+  }
+  static __device__ __forceinline__ uint32_t low() {  // two (one) elements of -inf
+    return DT == SS_F32 ? 0xff800000u : DT == SS_F16 ? 0xfc00fc00u : 0xff80ff80u;
+  }
+};
+
+// (a, b) op (x, y) as packed fp32
+__device__ __forceinline__ void fma_f32x2(float& a, float& b, float x0, float x1, float y0, float y1) {
+  asm("{\n .reg .b64 t, u, v;\n mov.b64 t, {%0, %1};\n mov.b64 u, {%2, %3};\n mov.b64 v, {%4, %5};\n"
+      " fma.rn.f32x2 t, u, v, t;\n mov.b64 {%0, %1}, t;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
+
+// Adds n elements to the sums; m already covers them.
+template <int N>
+__device__ __forceinline__ void add_up(const float (&x)[N], float m, float (&l)[2], float (&a)[2]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float d0 = x[i], d1 = x[i + 1];
+    add_f32x2(d0, d1, -m, -m);
+    d0 = fmaxf(d0, kFar);  // -inf, and -inf - -inf
+    d1 = fmaxf(d1, kFar);
+    float t0 = d0, t1 = d1;
+    mul_f32x2(t0, t1, kLog2e);
+    const float e0 = lp_ex2(t0), e1 = lp_ex2(t1);
+    add_f32x2(l[0], l[1], e0, e1);
+    fma_f32x2(a[0], a[1], e0, e1, d0, d1);
+  }
+}
+
+struct LpShared {
+  Sums warp[kLpWarps];
+  Sums sums;                     // this CTA's
+  float tmax[kLpThreads];        // the threads' maxima
+  uint32_t key[kLpCap];          // candidates
+  int idx[kLpCap];
+  uint32_t top_key[kLpMaxTop];   // this CTA's best, in order
+  int top_idx[kLpMaxTop];
+  uint32_t tau;
+  int hot[kLpThreads];
+  int n_hot, n_cand, n_top, base;
+  int wsum[kLpWarps];
+};
+
+// Ranks the n candidates of s and leaves the best k in order (dst may be s's own top).
+__device__ __forceinline__ void rank_candidates(const uint32_t* key, const int* idx, int n, int k, uint32_t* dk, int* di) {
+  for (int c = threadIdx.x; c < n; c += kLpThreads) {
+    const uint32_t kc = key[c];
+    const int ic = idx[c];
+    int r = 0;
+    for (int j = 0; j < n && r < k; ++j) r += before(key[j], idx[j], kc, ic);
+    if (r < k) {
+      dk[r] = kc;
+      di[r] = ic;
     }
   }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const __grid_constant__ LpParams p, int split) {
+  constexpr int E = Vec<DT>::E;
+  __shared__ LpShared s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x / split;
+  const int part = blockIdx.x % split;
+  constexpr int ES = DT == SS_F32 ? 4 : 2;
+  const char* base = reinterpret_cast<const char*>(p.x) + row * p.row_stride * ES;
+  // elements before the first 16-byte boundary, then vectors, then the rest
+  int head = (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / ES;
+  head = min(head, p.vocab);
+  const int vecs = (p.vocab - head) / E, tail0 = head + vecs * E;
+  const int per = (vecs + split - 1) / split, v0 = min(vecs, part * per), v1 = min(vecs, v0 + per);
+  const uint4* body = reinterpret_cast<const uint4*>(base + head * ES);
+  if (tid == 0) s.n_hot = s.n_cand = 0;
+
+  // ---- sums ----
+  float m = -INFINITY, l[2] = {0.f, 0.f}, a[2] = {0.f, 0.f};
+  auto raise = [&](float lm) {  // m must cover lm
+    if (lm > m) {
+      const float d = fmaxf(m - lm, kFar), e = lp_ex2(d * kLog2e);
+      a[0] = e * fmaf(d, l[0], a[0]);
+      a[1] = e * fmaf(d, l[1], a[1]);
+      l[0] *= e;
+      l[1] *= e;
+    }
+    m = max_nan(m, lm);
+  };
+  uint4 buf[kLpVecs];
+  auto load = [&](int v) {
+#pragma unroll
+    for (int u = 0; u < kLpVecs; ++u) {
+      const int at = v + u * kLpThreads;
+      buf[u] = at < v1 ? __ldcs(body + at) : make_uint4(Vec<DT>::low(), Vec<DT>::low(), Vec<DT>::low(), Vec<DT>::low());
+    }
+  };
+  if (v0 + tid < v1) load(v0 + tid);
+  for (int v = v0 + tid; v < v1; v += kLpVecs * kLpThreads) {
+    float x[kLpVecs][E];
+#pragma unroll
+    for (int u = 0; u < kLpVecs; ++u) Vec<DT>::get(buf[u], x[u]);
+    if (v + kLpVecs * kLpThreads < v1) load(v + kLpVecs * kLpThreads);
+    float lm = x[0][0];
+#pragma unroll
+    for (int u = 0; u < kLpVecs; ++u) {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) lm = max3_nan(lm, x[u][i], x[u][i + 1]);
+    }
+    raise(lm);
+#pragma unroll
+    for (int u = 0; u < kLpVecs; ++u) add_up(x[u], m, l, a);
+  }
+  // the ragged ends belong to the first part: a thread takes at most one element of each
+  const int n_ends = part == 0 ? head + p.vocab - tail0 : 0;
+  const int end_at = tid < head ? tid : tail0 + tid - head;
+  const float end_x = tid < n_ends ? load_as_f32(base, DT, end_at) : -INFINITY;
+  if (tid < n_ends) {
+    const float x[2] = {end_x, -INFINITY};
+    raise(end_x);
+    add_up(x, m, l, a);
+  }
+  s.tmax[tid] = m;
+  Sums t{m, l[0] + l[1], a[0] + a[1]};
+  float worst = m;  // NaN or +inf anywhere shows here
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Sums y{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.l, o), __shfl_xor_sync(0xffffffffu, t.a, o)};
+    t = merge(t, y);
+    worst = max_nan(worst, __shfl_xor_sync(0xffffffffu, worst, o));
+  }
+  if (lane == 0) s.warp[warp] = Sums{worst, t.l, t.a};
+  __syncthreads();
+
+  // ---- warp 0: the CTA's sums; the k-th largest of the threads' maxima ----
+  const int k = p.top;
+  if (warp == 0) {
+    Sums y = lane < kLpWarps ? s.warp[lane] : Sums{-INFINITY, 0.f, 0.f};
+    float w = y.m;
+#pragma unroll
+    for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+      const Sums z{__shfl_xor_sync(0xffffffffu, y.m, o), __shfl_xor_sync(0xffffffffu, y.l, o), __shfl_xor_sync(0xffffffffu, y.a, o)};
+      w = max_nan(w, __shfl_xor_sync(0xffffffffu, w, o));
+      y = merge(y, z);
+    }
+    if (lane == 0) s.sums = Sums{w, y.l, y.a};
+    if (k > 0) {
+      uint32_t key[kLpThreads / 32];
+#pragma unroll
+      for (int i = 0; i < kLpThreads / 32; ++i) key[i] = order_key(s.tmax[i * 32 + lane]);
+      // bit by bit from the top; fp16 and bf16 values leave the low bits of fp32 alike
+      constexpr int kBits = DT == SS_BF16 ? 16 : DT == SS_F16 ? 19 : 32;
+      uint32_t tau = 0;
+      for (int b = 31; b >= 32 - kBits; --b) {
+        const uint32_t trial = tau | 1u << b;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kLpThreads / 32; ++i) n += key[i] >= trial;
+        if ((int)__reduce_add_sync(0xffffffffu, (unsigned)n) >= k) tau = trial;
+      }
+      if (lane == 0) s.tau = tau;
+    }
+  }
+  __syncthreads();
+
+  // ---- candidates: elements that reach tau ----
+  if (k > 0) {
+    const uint32_t tau = s.tau;
+    auto offer = [&](float x, int i) {
+      const uint32_t key = order_key(x);
+      if (key >= tau) {
+        const int c = atomicAdd(&s.n_cand, 1);  // the order of arrival does not matter: they are ranked
+        if (c < kLpCap) {
+          s.key[c] = key;
+          s.idx[c] = i;
+        }
+      }
+    };
+    if (order_key(m) >= tau) s.hot[atomicAdd(&s.n_hot, 1)] = tid;
+    __syncthreads();
+    const int n_hot = s.n_hot, nv = (v1 - v0 + kLpThreads - 1) / kLpThreads;
+    if (n_hot * nv <= 8 * kLpThreads) {
+      for (int w = tid; w < n_hot * nv; w += kLpThreads) {
+        const int v = v0 + w / n_hot * kLpThreads + s.hot[w % n_hot];
+        if (v < v1) {
+          float x[E];
+          Vec<DT>::get(body[v], x);
+#pragma unroll
+          for (int i = 0; i < E; ++i) offer(x[i], head + v * E + i);
+        }
+      }
+      if (tid < n_ends) offer(end_x, end_at);
+    } else if (tid == 0) {
+      s.n_cand = kLpCap + 1;  // many equal maxima
+    }
+    __syncthreads();
+    if (s.n_cand <= kLpCap) {
+      if (tid == 0) s.n_top = min(k, s.n_cand);
+      rank_candidates(s.key, s.idx, s.n_cand, k, s.top_key, s.top_idx);
+    } else {
+      // Many elements reach tau: one after the other, each the first in order after the one before.
+      uint32_t pk = 0xffffffffu;
+      int pi = -1, got = 0;
+      for (int r = 0; r < k; ++r) {
+        uint32_t bk = 0;
+        int bi = 0x7fffffff;
+        auto look = [&](float x, int i) {
+          const uint32_t key = order_key(x);
+          if (before(pk, pi, key, i) && (bi == 0x7fffffff || before(key, i, bk, bi))) { bk = key; bi = i; }
+        };
+        for (int v = v0 + tid; v < v1; v += kLpThreads) {
+          float x[E];
+          Vec<DT>::get(body[v], x);
+#pragma unroll
+          for (int i = 0; i < E; ++i) look(x[i], head + v * E + i);
+        }
+        if (tid < n_ends) look(end_x, end_at);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint32_t k2 = __shfl_xor_sync(0xffffffffu, bk, o);
+          const int i2 = __shfl_xor_sync(0xffffffffu, bi, o);
+          if (i2 != 0x7fffffff && (bi == 0x7fffffff || before(k2, i2, bk, bi))) { bk = k2; bi = i2; }
+        }
+        __syncthreads();
+        if (lane == 0) { s.key[warp] = bk; s.idx[warp] = bi; }
+        __syncthreads();
+        bk = 0; bi = 0x7fffffff;
+        for (int w = 0; w < kLpWarps; ++w)
+          if (s.idx[w] != 0x7fffffff && (bi == 0x7fffffff || before(s.key[w], s.idx[w], bk, bi))) { bk = s.key[w]; bi = s.idx[w]; }
+        if (bi == 0x7fffffff) break;
+        pk = bk;
+        pi = bi;
+        if (tid == 0) { s.top_key[got] = bk; s.top_idx[got] = bi; }
+        ++got;
+      }
+      __syncthreads();
+      if (tid == 0) s.n_top = got;
+    }
+  } else if (tid == 0) {
+    s.n_top = 0;
+  }
+  __syncthreads();
+
+  // ---- join the parts of a row ----
+  Sums sum = s.sums;
+  int n_top = s.n_top;
+  const uint32_t* tk = s.top_key;
+  const int* ti = s.top_idx;
+  if (split > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (part == 0) {
+      int n = 0;
+      for (int c = 0; c < split; ++c) {
+        const LpShared* o = cluster.map_shared_rank(&s, c);
+        const int oc = o->n_top;
+        for (int i = tid; i < oc; i += kLpThreads) {
+          s.key[n + i] = o->top_key[i];
+          s.idx[n + i] = o->top_idx[i];
+        }
+        n += oc;
+        if (c > 0) {
+          const Sums y = o->sums;
+          const float w = max_nan(sum.m, y.m);
+          sum = merge(sum, y);
+          sum.m = w;
+        }
+      }
+      __syncthreads();
+      // the places 8 * 32 .. of the lists are free
+      rank_candidates(s.key, s.idx, n, k, s.key + kLpMaxSplit * kLpMaxTop, s.idx + kLpMaxSplit * kLpMaxTop);
+      __syncthreads();
+      tk = s.key + kLpMaxSplit * kLpMaxTop;
+      ti = s.idx + kLpMaxSplit * kLpMaxTop;
+      n_top = min(n, k);
+    }
+    cluster.sync();  // nobody leaves while its shared memory is read
+    if (part != 0) return;
+  }
+
+  const bool bad = !(sum.m < INFINITY), none = sum.m == -INFINITY;
+  const float nan = __int_as_float(0x7fffffff);
+  const float ll = logf(sum.l);
+  auto lp = [&](float x) { return bad ? nan : none ? -INFINITY : (x - sum.m) - ll; };
+  if (tid < k) {
+    const bool has = tid < n_top;
+    const uint32_t u = has ? tk[tid] : 0u;
+    const float x = __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+    p.top_ids[row * k + tid] = bad || !has ? -1 : ti[tid];
+    p.top_lp[row * k + tid] = bad ? nan : has ? lp(x) : -INFINITY;
+  }
+  if (tid == kLpThreads - 1) {
+    const int64_t tg = p.targets ? p.targets[row] : -1;
+    p.logprobs[row] = tg < 0 ? 0.f : tg >= p.vocab ? nan : lp(load_as_f32(base, DT, tg));
+    p.entropy[row] = bad ? nan : none ? 0.f : ll - sum.a / sum.l;
+  }
+}
+
+// CTAs for a row: the split whose waves of CTAs (two an SM) take least, at about 22 GB/s a CTA
+// and 3 us for what a CTA does after its pass.
+int lp_split(int64_t rows, int64_t row_bytes) {
+  const int64_t slots = 2LL * sm_count();
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= kLpMaxSplit; s *= 2) {
+    const double waves = (double)((rows * s + slots - 1) / slots);
+    const double t = waves * ((double)row_bytes / s / 22e3 + 3.0);
+    if (s == 1 || t < least) { least = t; best = s; }
+  }
+  return best;
+}
+
+template <int DT>
+int launch_logprobs(const LpParams& p, int split, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.rows * split));
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<DT>, p, split);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SS_ERR_CUDA, std::string("ss_token_logprobs: ") + cudaGetErrorString(e));
+  }
+  return check_launch("ss_token_logprobs");
 }
 
 }  // namespace
@@ -135,13 +448,13 @@ extern "C" int ss_token_logprobs(const void* logits, int dtype, int64_t rows, in
     SS_REQUIRE(vocab >= 1, "ss_token_logprobs: empty vocabulary");
     SS_REQUIRE(top >= 0 && top <= kLpMaxTop, "ss_token_logprobs: top must be in [0, 32]");
     SS_REQUIRE(top == 0 || (top_ids && top_logprobs), "ss_token_logprobs: null pointer");
-    SS_REQUIRE(rows <= 0x7fffffff, "ss_token_logprobs: too many rows");
+    SS_REQUIRE(rows <= 0x7fffffff / kLpMaxSplit, "ss_token_logprobs: too many rows");
     count_dispatch("ss_token_logprobs");
     LpParams p{logits, rows, row_stride, vocab, targets, top, logprobs, entropy, top_logprobs, top_ids};
     cudaStream_t st = as_stream(stream);
-    if (dtype == SS_F32) logprobs_kernel<SS_F32><<<(unsigned)rows, kLpThreads, 0, st>>>(p);
-    else if (dtype == SS_F16) logprobs_kernel<SS_F16><<<(unsigned)rows, kLpThreads, 0, st>>>(p);
-    else logprobs_kernel<SS_BF16><<<(unsigned)rows, kLpThreads, 0, st>>>(p);
-    return check_launch("ss_token_logprobs");
+    const int split = lp_split(rows, (int64_t)vocab * (dtype == SS_F32 ? 4 : 2));
+    if (dtype == SS_F32) return launch_logprobs<SS_F32>(p, split, st);
+    if (dtype == SS_F16) return launch_logprobs<SS_F16>(p, split, st);
+    return launch_logprobs<SS_BF16>(p, split, st);
   });
 }
