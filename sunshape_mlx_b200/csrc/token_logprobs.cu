@@ -13,11 +13,18 @@
 //
 // One pass over a row, by a CTA or, for few rows, by a cluster whose first
 // CTA joins the others' results out of their shared memory. A thread keeps
-// (M, l, A) of its own elements in fp32 and rescales only when 32 new ones
+// (M, l, A) of its own elements in fp32 and rescales only when 16 new ones
 // raise its maximum. The k-th largest of the threads' maxima bounds the k-th
 // largest element from below, so only the few threads whose maximum reaches it
 // hold candidates: their elements alone are read again (3 % of a row at k =
-// 20), by all threads together, and ranked against each other.
+// 8), by all threads together, and ranked against each other. Where more
+// elements reach the bound than are listed (a constant row), those above it are
+// listed and the first equal ones taken in order.
+//
+// Bound by HBM; an element costs about 5.5 issue slots, one of them exp2, at
+// half of what an SM can issue at full bandwidth. 256 threads and five CTAs an
+// SM, so that rows in their last phase overlap rows that stream: 2047 x 128256
+// bf16, top 8: 109 us (4.8 TB/s), 112 us with 512 threads and two CTAs.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -27,12 +34,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxSplit = 8;
-constexpr int kLpCap = 1024;     // candidates of a CTA; more (many equal logits) take the ordered path
-constexpr int kLpVecs = 4;       // 16-byte loads of a thread in flight
+constexpr int kLpCap = 1024;     // candidates of a CTA
+constexpr int kLpVecs = 2;       // 16-byte loads of a thread in flight
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -1e30f;   // stands for -inf in differences: its exponential is 0, times it is 0
 
@@ -143,7 +150,7 @@ struct LpShared {
   int top_idx[kLpMaxTop];
   uint32_t tau;
   int hot[kLpThreads];
-  int n_hot, n_cand, n_top, base;
+  int n_hot, n_cand, n_top;
   int wsum[kLpWarps];
 };
 
@@ -153,7 +160,8 @@ __device__ __forceinline__ void rank_candidates(const uint32_t* key, const int* 
     const uint32_t kc = key[c];
     const int ic = idx[c];
     int r = 0;
-    for (int j = 0; j < n && r < k; ++j) r += before(key[j], idx[j], kc, ic);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) r += before(key[j], idx[j], kc, ic);
     if (r < k) {
       dk[r] = kc;
       di[r] = ic;
@@ -162,8 +170,10 @@ __device__ __forceinline__ void rank_candidates(const uint32_t* key, const int* 
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const __grid_constant__ LpParams p, int split) {
+__global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_constant__ LpParams p, int split) {
   constexpr int E = Vec<DT>::E;
+  constexpr int kBits = DT == SS_BF16 ? 16 : DT == SS_F16 ? 19 : 32;  // of the fp32 key that tell two values apart
+  constexpr uint32_t kMask = 0xffffffffu << (32 - kBits);
   __shared__ LpShared s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / split;
@@ -252,7 +262,6 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const __grid_co
 #pragma unroll
       for (int i = 0; i < kLpThreads / 32; ++i) key[i] = order_key(s.tmax[i * 32 + lane]);
       // bit by bit from the top; fp16 and bf16 values leave the low bits of fp32 alike
-      constexpr int kBits = DT == SS_BF16 ? 16 : DT == SS_F16 ? 19 : 32;
       uint32_t tau = 0;
       for (int b = 31; b >= 32 - kBits; --b) {
         const uint32_t trial = tau | 1u << b;
@@ -282,7 +291,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const __grid_co
     if (order_key(m) >= tau) s.hot[atomicAdd(&s.n_hot, 1)] = tid;
     __syncthreads();
     const int n_hot = s.n_hot, nv = (v1 - v0 + kLpThreads - 1) / kLpThreads;
-    if (n_hot * nv <= 8 * kLpThreads) {
+    if (n_hot * nv <= 4096) {
       for (int w = tid; w < n_hot * nv; w += kLpThreads) {
         const int v = v0 + w / n_hot * kLpThreads + s.hot[w % n_hot];
         if (v < v1) {
@@ -297,11 +306,90 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const __grid_co
       s.n_cand = kLpCap + 1;  // many equal maxima
     }
     __syncthreads();
-    if (s.n_cand <= kLpCap) {
+    bool listed = s.n_cand <= kLpCap;
+    if (!listed) {
+      // Many elements equal tau (a constant row, a mask): list those above it, which at most k - 1
+      // threads hold, and take the first equal ones in the order of their indices.
+      __syncthreads();
+      if (tid == 0) s.n_hot = s.n_cand = 0;
+      __syncthreads();
+      auto above = [&](float x) { return (order_key(x) & kMask) > tau; };
+      if (above(m)) s.hot[atomicAdd(&s.n_hot, 1)] = tid;
+      __syncthreads();
+      const int n_above = s.n_hot;
+      auto list = [&](float x, int i) {
+        if (above(x)) {
+          const int c = atomicAdd(&s.n_cand, 1);
+          if (c < kLpCap) {
+            s.key[c] = order_key(x);
+            s.idx[c] = i;
+          }
+        }
+      };
+      for (int w = tid; w < n_above * nv; w += kLpThreads) {
+        const int v = v0 + w / n_above * kLpThreads + s.hot[w % n_above];
+        if (v < v1) {
+          float x[E];
+          Vec<DT>::get(body[v], x);
+#pragma unroll
+          for (int i = 0; i < E; ++i) list(x[i], head + v * E + i);
+        }
+      }
+      if (tid < n_ends) list(end_x, end_at);
+      __syncthreads();
+      listed = s.n_cand + k <= kLpCap;
+      int have = s.n_cand;
+      // steps in the order of the indices: the row's head, the vectors, the row's tail
+      for (int st = -1; listed && st <= nv && have < k; ++st) {
+        float x[E];
+        int at = 0, n = 0;  // this thread's elements of the step: at, at + 1, ...
+        if (st < 0 || st == nv) {
+          n = tid < n_ends && (tid < head) == (st < 0) ? 1 : 0;
+          at = end_at;
+          x[0] = end_x;
+        } else if (v0 + st * kLpThreads + tid < v1) {
+          const int v = v0 + st * kLpThreads + tid;
+          Vec<DT>::get(body[v], x);
+          at = head + v * E;
+          n = E;
+        }
+        int eq = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) eq |= (i < n && (order_key(x[i]) & kMask) == tau ? 1 : 0) << i;
+        int inc = __popc(eq);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += y;
+        }
+        if (lane == 31) s.wsum[warp] = inc;
+        __syncthreads();
+        int at_rank = have + inc - __popc(eq), total = 0;
+        for (int w = 0; w < kLpWarps; ++w) {
+          if (w < warp) at_rank += s.wsum[w];
+          total += s.wsum[w];
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          if (eq >> i & 1) {
+            if (at_rank < k) {
+              s.key[at_rank] = order_key(x[i]);
+              s.idx[at_rank] = at + i;
+            }
+            ++at_rank;
+          }
+        }
+        have += total;
+        __syncthreads();
+      }
+      if (listed && tid == 0) s.n_cand = max(s.n_cand, min(have, k));
+      __syncthreads();
+    }
+    if (listed) {
       if (tid == 0) s.n_top = min(k, s.n_cand);
       rank_candidates(s.key, s.idx, s.n_cand, k, s.top_key, s.top_idx);
     } else {
-      // Many elements reach tau: one after the other, each the first in order after the one before.
+      // Many elements above tau too: one after the other, each the first in order after the one before.
       uint32_t pk = 0xffffffffu;
       int pi = -1, got = 0;
       for (int r = 0; r < k; ++r) {
@@ -399,15 +487,15 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const __grid_co
   }
 }
 
-// CTAs for a row: the split whose waves of CTAs (two an SM) take least, at about 22 GB/s a CTA
+// CTAs for a row: the split whose waves of CTAs (five an SM) take least, at about 9 GB/s a CTA
 // and 3 us for what a CTA does after its pass.
 int lp_split(int64_t rows, int64_t row_bytes) {
-  const int64_t slots = 2LL * sm_count();
+  const int64_t slots = 5LL * sm_count();
   int best = 1;
   double least = 0;
   for (int s = 1; s <= kLpMaxSplit; s *= 2) {
     const double waves = (double)((rows * s + slots - 1) / slots);
-    const double t = waves * ((double)row_bytes / s / 22e3 + 3.0);
+    const double t = waves * ((double)row_bytes / s / 9e3 + 3.0);
     if (s == 1 || t < least) { least = t; best = s; }
   }
   return best;
