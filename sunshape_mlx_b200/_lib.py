@@ -206,7 +206,7 @@ def _attach_error_sink(lib) -> None:
 
 
 WAIT_CODES = {1: "decode producer stage wait", 2: "decode copy drain", 4: "decode tile wait",
-              8: "decode table wait", 16: "tensor-core assignment pipeline wait"}
+              8: "decode table wait", 16: "tensor-core assignment pipeline wait", 32: "int4_attention tile wait"}
 
 
 def poll_device_errors() -> None:

@@ -34,40 +34,13 @@
 //   the output's); for up to 4 rows lo uses the columns that are free anyway.
 // The softmax reference of a row moves only when a logit exceeds it by 2^8:
 // the usual block needs one vote and no shuffles.
-#include "int4_pages.cuh"
+#include "int4_attn.cuh"
 
 namespace ss {
 namespace {
 
-struct AttnParams {
-  const void* q;
-  int dtype, q_vec;  // q_vec: rows of q are 16-byte aligned
-  int64_t q_st, q_sh;
-  int64_t n_tokens;
-  int hq, hkv, grp;
-  const uint8_t* pages;
-  int n_pages;
-  int64_t page_stride, head_stride;
-  int page, page_blocks;  // tokens and blocks of a page
-  uint32_t page_inv;      // 2^32 / page_blocks, rounded up
-  const int32_t* table;
-  int64_t table_stride;
-  int width;
-  const int32_t *seq_lens, *cu_q;
-  int n;
-  float scale;
-  int causal, window;
-  void* out;
-  float* lse;
-  uint8_t* ws;
-  int n_slots;  // CTAs the workspace was sized for
-};
-
 constexpr int kSegCost = 48;     // blocks' worth of time that the ends of a unit take
 constexpr int kMinCost = 96;     // a range is not cut below this many blocks' worth
-constexpr float kLow = -1e30f;   // softmax reference before any key
-constexpr float kSlack = 8.f;    // a logit may exceed the reference by this (base 2)
-constexpr float kLog2e = 1.4426950408889634f;
 
 // Modes: query rows of a unit, and whether probabilities are hi + lo.
 enum { kRows4, kRows8, kRows8Lo, kRows16, kRows16Lo };
@@ -86,23 +59,6 @@ struct Shape {
   static constexpr int kMerge = W * R * (D + 4) * 4;  // rows padded by 4 floats
   static constexpr int kSmem = kRing + kMerge + 2 * W * R * 4 + (W * 32 + 1) * 8;
 };
-
-// What a request contributes to the schedule.
-struct Req {
-  int nq, len, rbs, blk0, nblk;  // query rows' tokens, keys, row blocks, first key block, key blocks (>= 1)
-};
-
-template <int R>
-__device__ __forceinline__ Req load_req(const AttnParams& p, int b) {
-  Req r;
-  const int c0 = max(p.cu_q[b], 0);
-  r.nq = max(p.cu_q[b + 1] - c0, 0);
-  r.len = min(max(p.seq_lens[b], 0), p.width * p.page);
-  r.rbs = (int)(((int64_t)r.nq * p.grp + R - 1) / R);
-  r.blk0 = p.window > 0 ? max(0, r.len - r.nq - p.window + 1) / kBlkTokens : 0;
-  r.nblk = max(1, (r.len + kBlkTokens - 1) / kBlkTokens - r.blk0);
-  return r;
-}
 
 // One CTA's walk over its range: unit after unit.
 template <int R>
@@ -130,26 +86,6 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ uint32_t lop_or(uint32_t x, uint32_t mask, uint32_t magic) {
-  uint32_t r;  // (x & mask) | magic
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(magic));
-  return r;
-}
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // D(16x8) += A(16x16) B(16x8) as mma_16816, free to be scheduled among independent ones.
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -162,32 +98,11 @@ __device__ __forceinline__ void mma0(float* d, uint32_t a0, uint32_t a1, uint32_
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ float lo_h(uint32_t x) { return __low2float(*reinterpret_cast<__half2*>(&x)); }
-__device__ __forceinline__ float hi_h(uint32_t x) { return __high2float(*reinterpret_cast<__half2*>(&x)); }
-
-// Page of a request's block k, and the block's place in it.
-__device__ __forceinline__ int page_of(const AttnParams& p, int k, int& in_page) {
-  if (p.page_blocks == 1) {
-    in_page = 0;
-    return k;
-  }
-  int q = (int)__umulhi((uint32_t)k, p.page_inv);  // k / page_blocks, or one more
-  int r = k - q * p.page_blocks;
-  if (r < 0) { --q; r += p.page_blocks; }
-  in_page = r;
-  return q;
-}
-
 template <int N>
 __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&v)[N]) {
   if constexpr (N == 2) {
@@ -868,7 +783,12 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.ws = static_cast<uint8_t*>(a->workspace); p.n_slots = 0;
     const int64_t most = (int64_t)a->max_q * p.grp;
     const int rows = most > 16 ? 16 : (int)most;
+    p.tiles = most > 16 && a->d != 256;
+    p.sink = error_sink();
     cudaStream_t st = as_stream(stream);
+    if (p.tiles) {
+      if (int rc = launch_tiles(p, a->d, st)) return rc;
+    }
     return a->d == 64 ? launch_mode<64>(p, rows, st) : a->d == 128 ? launch_mode<128>(p, rows, st) : launch_mode<256>(p, rows, st);
   });
 }

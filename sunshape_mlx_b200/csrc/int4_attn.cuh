@@ -1,0 +1,110 @@
+// What the two kernels of int4_attention share: the call's parameters, which
+// requests go to which kernel, and fp16 pair arithmetic on 4-bit codes.
+#pragma once
+
+#include "int4_pages.cuh"
+
+namespace ss {
+
+struct AttnParams {
+  const void* q;
+  int dtype, q_vec;  // q_vec: rows of q are 16-byte aligned
+  int64_t q_st, q_sh;
+  int64_t n_tokens;
+  int hq, hkv, grp;
+  const uint8_t* pages;
+  int n_pages;
+  int64_t page_stride, head_stride;
+  int page, page_blocks;  // tokens and blocks of a page
+  uint32_t page_inv;      // 2^32 / page_blocks, rounded up
+  const int32_t* table;
+  int64_t table_stride;
+  int width;
+  const int32_t *seq_lens, *cu_q;
+  int n;
+  float scale;
+  int causal, window;
+  void* out;
+  float* lse;
+  uint8_t* ws;
+  int n_slots;  // CTAs of the warp-MMA kernel
+  int tiles;    // the tile kernel runs too
+  int* sink;    // process error sink (host word) or null
+};
+
+constexpr float kLow = -1e30f;   // softmax reference before any key
+constexpr float kSlack = 8.f;    // a logit may exceed the reference by this (base 2)
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Rows (query tokens times heads of a group) from which a request's queries go to the tiles of
+// 128 rows of the tcgen05 kernel instead of the 16-row units of the warp-MMA kernel. A tile is a
+// CTA's work alone, the units of a request are spread over all SMs: the tiles win once about nine
+// CTAs' worth of full tiles run at once.
+__device__ __forceinline__ bool to_tiles(const AttnParams& p, int nq) {
+  const int64_t rows = (int64_t)nq * p.grp;
+  return p.tiles && rows > 16 && rows * p.hkv >= 1152;
+}
+
+// What a request contributes to the schedule of the warp-MMA kernel.
+struct Req {
+  int nq, len, rbs, blk0, nblk;  // query rows' tokens, keys, row blocks, first key block, key blocks (>= 1)
+};
+
+template <int R>
+__device__ __forceinline__ Req load_req(const AttnParams& p, int b) {
+  Req r;
+  const int c0 = max(p.cu_q[b], 0);
+  r.nq = max(p.cu_q[b + 1] - c0, 0);
+  r.len = min(max(p.seq_lens[b], 0), p.width * p.page);
+  r.rbs = to_tiles(p, r.nq) ? 0 : (int)(((int64_t)r.nq * p.grp + R - 1) / R);
+  r.blk0 = p.window > 0 ? max(0, r.len - r.nq - p.window + 1) / kBlkTokens : 0;
+  r.nblk = max(1, (r.len + kBlkTokens - 1) / kBlkTokens - r.blk0);
+  return r;
+}
+
+// Page of a request's block k, and the block's place in it.
+__device__ __forceinline__ int page_of(const AttnParams& p, int k, int& in_page) {
+  if (p.page_blocks == 1) {
+    in_page = 0;
+    return k;
+  }
+  int q = (int)__umulhi((uint32_t)k, p.page_inv);  // k / page_blocks, or one more
+  int r = k - q * p.page_blocks;
+  if (r < 0) { --q; r += p.page_blocks; }
+  in_page = r;
+  return q;
+}
+
+__device__ __forceinline__ uint32_t lop_or(uint32_t x, uint32_t mask, uint32_t magic) {
+  uint32_t r;  // (x & mask) | magic
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(magic));
+  return r;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float lo_h(uint32_t x) { return __low2float(*reinterpret_cast<__half2*>(&x)); }
+__device__ __forceinline__ float hi_h(uint32_t x) { return __high2float(*reinterpret_cast<__half2*>(&x)); }
+
+
+// The requests of a batch that have query rows for the tiles, see int4_prompt.cu.
+int launch_tiles(AttnParams& p, int d, cudaStream_t st);
+
+}  // namespace ss

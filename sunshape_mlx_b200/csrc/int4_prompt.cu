@@ -1,0 +1,573 @@
+// Attention of many query rows over 4-bit KV pages on the 5th-generation
+// tensor cores (tcgen05): the tile kernel of int4_attention.
+//
+// A unit is (request, kv-head, 128 query rows); the rows of a group's heads and
+// of consecutive tokens share a tile, so keys and values are decoded once for
+// // all of them. CTAs (one an SM) take units in turn, those with most keys of a
+// request first. Per tile of 64 tokens: Per tile of 64 tokens:
+//   decode   (8 warps)  codes -> fp16 operands in shared memory
+//   S = Q K^T (1 thread) M = 128, N = 64, fp32 in TMEM, two buffers
+//   softmax  (4 warps)  a thread per row, P as fp16 in shared memory
+//   O += P V (same thread) M = 128, N = D, fp32 in TMEM
+// and the four run on different tiles at the same time, handing over through
+// mbarriers (two stages of keys and values, two S and P buffers).
+//
+// Keys enter exactly: c s is the pair of fp16 values hi = fp16(c s) and
+// lo = c s - hi (15 bits in all, so lo is exact), and q . z is one more K step
+// of 16, z as stored against the row's group sums in two fp16 terms. One
+// rounded fp16 key would move a logit by 3e-4, which rows with few keys show
+// in their log-sum-exp; the second product costs 136 / 264 of the tensor time
+// of a tile. s enters halved: 15 s can be one place above fp16's largest.
+// Values are fp16(c s + z), probabilities fp16, or hi + lo (a second pass of
+// P V) where the output is fp16 and the rounding would show. Row statistics
+// and both products accumulate in fp32. O in TMEM is rescaled only when a row's
+// logits exceed its reference by 2^8.
+//
+// Every wait is bounded (2 s) and reports through the process error sink.
+#include "int4_attn.cuh"
+#include "tcgen05.cuh"
+
+namespace ss {
+namespace {
+
+constexpr int kTileRows = 128, kTileKeys = 64;
+constexpr int kSoftWarps = 4, kDecWarps = 8, kMmaWarp = kSoftWarps + kDecWarps;
+constexpr int kTileThreads = (kMmaWarp + 1) * 32;
+constexpr uint64_t kTileWaitNs = 2000000000ull;
+constexpr int kTileWaitCode = 32;
+
+template <int D>
+struct Tile {
+  static constexpr int kQ = (D / 8 + 2) * 2048;     // [dim chunk, then 2 of group sums][row] 16 bytes
+  static constexpr int kChunk = kTileKeys * 16 + 32;  // a dim chunk of keys; + 32: no bank conflicts
+  static constexpr int kKey = D / 8 * kChunk;       // hi; lo behind it
+  static constexpr int kZ = 2 * kTileKeys * 16;     // zeros, twice
+  static constexpr int kVal = kTileKeys * D * 2;    // [8 tokens][dim chunk][token] 16 bytes
+  static constexpr int kStage = 2 * kKey + kZ + kVal;
+  static constexpr int kProb = kTileRows * kTileKeys * 2;  // [8 tokens][row] 16 bytes
+  static constexpr int kOffStage = kQ, kOffProb = kQ + 2 * kStage, kOffMisc = kOffProb + 2 * kProb;
+  static constexpr int kSmem = kOffMisc + 512 + kTileThreads * 4;
+};
+
+__device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {  // fp16 in, fp32 out, M = 128
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+}
+// 32 columns of this thread's TMEM lane, fp32.
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A unit: its rows, and the key tiles [kt0, kt1) that any of them sees.
+struct Unit {
+  int b, h, row0, rows, nq, len, tok0, kt0, kt1, all0, all1;  // rows see the keys [all0, all1) whole
+};
+
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
+  const int nq = max(p.cu_q[b + 1] - max(p.cu_q[b], 0), 0);
+  return to_tiles(p, nq) ? (int)(((int64_t)nq * p.grp + kTileRows - 1) / kTileRows) : 0;
+}
+// Keys [beg, end) that the row of query token i sees.
+__device__ __forceinline__ void row_keys(const AttnParams& p, int nq, int len, int i, int& beg, int& end) {
+  const int pos = len - nq + i;
+  end = p.causal ? max(0, min(len, pos + 1)) : len;
+  beg = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+}
+
+template <int D, bool LO>
+__global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid_constant__ AttnParams p) {
+  using B = Int4Blk<D>;
+  using T = Tile<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* s_q = smem;
+  uint8_t* s_prob = smem + T::kOffProb;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kOffMisc);
+  uint64_t* kv_full = bars;        // [2] the 8 decode warps
+  uint64_t* kv_empty = bars + 2;   // [2] P V of the stage's tile is done
+  uint64_t* s_full = bars + 4;     // [2] Q K^T is done
+  uint64_t* s_empty = bars + 6;    // [2] the 4 softmax warps have read S
+  uint64_t* p_full = bars + 8;     // [2] the 4 softmax warps have written P
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 14);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [2][4] blocks of a stage without a page
+  int* s_sum = reinterpret_cast<int*>(smem + T::kOffMisc + 256);      // [13] warps' units
+  int* s_cum = reinterpret_cast<int*>(smem + T::kOffMisc + 512);      // [threads] units before a thread's requests
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  // ---- setup ---------------------------------------------------------------
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(kv_full + s, kDecWarps);
+      mbar_init(kv_empty + s, 1);
+      mbar_init(s_full + s, 1);
+      mbar_init(s_empty + s, kSoftWarps);
+      mbar_init(p_full + s, kSoftWarps);
+    }
+    mbar_init(bars + 12, 1);  // end of an abandoned unit's MMAs
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tc_alloc(s_tmem, 256);
+    tc_relinquish();
+  }
+  const int per = (p.n + kTileThreads - 1) / kTileThreads;
+  const int b0 = min(p.n, tid * per), b1 = min(p.n, b0 + per);
+  int units = 0;
+  for (int b = b0; b < b1; ++b) units += tiles_of(p, b) * p.hkv;
+  int inc = units;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) s_sum[warp] = inc;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int total = 0, before = 0;
+  for (int w = 0; w <= kMmaWarp; ++w) {
+    if (w == warp) before = total;
+    total += s_sum[w];
+  }
+  s_cum[tid] = before + inc - units;
+  __syncthreads();
+  const uint32_t tmem = *s_tmem;
+  const uint32_t t_o = tmem + 2 * kTileKeys;
+
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+      if (mbar_try_wait(bar, parity)) return true;
+      if (*s_abort) return false;
+      if (global_ns() - t0 > kTileWaitNs) {
+        if (!*s_abort) report_wait_failure(nullptr, p.sink, kTileWaitCode);
+        *s_abort = 1;
+        return false;
+      }
+    }
+  };
+
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+  // ---- unit after unit -------------------------------------------------------
+  uint32_t n0 = 0;  // tiles of this CTA's earlier units: the barriers' phases go on
+  for (int round = 0;; ++round) {
+    // longest first within a request, rounds in alternating direction: nearly equal sums
+    const int u = round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if (round * (int64_t)gridDim.x >= total || *s_abort) break;
+    if (u >= total) continue;
+    Unit un;
+    {
+      int a = 0, e = kTileThreads;
+      while (e - a > 1) {
+        const int mid = (a + e) >> 1;
+        if (s_cum[mid] <= u) a = mid; else e = mid;
+      }
+      int at = s_cum[a], b = a * per, nt = 0;
+      for (;; ++b) {
+        nt = tiles_of(p, b);
+        if (at + nt * p.hkv > u) break;
+        at += nt * p.hkv;
+      }
+      const int qt = nt - 1 - (u - at) / p.hkv;  // the last rows of a causal request see most keys
+      un.b = b;
+      un.h = (u - at) % p.hkv;
+      un.tok0 = max(p.cu_q[b], 0);
+      un.nq = max(p.cu_q[b + 1] - un.tok0, 0);
+      un.len = min(max(p.seq_lens[b], 0), p.width * p.page);
+      un.row0 = qt * kTileRows;
+      un.rows = (int)min((int64_t)kTileRows, (int64_t)un.nq * p.grp - un.row0);
+      int beg0, end0, beg1, end1;
+      row_keys(p, un.nq, un.len, un.row0 / p.grp, beg0, end0);
+      row_keys(p, un.nq, un.len, (un.row0 + un.rows - 1) / p.grp, beg1, end1);
+      un.kt0 = beg0 / kTileKeys;
+      un.kt1 = max(un.kt0, (end1 + kTileKeys - 1) / kTileKeys);
+      if (end1 <= beg0) un.kt1 = un.kt0;
+      un.all0 = beg1;
+      un.all1 = end0;
+    }
+    const int nt = un.kt1 - un.kt0;
+
+    if (warp < kSoftWarps) {
+      // ================= softmax: a thread per row ==============================
+      const int r = tid, rr = un.row0 + r, i = rr / p.grp, hd = un.h * p.grp + rr % p.grp;
+      const int64_t tok = un.tok0 + (int64_t)i;
+      const bool live = r < un.rows && tok < p.n_tokens;
+      const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+      float fac;
+      {  // the row's queries, scaled by a power of two into [256, 512), and its group sums
+        uint4 x[D / 8];
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + tok * p.q_st + hd * p.q_sh;
+        float big = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint32_t w[4] = {0u, 0u, 0u, 0u};
+          if (live) {
+            if (p.q_vec) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(qp) + c);
+              w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = qp[c * 8 + 2 * e] | (uint32_t)qp[c * 8 + 2 * e + 1] << 16;
+            }
+          }
+          x[c] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16);
+            const float b = p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u);
+            big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
+          }
+        }
+        int ex = 0;
+        if (big > 0.f && big < INFINITY) ex = 135 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
+        const float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
+        uint8_t* dst = s_q + (r >> 3) * 128 + (r & 7) * 16;
+        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+        static_assert(B::G <= 8, "group sums fill one chunk");
+        float sum[B::G];
+#pragma unroll
+        for (int g = 0; g < B::G; ++g) sum[g] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[2 * e] = (p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16)) * up;
+            f[2 * e + 1] = (p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u)) * up;
+          }
+          uint32_t o[4];  // dims (e, e + 4) side by side, as the key words' nibbles come
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[e] = pack_h2(f[e], f[e + 4]);
+            sum[c / 4] += lo_h(o[e]) + hi_h(o[e]);
+          }
+          *reinterpret_cast<uint4*>(dst + c * 2048) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+#pragma unroll
+        for (int g = 0; g < B::G; g += 2) {  // halved, as the keys are
+          const float a = 0.5f * sum[g], b = 0.5f * sum[g + 1];
+          hi[g / 2] = pack_h2(a, b);
+          lo[g / 2] = pack_h2(a - lo_h(hi[g / 2]), b - hi_h(hi[g / 2]));
+        }
+        *reinterpret_cast<uint4*>(dst + (D / 8) * 2048) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + (D / 8 + 1) * 2048) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        fac = 2.f * p.scale * kLog2e / up;
+        fence_proxy_async_smem();
+      }
+      named_bar_sync(1, (kSoftWarps + 1) * 32);  // the MMA warp may read Q
+
+      int beg = 0, end = 0;
+      if (r < un.rows) row_keys(p, un.nq, un.len, i, beg, end);
+      float m = kLow, l0 = 0.f, l1 = 0.f;
+      bool ok = true;
+      for (int j = 0; j < nt; ++j) {
+        const uint32_t n = n0 + j, buf = n & 1, ph = (n >> 1) & 1;
+        if (!(ok = warp_wait(s_full + buf, ph))) break;
+        tc_fence_after();
+        float y[kTileKeys];
+#pragma unroll
+        for (int c = 0; c < kTileKeys; c += 32) {
+          uint32_t v[32];
+          tc_ld32(tmem + lane_base + buf * kTileKeys + c, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[c + e] = __uint_as_float(v[e]);
+        }
+        const uint32_t hid = *reinterpret_cast<volatile uint32_t*>(s_hidden + buf * 4);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty + buf);
+
+        const int t0 = (un.kt0 + j) * kTileKeys;
+#pragma unroll
+        for (int e = 0; e < kTileKeys; e += 2) mul_f32x2(y[e], y[e + 1], fac);
+        if (t0 < un.all0 || t0 + kTileKeys > un.all1 || hid != 0) {
+#pragma unroll
+          for (int e = 0; e < kTileKeys; ++e)
+            if (t0 + e >= end || t0 + e < beg || (hid >> (e / 16 * 8) & 1)) y[e] = -INFINITY;
+        }
+        float top = y[0];
+#pragma unroll
+        for (int e = 0; e < kTileKeys; e += 2) top = fmax3(top, y[e], y[e + 1]);
+        if (__any_sync(0xffffffffu, top > m + kSlack)) {
+          const float mn = fmaxf(m, top), f = ex2(m - mn);
+          m = mn;
+          l0 *= f;
+          l1 *= f;
+          if (j > 0) {  // O holds the tiles before: all of them, once the last one's P V is done
+            if (!(ok = warp_wait(kv_empty + (buf ^ 1), ((n - 1) >> 1) & 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              tc_ld32(t_o + lane_base + c, v);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              tc_st32(t_o + lane_base + c, v);
+            }
+            tc_wait_st();
+            tc_fence_before();
+          }
+        }
+        // the P buffer is free once P V of the tile two before (one buffer with lo: one before) is done
+        if (!LO) ok = warp_wait(kv_empty + buf, ph ^ 1);
+        else if (j > 0) ok = warp_wait(kv_empty + (buf ^ 1), ((n - 1) >> 1) & 1);
+        if (!ok) break;
+        uint8_t* dst = s_prob + (LO ? 0 : buf * T::kProb) + (r >> 3) * 128 + (r & 7) * 16;
+#pragma unroll
+        for (int c = 0; c < kTileKeys / 8; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float& a = y[c * 8 + 2 * e];
+            float& b = y[c * 8 + 2 * e + 1];
+            add_f32x2(a, b, -m, -m);
+            a = ex2(a);
+            b = ex2(b);
+            add_f32x2(l0, l1, a, b);
+            w[e] = pack_h2(a, b);
+          }
+          *reinterpret_cast<uint4*>(dst + c * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
+          if constexpr (LO) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_h2(y[c * 8 + 2 * e] - lo_h(w[e]), y[c * 8 + 2 * e + 1] - hi_h(w[e]));
+            *reinterpret_cast<uint4*>(dst + T::kProb + c * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + buf);
+      }
+      // ---- output ----
+      const float l = l0 + l1;
+      if (ok && nt > 0) ok = warp_wait(kv_empty + ((n0 + nt - 1) & 1), ((n0 + nt - 1) >> 1) & 1);
+      if (ok) {
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (tok * p.hq + hd) * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          if (nt > 0) {
+            tc_ld32(t_o + lane_base + c, v);
+            tc_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
+          if (live) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {  // columns of a chunk: dims 0, 4, 1, 5, 2, 6, 3, 7
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e / 2 + e % 2 * 4] = __uint_as_float(v[x * 8 + e]) * inv;
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (p.dtype == SS_F16) {
+                  w[e] = pack_h2(f[2 * e], f[2 * e + 1]);
+                } else {
+                  __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+                  w[e] = *reinterpret_cast<uint32_t*>(&b);
+                }
+              }
+              *reinterpret_cast<uint4*>(out + c + x * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (live && p.lse) p.lse[tok * p.hq + hd] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+        tc_fence_before();
+      }
+    } else if (warp < kMmaWarp) {
+      // ================= decode: 64 threads per block of 16 tokens ==============
+      const int d = tid - kSoftWarps * 32, bi = d >> 6, piece = d & 63;
+      constexpr int N = B::N, VW = 2 * B::W;          // key words and value words of a thread
+      static_assert(B::G == N, "one key piece per token and lane");
+      const int ktok = piece >> 2, kj = piece & 3;    // key piece: a token's words 4 g + kj
+      const int vhi = D == 128 ? piece >> 5 : piece & 1, vl = D == 128 ? piece & 31 : piece >> 1;
+      const int vi = vl >> 2, vj = vl & 3;            // value piece: tokens 8 vhi + 2 vj, + 1; words W vi ..
+      uint32_t kw[N], ks[N], vw[VW], vs[2];
+      bool there = false;
+      auto load = [&](int j) {  // this thread's pieces of the unit's tile j
+        const int k = (un.kt0 + j) * (kTileKeys / kBlkTokens) + bi;
+        there = false;
+        if (k * kBlkTokens < un.len) {
+          int in_page;
+          const int id = __ldg(p.table + un.b * p.table_stride + page_of(p, k, in_page));
+          if (id >= 0 && id < p.n_pages) {
+            there = true;
+            const uint8_t* blk = p.pages + id * p.page_stride + un.h * p.head_stride + in_page * B::kBytes;
+            auto get = [](const uint8_t* at, auto& v) {
+              if constexpr (sizeof(v) == 16) {
+                const uint4 x = *reinterpret_cast<const uint4*>(at);
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(at);
+                v[0] = x.x; v[1] = x.y;
+              }
+            };
+            get(blk + B::key_word(ktok, 0, kj), kw);
+            get(blk + B::key_sz(ktok, 0), ks);
+            get(blk + B::kV + piece * (VW * 4), vw);
+            get(blk + B::value_sz(8 * vhi + 2 * vj, vi * B::W / 4), vs);
+          }
+        }
+      };
+      if (nt > 0) load(0);
+      for (int j = 0; j < nt; ++j) {
+        const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
+        if (!warp_wait(kv_empty + st, ph ^ 1)) break;
+        uint8_t* stage = smem + T::kOffStage + st * T::kStage;
+        const int t0 = (un.kt0 + j) * kTileKeys + bi * kBlkTokens;
+        const bool have = there;
+        // places without a token yet, or without a page: zeros, whatever their bits
+        uint32_t k_w[N], k_s[N], v_w[VW], v_s[2];
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          k_w[g] = kw[g];
+          k_s[g] = have && t0 + ktok < un.len ? ks[g] : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < VW; ++e) v_w[e] = vw[e];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v_s[e] = have && t0 + 8 * vhi + 2 * vj + e < un.len ? vs[e] : 0u;
+        if (j + 1 < nt) load(j + 1);
+
+        const int row = bi * kBlkTokens + ktok;
+        uint8_t* kd = stage + (row >> 3) * 128 + (row & 7) * 16;
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          const uint32_t s2 = hmul2(__byte_perm(k_s[g], 0, 0x1010), 0x38003800u);  // s / 2
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = e < 2 ? k_w[g] : k_w[g] >> 8;
+            const uint32_t c = e & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
+                                     : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
+            hi[e] = hmul2(c, s2);
+            lo[e] = hfma2(c, s2, hi[e] ^ 0x80008000u);
+          }
+          *reinterpret_cast<uint4*>(kd + (4 * g + kj) * T::kChunk) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(kd + T::kKey + (4 * g + kj) * T::kChunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (kj < 2) {  // zeros of the token's groups, against the sums' hi and against their lo
+          uint32_t z[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int g = 0; g < N; g += 2) z[g / 2] = __byte_perm(k_s[g], k_s[g + 1], 0x7632);
+          *reinterpret_cast<uint4*>(stage + 2 * T::kKey + kj * (kTileKeys * 16) + row * 16) = make_uint4(z[0], z[1], z[2], z[3]);
+        }
+        uint8_t* vd = stage + 2 * T::kKey + T::kZ + (bi * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {  // word e: token e / W, dim chunk W vi + e % W
+          const uint32_t s2 = __byte_perm(v_s[e / B::W], 0, 0x1010), z2 = __byte_perm(v_s[e / B::W], 0, 0x3232);
+          uint32_t o[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t x = q < 2 ? v_w[e] : v_w[e] >> 8;
+            const uint32_t c = q & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
+                                     : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
+            o[q] = hfma2(c, s2, z2);
+          }
+          *reinterpret_cast<uint4*>(vd + (B::W * vi + e % B::W) * 128 + e / B::W * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if (piece == 0) s_hidden[st * 4 + bi] = have ? 0 : 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kv_full + st);
+      }
+    } else {
+      // ================= MMA: one thread issues ==================================
+      named_bar_sync(1, (kSoftWarps + 1) * 32);  // Q is in shared memory
+      if (lane == 0) {
+        const uint32_t qa = smem_u32(s_q), pa = smem_u32(s_prob);
+        const uint32_t id_s = idesc(kTileKeys, false), id_o = idesc(D, true);
+        bool ok = true;
+        for (int j = 0; j <= nt && ok; ++j) {
+          if (j < nt) {
+            const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
+            ok = wait(kv_full + st, ph) && wait(s_empty + st, ph ^ 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t ka = smem_u32(smem + T::kOffStage + st * T::kStage), ts = tmem + st * kTileKeys;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // hi, lo
+#pragma unroll
+              for (int c = 0; c < D / 8; c += 2)
+                tc_mma_f16(ts, smem_desc(qa + c * 2048, 2048, 128),
+                           smem_desc(ka + half * T::kKey + c * T::kChunk, T::kChunk, 128), id_s, (half | c) != 0);
+            }
+            tc_mma_f16(ts, smem_desc(qa + D / 8 * 2048, 2048, 128),
+                       smem_desc(ka + 2 * T::kKey, kTileKeys * 16, 128), id_s, 1);
+            tc_commit(s_full + st);
+          }
+          if (j > 0) {
+            const uint32_t n = n0 + j - 1, st = n & 1, ph = (n >> 1) & 1;
+            ok = wait(p_full + st, ph);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t va = smem_u32(smem + T::kOffStage + st * T::kStage + 2 * T::kKey + T::kZ);
+#pragma unroll
+            for (int half = 0; half < (LO ? 2 : 1); ++half) {
+#pragma unroll
+              for (int c = 0; c < kTileKeys / 8; c += 2)
+                tc_mma_f16(t_o, smem_desc(pa + (LO ? half : st) * T::kProb + c * 2048, 2048, 128),
+                           smem_desc(va + c * (D / 8 * 128), D / 8 * 128, 128), id_o, j > 1 || (half | c) != 0);
+            }
+            tc_commit(kv_empty + st);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    n0 += nt;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  if (*s_abort && tid == kMmaWarp * 32) {  // a wait gave up: what was issued must end before the CTA does
+    tc_commit(bars + 12);
+    mbar_wait_bounded(bars + 12, 0, kTileWaitNs);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) tc_dealloc(tmem, 256);
+}
+
+template <int D, bool LO>
+int launch(AttnParams& p, cudaStream_t st) {
+  static_assert(Tile<D>::kSmem <= 227 * 1024, "shared memory");
+  const cudaError_t e = cudaFuncSetAttribute(attn_tile_kernel<D, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::kSmem);
+  if (e != cudaSuccess) return fail(SS_ERR_CUDA, std::string("ss_int4_attention: ") + cudaGetErrorString(e));
+  attn_tile_kernel<D, LO><<<sm_count(), kTileThreads, Tile<D>::kSmem, st>>>(p);
+  return check_launch("ss_int4_attention");
+}
+
+}  // namespace
+
+int launch_tiles(AttnParams& p, int d, cudaStream_t st) {
+  const bool lo = p.dtype == SS_F16;
+  if (d == 64) return lo ? launch<64, true>(p, st) : launch<64, false>(p, st);
+  return lo ? launch<128, true>(p, st) : launch<128, false>(p, st);
+}
+
+}  // namespace ss

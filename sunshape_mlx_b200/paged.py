@@ -209,6 +209,7 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     ``return_lse``, the natural log-sum-exp (n_tokens, n_q_heads) in fp32. A
     row that sees no key gives 0 and -inf, as does a token outside ``cu_q``.
     """
+    L.poll_device_errors()
     L.require_cuda(queries, pages)
     if queries.dim() != 3:
         raise ValueError("queries must be (n_tokens, n_q_heads, head_dim)")
