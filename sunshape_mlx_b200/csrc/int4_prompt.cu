@@ -95,14 +95,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   uint8_t* s_q = smem;
   uint8_t* s_prob = smem + T::kOffProb;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kOffMisc);
-  uint64_t* kv_full = bars;        // [2] the 8 decode warps
-  uint64_t* kv_empty = bars + 2;   // [2] P V of the stage's tile is done
-  uint64_t* s_full = bars + 4;     // [2] Q K^T is done
+  uint64_t* k_full = bars;         // [2] the 8 decode warps have written keys
+  uint64_t* v_full = bars + 10;    // [2] and values
+  uint64_t* o_done = bars + 2;     // [2] P V is done: the stage's values and P are free
+  uint64_t* s_full = bars + 4;     // [2] Q K^T is done: S is there, the stage's keys are free
   uint64_t* s_empty = bars + 6;    // [2] the 4 softmax warps have read S
   uint64_t* p_full = bars + 8;     // [2] the 4 softmax warps have written P
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [2][4] blocks of a stage without a page
+  uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [4][4] blocks of a tile without a page; read before S is freed
   int* s_sum = reinterpret_cast<int*>(smem + T::kOffMisc + 256);      // [13] warps' units
   int* s_cum = reinterpret_cast<int*>(smem + T::kOffMisc + 512);      // [threads] units before a thread's requests
 
@@ -111,8 +112,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   // ---- setup ---------------------------------------------------------------
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(kv_full + s, kDecWarps);
-      mbar_init(kv_empty + s, 1);
+      mbar_init(k_full + s, kDecWarps);
+      mbar_init(v_full + s, kDecWarps);
+      mbar_init(o_done + s, 1);
       mbar_init(s_full + s, 1);
       mbar_init(s_empty + s, kSoftWarps);
       mbar_init(p_full + s, kSoftWarps);
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[c + e] = __uint_as_float(v[e]);
         }
-        const uint32_t hid = *reinterpret_cast<volatile uint32_t*>(s_hidden + buf * 4);
+        const uint32_t hid = *reinterpret_cast<volatile uint32_t*>(s_hidden + (n & 3) * 4);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_empty + buf);
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           l0 *= f;
           l1 *= f;
           if (j > 0) {  // O holds the tiles before: all of them, once the last one's P V is done
-            if (!(ok = warp_wait(kv_empty + (buf ^ 1), ((n - 1) >> 1) & 1))) break;
+            if (!(ok = warp_wait(o_done + (buf ^ 1), ((n - 1) >> 1) & 1))) break;
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
@@ -329,8 +331,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           }
         }
         // the P buffer is free once P V of the tile two before (one buffer with lo: one before) is done
-        if (!LO) ok = warp_wait(kv_empty + buf, ph ^ 1);
-        else if (j > 0) ok = warp_wait(kv_empty + (buf ^ 1), ((n - 1) >> 1) & 1);
+        if (!LO) ok = warp_wait(o_done + buf, ph ^ 1);
+        else if (j > 0) ok = warp_wait(o_done + (buf ^ 1), ((n - 1) >> 1) & 1);
         if (!ok) break;
         uint8_t* dst = s_prob + (LO ? 0 : buf * T::kProb) + (r >> 3) * 128 + (r & 7) * 16;
 #pragma unroll
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       }
       // ---- output ----
       const float l = l0 + l1;
-      if (ok && nt > 0) ok = warp_wait(kv_empty + ((n0 + nt - 1) & 1), ((n0 + nt - 1) >> 1) & 1);
+      if (ok && nt > 0) ok = warp_wait(o_done + ((n0 + nt - 1) & 1), ((n0 + nt - 1) >> 1) & 1);
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       if (nt > 0) load(0);
       for (int j = 0; j < nt; ++j) {
         const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
-        if (!warp_wait(kv_empty + st, ph ^ 1)) break;
+        if (!warp_wait(s_full + st, ph ^ 1)) break;
         uint8_t* stage = smem + T::kOffStage + st * T::kStage;
         const int t0 = (un.kt0 + j) * kTileKeys + bi * kBlkTokens;
         const bool have = there;
@@ -476,6 +478,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           for (int g = 0; g < N; g += 2) z[g / 2] = __byte_perm(k_s[g], k_s[g + 1], 0x7632);
           *reinterpret_cast<uint4*>(stage + 2 * T::kKey + kj * (kTileKeys * 16) + row * 16) = make_uint4(z[0], z[1], z[2], z[3]);
         }
+        if (piece == 0) s_hidden[(n & 3) * 4 + bi] = have ? 0 : 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full + st);
+
+        if (!warp_wait(o_done + st, ph ^ 1)) break;
         uint8_t* vd = stage + 2 * T::kKey + T::kZ + (bi * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
 #pragma unroll
         for (int e = 0; e < VW; ++e) {  // word e: token e / W, dim chunk W vi + e % W
@@ -490,10 +498,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           }
           *reinterpret_cast<uint4*>(vd + (B::W * vi + e % B::W) * 128 + e / B::W * 16) = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        if (piece == 0) s_hidden[st * 4 + bi] = have ? 0 : 1;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(kv_full + st);
+        if (lane == 0) mbar_arrive(v_full + st);
       }
     } else {
       // ================= MMA: one thread issues ==================================
@@ -505,7 +512,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         for (int j = 0; j <= nt && ok; ++j) {
           if (j < nt) {
             const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
-            ok = wait(kv_full + st, ph) && wait(s_empty + st, ph ^ 1);
+            ok = wait(k_full + st, ph) && wait(s_empty + st, ph ^ 1);
             if (!ok) break;
             tc_fence_after();
             const uint32_t ka = smem_u32(smem + T::kOffStage + st * T::kStage), ts = tmem + st * kTileKeys;
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           }
           if (j > 0) {
             const uint32_t n = n0 + j - 1, st = n & 1, ph = (n >> 1) & 1;
-            ok = wait(p_full + st, ph);
+            ok = wait(v_full + st, ph) && wait(p_full + st, ph);
             if (!ok) break;
             tc_fence_after();
             const uint32_t va = smem_u32(smem + T::kOffStage + st * T::kStage + 2 * T::kKey + T::kZ);
@@ -533,7 +540,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 tc_mma_f16(t_o, smem_desc(pa + (LO ? half : st) * T::kProb + c * 2048, 2048, 128),
                            smem_desc(va + c * (D / 8 * 128), D / 8 * 128, 128), id_o, j > 1 || (half | c) != 0);
             }
-            tc_commit(kv_empty + st);
+            tc_commit(o_done + st);
           }
         }
       }
