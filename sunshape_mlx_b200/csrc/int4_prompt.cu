@@ -7,10 +7,12 @@
 // request first. Per tile of 64 tokens: Per tile of 64 tokens:
 //   decode   (8 warps)  codes -> fp16 operands in shared memory
 //   S = Q K^T (1 thread) M = 128, N = 64, fp32 in TMEM, two buffers
-//   softmax  (4 warps)  a thread per row, P as fp16 in shared memory
+//   softmax  (4 warps)  a thread per row, P as fp16 in TMEM
 //   O += P V (same thread) M = 128, N = D, fp32 in TMEM
 // and the four run on different tiles at the same time, handing over through
-// mbarriers (two stages of keys and values, two S and P buffers).
+// mbarriers (two stages of keys and values, two S and P buffers). Q and P are
+// A operands in TMEM: with N = 64 and A in shared memory a step of 16 takes 49
+// cycles instead of 32.
 //
 // Keys enter exactly: c s is the pair of fp16 values hi = fp16(c s) and
 // lo = c s - hi (15 bits in all, so lo is exact), and q . z is one more K step
@@ -32,21 +34,25 @@ namespace {
 
 constexpr int kTileRows = 128, kTileKeys = 64;
 constexpr int kSoftWarps = 4, kDecWarps = 8, kMmaWarp = kSoftWarps + kDecWarps;
-constexpr int kTileThreads = (kMmaWarp + 1) * 32;
+constexpr int kTileWarps = 16, kTileThreads = kTileWarps * 32;  // whole warpgroups: registers are moved between them
+// Registers of a thread: 128 at launch; 4 * 208 + 8 * 104 + 4 * 64 = 480 * 4 of the 512 * 4 there are.
+constexpr int kSoftRegs = 208, kDecRegs = 104, kMmaRegs = 64;
 constexpr uint64_t kTileWaitNs = 2000000000ull;
 constexpr int kTileWaitCode = 32;
 
 template <int D>
 struct Tile {
-  static constexpr int kQ = (D / 8 + 2) * 2048;     // [dim chunk, then 2 of group sums][row] 16 bytes
   static constexpr int kChunk = kTileKeys * 16 + 32;  // a dim chunk of keys; + 32: no bank conflicts
   static constexpr int kKey = D / 8 * kChunk;       // hi; lo behind it
   static constexpr int kZ = 2 * kTileKeys * 16;     // zeros, twice
   static constexpr int kVal = kTileKeys * D * 2;    // [8 tokens][dim chunk][token] 16 bytes
   static constexpr int kStage = 2 * kKey + kZ + kVal;
-  static constexpr int kProb = kTileRows * kTileKeys * 2;  // [8 tokens][row] 16 bytes
-  static constexpr int kOffStage = kQ, kOffProb = kQ + 2 * kStage, kOffMisc = kOffProb + 2 * kProb;
+  static constexpr int kOffMisc = 2 * kStage;
   static constexpr int kSmem = kOffMisc + 512 + kTileThreads * 4;
+  // TMEM columns: two S, O, then the A operands, two fp16 a column: Q, its group sums, two P
+  static constexpr int kTO = 2 * kTileKeys, kTQ = kTO + D, kTSum = kTQ + D / 2, kTP = kTSum + 32;
+  static constexpr int kCols = 512;
+  static_assert(kTP + kTileKeys <= kCols, "TMEM");
 };
 
 __device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {  // fp16 in, fp32 out, M = 128
@@ -69,7 +75,35 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+template <int N>
+__device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t* v) {
+  if constexpr (N == 32) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] = v[i];
+    tc_st32(taddr, w);
+  } else {
+    static_assert(N == 8, "columns");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  }
+}
+// D[tmem] (+)= A[tmem] * B[smem]; the descriptor of B in two words, so that steps are immediates.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.u32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(id), "r"((uint32_t)acc)
+      : "memory");
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t hfms2(uint32_t a, uint32_t b, uint32_t c) {  // a b - c
+  uint32_t r;
+  asm("{\n .reg .b32 n;\n neg.f16x2 n, %3;\n fma.rn.f16x2 %0, %1, %2, n;\n}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 
 // A unit: its rows, and the key tiles [kt0, kt1) that any of them sees.
 struct Unit {
@@ -92,8 +126,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   using B = Int4Blk<D>;
   using T = Tile<D>;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* s_q = smem;
-  uint8_t* s_prob = smem + T::kOffProb;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kOffMisc);
   uint64_t* k_full = bars;         // [2] the 8 decode warps have written keys
   uint64_t* v_full = bars + 10;    // [2] and values
@@ -101,10 +133,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   uint64_t* s_full = bars + 4;     // [2] Q K^T is done: S is there, the stage's keys are free
   uint64_t* s_empty = bars + 6;    // [2] the 4 softmax warps have read S
   uint64_t* p_full = bars + 8;     // [2] the 4 softmax warps have written P
+  uint64_t* q_full = bars + 13;    // and the unit's Q
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [4][4] blocks of a tile without a page; read before S is freed
-  int* s_sum = reinterpret_cast<int*>(smem + T::kOffMisc + 256);      // [13] warps' units
+  int* s_sum = reinterpret_cast<int*>(smem + T::kOffMisc + 256);      // [16] warps' units
   int* s_cum = reinterpret_cast<int*>(smem + T::kOffMisc + 512);      // [threads] units before a thread's requests
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -119,12 +152,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       mbar_init(s_empty + s, kSoftWarps);
       mbar_init(p_full + s, kSoftWarps);
     }
+    mbar_init(q_full, kSoftWarps);
     mbar_init(bars + 12, 1);  // end of an abandoned unit's MMAs
     *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
-    tc_alloc(s_tmem, 256);
+    tc_alloc(s_tmem, T::kCols);
     tc_relinquish();
   }
   const int per = (p.n + kTileThreads - 1) / kTileThreads;
@@ -142,14 +176,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   __syncthreads();
   tc_fence_after();
   int total = 0, before = 0;
-  for (int w = 0; w <= kMmaWarp; ++w) {
+  for (int w = 0; w < kTileWarps; ++w) {
     if (w == warp) before = total;
     total += s_sum[w];
   }
   s_cum[tid] = before + inc - units;
   __syncthreads();
   const uint32_t tmem = *s_tmem;
-  const uint32_t t_o = tmem + 2 * kTileKeys;
+  const uint32_t t_o = tmem + T::kTO;
 
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     if (mbar_try_wait(bar, parity)) return true;
@@ -167,47 +201,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-  // ---- unit after unit -------------------------------------------------------
-  uint32_t n0 = 0;  // tiles of this CTA's earlier units: the barriers' phases go on
-  for (int round = 0;; ++round) {
-    // longest first within a request, rounds in alternating direction: nearly equal sums
-    const int u = round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (round * (int64_t)gridDim.x >= total || *s_abort) break;
-    if (u >= total) continue;
-    Unit un;
-    {
-      int a = 0, e = kTileThreads;
-      while (e - a > 1) {
-        const int mid = (a + e) >> 1;
-        if (s_cum[mid] <= u) a = mid; else e = mid;
-      }
-      int at = s_cum[a], b = a * per, nt = 0;
-      for (;; ++b) {
-        nt = tiles_of(p, b);
-        if (at + nt * p.hkv > u) break;
-        at += nt * p.hkv;
-      }
-      const int qt = nt - 1 - (u - at) / p.hkv;  // the last rows of a causal request see most keys
-      un.b = b;
-      un.h = (u - at) % p.hkv;
-      un.tok0 = max(p.cu_q[b], 0);
-      un.nq = max(p.cu_q[b + 1] - un.tok0, 0);
-      un.len = min(max(p.seq_lens[b], 0), p.width * p.page);
-      un.row0 = qt * kTileRows;
-      un.rows = (int)min((int64_t)kTileRows, (int64_t)un.nq * p.grp - un.row0);
-      int beg0, end0, beg1, end1;
-      row_keys(p, un.nq, un.len, un.row0 / p.grp, beg0, end0);
-      row_keys(p, un.nq, un.len, (un.row0 + un.rows - 1) / p.grp, beg1, end1);
-      un.kt0 = beg0 / kTileKeys;
-      un.kt1 = max(un.kt0, (end1 + kTileKeys - 1) / kTileKeys);
-      if (end1 <= beg0) un.kt1 = un.kt0;
-      un.all0 = beg1;
-      un.all1 = end0;
+  // The CTA's next unit; false when there is none. Each role walks the units by itself.
+  int round = 0;
+  auto next_unit = [&](Unit& un) -> bool {
+    int u;
+    do {  // longest first within a request, rounds in alternating direction: nearly equal sums
+      if (round * (int64_t)gridDim.x >= total) return false;
+      u = round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      ++round;
+    } while (u >= total);
+    int a = 0, e = kTileThreads;
+    while (e - a > 1) {
+      const int mid = (a + e) >> 1;
+      if (s_cum[mid] <= u) a = mid; else e = mid;
     }
-    const int nt = un.kt1 - un.kt0;
+    int at = s_cum[a], b = a * per, tiles = 0;
+    for (;; ++b) {
+      tiles = tiles_of(p, b);
+      if (at + tiles * p.hkv > u) break;
+      at += tiles * p.hkv;
+    }
+    const int qt = tiles - 1 - (u - at) / p.hkv;  // the last rows of a causal request see most keys
+    un.b = b;
+    un.h = (u - at) % p.hkv;
+    un.tok0 = max(p.cu_q[b], 0);
+    un.nq = max(p.cu_q[b + 1] - un.tok0, 0);
+    un.len = min(max(p.seq_lens[b], 0), p.width * p.page);
+    un.row0 = qt * kTileRows;
+    un.rows = (int)min((int64_t)kTileRows, (int64_t)un.nq * p.grp - un.row0);
+    int beg0, end0, beg1, end1;
+    row_keys(p, un.nq, un.len, un.row0 / p.grp, beg0, end0);
+    row_keys(p, un.nq, un.len, (un.row0 + un.rows - 1) / p.grp, beg1, end1);
+    un.kt0 = beg0 / kTileKeys;
+    un.kt1 = end1 <= beg0 ? un.kt0 : max(un.kt0, (end1 + kTileKeys - 1) / kTileKeys);
+    un.all0 = beg1;
+    un.all1 = end0;
+    return true;
+  };
 
-    if (warp < kSoftWarps) {
-      // ================= softmax: a thread per row ==============================
+  Unit un;
+  uint32_t n0 = 0;  // tiles of this CTA's earlier units: the barriers' phases go on
+  bool ok = true;   // no wait gave up
+  if (warp < kSoftWarps) {
+    // ================= softmax: a thread per row ================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    while (ok && next_unit(un)) {
+      const int nt = un.kt1 - un.kt0;
       const int r = tid, rr = un.row0 + r, i = rr / p.grp, hd = un.h * p.grp + rr % p.grp;
       const int64_t tok = un.tok0 + (int64_t)i;
       const bool live = r < un.rows && tok < p.n_tokens;
@@ -240,8 +279,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         int ex = 0;
         if (big > 0.f && big < INFINITY) ex = 135 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
         const float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
-        uint8_t* dst = s_q + (r >> 3) * 128 + (r & 7) * 16;
-        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+        uint32_t qs[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};  // group sums: 8 hi, 8 lo
+        uint32_t qo[D / 2];
         static_assert(B::G <= 8, "group sums fill one chunk");
         float sum[B::G];
 #pragma unroll
@@ -255,43 +294,47 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             f[2 * e] = (p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16)) * up;
             f[2 * e + 1] = (p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u)) * up;
           }
-          uint32_t o[4];  // dims (e, e + 4) side by side, as the key words' nibbles come
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[e] = pack_h2(f[e], f[e + 4]);
-            sum[c / 4] += lo_h(o[e]) + hi_h(o[e]);
+          for (int e = 0; e < 4; ++e) {  // dims (e, e + 4) side by side, as the key words' nibbles come
+            const uint32_t o = pack_h2(f[e], f[e + 4]);
+            qo[c * 4 + e] = o;
+            sum[c / 4] += lo_h(o) + hi_h(o);
           }
-          *reinterpret_cast<uint4*>(dst + c * 2048) = make_uint4(o[0], o[1], o[2], o[3]);
         }
 #pragma unroll
         for (int g = 0; g < B::G; g += 2) {  // halved, as the keys are
           const float a = 0.5f * sum[g], b = 0.5f * sum[g + 1];
-          hi[g / 2] = pack_h2(a, b);
-          lo[g / 2] = pack_h2(a - lo_h(hi[g / 2]), b - hi_h(hi[g / 2]));
+          qs[g / 2] = pack_h2(a, b);
+          qs[4 + g / 2] = pack_h2(a - lo_h(qs[g / 2]), b - hi_h(qs[g / 2]));
         }
-        *reinterpret_cast<uint4*>(dst + (D / 8) * 2048) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + (D / 8 + 1) * 2048) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int c = 0; c < D / 2; c += 32) tc_st<32>(tmem + lane_base + T::kTQ + c, qo + c);
+        tc_st<8>(tmem + lane_base + T::kTSum, qs);
         fac = 2.f * p.scale * kLog2e / up;
-        fence_proxy_async_smem();
+        tc_wait_st();
+        tc_fence_before();
       }
-      named_bar_sync(1, (kSoftWarps + 1) * 32);  // the MMA warp may read Q
+      __syncwarp();
+      if (lane == 0 && nt > 0) mbar_arrive(q_full);  // and O of the unit before has been read
 
       int beg = 0, end = 0;
       if (r < un.rows) row_keys(p, un.nq, un.len, i, beg, end);
       float m = kLow, l0 = 0.f, l1 = 0.f;
-      bool ok = true;
       for (int j = 0; j < nt; ++j) {
         const uint32_t n = n0 + j, buf = n & 1, ph = (n >> 1) & 1;
         if (!(ok = warp_wait(s_full + buf, ph))) break;
         tc_fence_after();
         float y[kTileKeys];
-#pragma unroll
-        for (int c = 0; c < kTileKeys; c += 32) {
-          uint32_t v[32];
-          tc_ld32(tmem + lane_base + buf * kTileKeys + c, v);
+        {
+          uint32_t v0[32], v1[32];
+          tc_ld32(tmem + lane_base + buf * kTileKeys, v0);
+          tc_ld32(tmem + lane_base + buf * kTileKeys + 32, v1);
           tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[c + e] = __uint_as_float(v[e]);
+          for (int e = 0; e < 32; ++e) {
+            y[e] = __uint_as_float(v0[e]);
+            y[32 + e] = __uint_as_float(v1[e]);
+          }
         }
         const uint32_t hid = *reinterpret_cast<volatile uint32_t*>(s_hidden + (n & 3) * 4);
         tc_fence_before();
@@ -334,28 +377,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         if (!LO) ok = warp_wait(o_done + buf, ph ^ 1);
         else if (j > 0) ok = warp_wait(o_done + (buf ^ 1), ((n - 1) >> 1) & 1);
         if (!ok) break;
-        uint8_t* dst = s_prob + (LO ? 0 : buf * T::kProb) + (r >> 3) * 128 + (r & 7) * 16;
+        uint32_t w[kTileKeys / 2];
 #pragma unroll
-        for (int c = 0; c < kTileKeys / 8; ++c) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float& a = y[c * 8 + 2 * e];
-            float& b = y[c * 8 + 2 * e + 1];
-            add_f32x2(a, b, -m, -m);
-            a = ex2(a);
-            b = ex2(b);
-            add_f32x2(l0, l1, a, b);
-            w[e] = pack_h2(a, b);
-          }
-          *reinterpret_cast<uint4*>(dst + c * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
-          if constexpr (LO) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack_h2(y[c * 8 + 2 * e] - lo_h(w[e]), y[c * 8 + 2 * e + 1] - hi_h(w[e]));
-            *reinterpret_cast<uint4*>(dst + T::kProb + c * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+        for (int e = 0; e < kTileKeys / 2; ++e) {
+          float& a = y[2 * e];
+          float& b = y[2 * e + 1];
+          add_f32x2(a, b, -m, -m);
+          a = ex2(a);
+          b = ex2(b);
+          add_f32x2(l0, l1, a, b);
+          w[e] = pack_h2(a, b);
         }
-        fence_proxy_async_smem();
+        tc_st<32>(tmem + lane_base + T::kTP + (LO ? 0 : buf * 32), w);
+        if constexpr (LO) {
+#pragma unroll
+          for (int e = 0; e < kTileKeys / 2; ++e) w[e] = pack_h2(y[2 * e] - lo_h(w[e]), y[2 * e + 1] - hi_h(w[e]));
+          tc_st<32>(tmem + lane_base + T::kTP + 32, w);
+        }
+        tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + buf);
@@ -400,8 +439,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         if (live && p.lse) p.lse[tok * p.hq + hd] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
         tc_fence_before();
       }
-    } else if (warp < kMmaWarp) {
-      // ================= decode: 64 threads per block of 16 tokens ==============
+      n0 += nt;
+    }
+  } else if (warp < kMmaWarp) {
+    // ================= decode: 64 threads per block of 16 tokens ================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecRegs));
+    while (ok && next_unit(un)) {
+      const int nt = un.kt1 - un.kt0;
       const int d = tid - kSoftWarps * 32, bi = d >> 6, piece = d & 63;
       constexpr int N = B::N, VW = 2 * B::W;          // key words and value words of a thread
       static_assert(B::G == N, "one key piece per token and lane");
@@ -438,8 +482,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       if (nt > 0) load(0);
       for (int j = 0; j < nt; ++j) {
         const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
-        if (!warp_wait(s_full + st, ph ^ 1)) break;
-        uint8_t* stage = smem + T::kOffStage + st * T::kStage;
+        if (!(ok = warp_wait(s_full + st, ph ^ 1))) break;
+        uint8_t* stage = smem + st * T::kStage;
         const int t0 = (un.kt0 + j) * kTileKeys + bi * kBlkTokens;
         const bool have = there;
         // places without a token yet, or without a page: zeros, whatever their bits
@@ -467,7 +511,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             const uint32_t c = e & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
                                      : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
             hi[e] = hmul2(c, s2);
-            lo[e] = hfma2(c, s2, hi[e] ^ 0x80008000u);
+            lo[e] = hfms2(c, s2, hi[e]);
           }
           *reinterpret_cast<uint4*>(kd + (4 * g + kj) * T::kChunk) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *reinterpret_cast<uint4*>(kd + T::kKey + (4 * g + kj) * T::kChunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -483,7 +527,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full + st);
 
-        if (!warp_wait(o_done + st, ph ^ 1)) break;
+        if (!(ok = warp_wait(o_done + st, ph ^ 1))) break;
         uint8_t* vd = stage + 2 * T::kKey + T::kZ + (bi * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
 #pragma unroll
         for (int e = 0; e < VW; ++e) {  // word e: token e / W, dim chunk W vi + e % W
@@ -502,29 +546,38 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         __syncwarp();
         if (lane == 0) mbar_arrive(v_full + st);
       }
-    } else {
-      // ================= MMA: one thread issues ==================================
-      named_bar_sync(1, (kSoftWarps + 1) * 32);  // Q is in shared memory
-      if (lane == 0) {
-        const uint32_t qa = smem_u32(s_q), pa = smem_u32(s_prob);
+      n0 += nt;
+    }
+  } else {
+    // ================= MMA: one thread issues ====================================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == kMmaWarp && lane == 0) {
+      uint32_t q_phase = 0;
+      while (ok && next_unit(un)) {
+        const int nt = un.kt1 - un.kt0;
+        if (nt > 0) {
+          ok = wait(q_full, q_phase);
+          q_phase ^= 1;
+        }
         const uint32_t id_s = idesc(kTileKeys, false), id_o = idesc(D, true);
-        bool ok = true;
+        // B descriptors: start address, bytes between core matrices along K (lbo) and along N (sbo)
+        auto lo_word = [](uint32_t at, uint32_t lbo) { return (at >> 4 & 0x3fff) | (lbo >> 4) << 16; };
+        constexpr uint32_t hi_word = 128 >> 4 | 1u << 14;
         for (int j = 0; j <= nt && ok; ++j) {
           if (j < nt) {
             const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
             ok = wait(k_full + st, ph) && wait(s_empty + st, ph ^ 1);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t ka = smem_u32(smem + T::kOffStage + st * T::kStage), ts = tmem + st * kTileKeys;
+            const uint32_t ka = smem_u32(smem + st * T::kStage), ts = tmem + st * kTileKeys;
+            const uint32_t k_lo = lo_word(ka, T::kChunk), z_lo = lo_word(ka + 2 * T::kKey, kTileKeys * 16);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // hi, lo
 #pragma unroll
               for (int c = 0; c < D / 8; c += 2)
-                tc_mma_f16(ts, smem_desc(qa + c * 2048, 2048, 128),
-                           smem_desc(ka + half * T::kKey + c * T::kChunk, T::kChunk, 128), id_s, (half | c) != 0);
+                tc_mma_ts(ts, tmem + T::kTQ + c * 4, k_lo + (half * T::kKey + c * T::kChunk) / 16, hi_word, id_s, (half | c) != 0);
             }
-            tc_mma_f16(ts, smem_desc(qa + D / 8 * 2048, 2048, 128),
-                       smem_desc(ka + 2 * T::kKey, kTileKeys * 16, 128), id_s, 1);
+            tc_mma_ts(ts, tmem + T::kTSum, z_lo, hi_word, id_s, true);
             tc_commit(s_full + st);
           }
           if (j > 0) {
@@ -532,32 +585,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             ok = wait(v_full + st, ph) && wait(p_full + st, ph);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t va = smem_u32(smem + T::kOffStage + st * T::kStage + 2 * T::kKey + T::kZ);
+            const uint32_t v_lo = lo_word(smem_u32(smem + st * T::kStage + 2 * T::kKey + T::kZ), D / 8 * 128);
 #pragma unroll
             for (int half = 0; half < (LO ? 2 : 1); ++half) {
 #pragma unroll
               for (int c = 0; c < kTileKeys / 8; c += 2)
-                tc_mma_f16(t_o, smem_desc(pa + (LO ? half : st) * T::kProb + c * 2048, 2048, 128),
-                           smem_desc(va + c * (D / 8 * 128), D / 8 * 128, 128), id_o, j > 1 || (half | c) != 0);
+                tc_mma_ts(t_o, tmem + T::kTP + (LO ? half : st) * 32 + c * 4, v_lo + c * (D / 8 * 128) / 16, hi_word, id_o,
+                          j > 1 || (half | c) != 0);
             }
             tc_commit(o_done + st);
           }
         }
+        n0 += nt;
       }
-      __syncwarp();
     }
-    n0 += nt;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    __syncwarp();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   if (*s_abort && tid == kMmaWarp * 32) {  // a wait gave up: what was issued must end before the CTA does
     tc_commit(bars + 12);
     mbar_wait_bounded(bars + 12, 0, kTileWaitNs);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tc_dealloc(tmem, 256);
+  if (warp == kMmaWarp) tc_dealloc(tmem, T::kCols);
 }
 
 template <int D, bool LO>
