@@ -4,15 +4,16 @@
 // A unit is (request, kv-head, 128 query rows); the rows of a group's heads and
 // of consecutive tokens share a tile, so keys and values are decoded once for
 // // all of them. CTAs (one an SM) take units in turn, those with most keys of a
-// request first. Per tile of 64 tokens: Per tile of 64 tokens:
-//   decode   (8 warps)  codes -> fp16 operands in shared memory
-//   S = Q K^T (1 thread) M = 128, N = 64, fp32 in TMEM, two buffers
-//   softmax  (4 warps)  a thread per row, P as fp16 in TMEM
-//   O += P V (same thread) M = 128, N = D, fp32 in TMEM
+// request first. Per tile of 128 tokens: Per tile of 128 tokens:
+//   decode    (8 warps)  codes -> fp16 operands in shared memory
+//   S = Q K^T (1 thread) M = 128, N = 128, fp32 in TMEM, two buffers
+//   softmax   (4 warps)  a thread per row, P as fp16 over its S in TMEM
+//   O += P V  (1 thread) M = 128, N = D, fp32 in TMEM
 // and the four run on different tiles at the same time, handing over through
-// mbarriers (two stages of keys and values, two S and P buffers). Q and P are
-// A operands in TMEM: with N = 64 and A in shared memory a step of 16 takes 49
-// cycles instead of 32.
+// mbarriers (two stages of keys and values, two S buffers). Q and P are A
+// operands in TMEM, which leaves shared memory to the two stages. Issuing an
+// MMA takes the thread about 75 cycles beside the other warps' work, a tile of
+// 64 tokens as long as one of 128.
 //
 // Keys enter exactly: c s is the pair of fp16 values hi = fp16(c s) and
 // lo = c s - hi (15 bits in all, so lo is exact), and q . z is one more K step
@@ -32,8 +33,8 @@
 namespace ss {
 namespace {
 
-constexpr int kTileRows = 128, kTileKeys = 64;
-constexpr int kSoftWarps = 4, kDecWarps = 8, kMmaWarp = kSoftWarps + kDecWarps;
+constexpr int kTileRows = 128, kTileKeys = 128;
+constexpr int kSoftWarps = 4, kDecWarps = 8, kMmaWarp = kSoftWarps + kDecWarps;  // two warps issue MMAs
 constexpr int kTileWarps = 16, kTileThreads = kTileWarps * 32;  // whole warpgroups: registers are moved between them
 // Registers of a thread: 128 at launch; 4 * 208 + 8 * 104 + 4 * 64 = 480 * 4 of the 512 * 4 there are.
 constexpr int kSoftRegs = 208, kDecRegs = 104, kMmaRegs = 64;
@@ -49,13 +50,13 @@ struct Tile {
   static constexpr int kStage = 2 * kKey + kZ + kVal;
   static constexpr int kOffMisc = 2 * kStage;
   static constexpr int kSmem = kOffMisc + 512 + kTileThreads * 4;
-  // TMEM columns: two S, O, then the A operands, two fp16 a column: Q, its group sums, two P
-  static constexpr int kTO = 2 * kTileKeys, kTQ = kTO + D, kTSum = kTQ + D / 2, kTP = kTSum + 32;
+  // TMEM columns: two S, each overwritten by its P (hi, then lo; two fp16 a column), O, Q, its group sums
+  static constexpr int kTO = 2 * kTileKeys, kTQ = kTO + D, kTSum = kTQ + D / 2;
   static constexpr int kCols = 512;
-  static_assert(kTP + kTileKeys <= kCols, "TMEM");
+  static_assert(kTSum + 8 <= kCols, "TMEM");
 };
 
-__device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {  // fp16 in, fp32 out, M = 128
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {  // fp16 in, fp32 out, M = 128
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
 }
 // 32 columns of this thread's TMEM lane, fp32.
@@ -105,6 +106,37 @@ __device__ __forceinline__ uint32_t hfms2(uint32_t a, uint32_t b, uint32_t c) { 
   return r;
 }
 
+// The MMAs of a tile in stage ST. Shared memory starts at 16 * base; TMEM at 0. A descriptor's
+// words: start address and bytes between core matrices along K; bytes along N (128) and version.
+__host__ __device__ constexpr uint32_t b_word(int at, int lbo) { return (uint32_t)at / 16 | (uint32_t)lbo / 16 << 16; }
+constexpr uint32_t kBHi = 128 >> 4 | 1u << 14;
+
+template <int D, int ST>
+__device__ __forceinline__ void issue_qk(uint32_t base) {
+  using T = Tile<D>;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {  // hi, lo
+#pragma unroll
+    for (int c = 0; c < D / 8; c += 2)
+      tc_mma_ts(ST * kTileKeys, T::kTQ + c * 4, base + b_word(ST * T::kStage + half * T::kKey + c * T::kChunk, T::kChunk), kBHi,
+                idesc(kTileKeys, false), (half | c) != 0);
+  }
+  tc_mma_ts(ST * kTileKeys, T::kTSum, base + b_word(ST * T::kStage + 2 * T::kKey, kTileKeys * 16), kBHi, idesc(kTileKeys, false), true);
+}
+
+template <int D, bool LO, int ST>
+__device__ __forceinline__ void issue_pv(uint32_t base, bool acc) {
+  using T = Tile<D>;
+#pragma unroll
+  for (int half = 0; half < (LO ? 2 : 1); ++half) {
+#pragma unroll
+    for (int c = 0; c < kTileKeys / 8; c += 2)
+      tc_mma_ts(T::kTO, ST * kTileKeys + half * (kTileKeys / 2) + c * 4,
+                base + b_word(ST * T::kStage + 2 * T::kKey + T::kZ + c * (D / 8 * 128), D / 8 * 128), kBHi, idesc(D, true),
+                (half | c) != 0 || acc);
+  }
+}
+
 // A unit: its rows, and the key tiles [kt0, kt1) that any of them sees.
 struct Unit {
   int b, h, row0, rows, nq, len, tok0, kt0, kt1, all0, all1;  // rows see the keys [all0, all1) whole
@@ -129,14 +161,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kOffMisc);
   uint64_t* k_full = bars;         // [2] the 8 decode warps have written keys
   uint64_t* v_full = bars + 10;    // [2] and values
-  uint64_t* o_done = bars + 2;     // [2] P V is done: the stage's values and P are free
+  uint64_t* o_done = bars + 2;     // [2] P V is done: the stage's values and its S are free
   uint64_t* s_full = bars + 4;     // [2] Q K^T is done: S is there, the stage's keys are free
-  uint64_t* s_empty = bars + 6;    // [2] the 4 softmax warps have read S
   uint64_t* p_full = bars + 8;     // [2] the 4 softmax warps have written P
   uint64_t* q_full = bars + 13;    // and the unit's Q
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [4][4] blocks of a tile without a page; read before S is freed
+  uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [4][8] blocks of a tile without a page; read before S is freed
   int* s_sum = reinterpret_cast<int*>(smem + T::kOffMisc + 256);      // [16] warps' units
   int* s_cum = reinterpret_cast<int*>(smem + T::kOffMisc + 512);      // [threads] units before a thread's requests
 
@@ -149,11 +180,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       mbar_init(v_full + s, kDecWarps);
       mbar_init(o_done + s, 1);
       mbar_init(s_full + s, 1);
-      mbar_init(s_empty + s, kSoftWarps);
       mbar_init(p_full + s, kSoftWarps);
     }
     mbar_init(q_full, kSoftWarps);
-    mbar_init(bars + 12, 1);  // end of an abandoned unit's MMAs
+    mbar_init(bars + 12, 2);  // end of an abandoned unit's MMAs
     *s_abort = 0;
     fence_mbar_init();
   }
@@ -182,8 +212,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   }
   s_cum[tid] = before + inc - units;
   __syncthreads();
-  const uint32_t tmem = *s_tmem;
-  const uint32_t t_o = tmem + T::kTO;
+  if (tid == 0 && *s_tmem != 0) {  // all columns were asked for: they start at 0
+    report_wait_failure(nullptr, p.sink, kTileWaitCode);
+    *s_abort = 1;
+  }
+  constexpr uint32_t tmem = 0, t_o = T::kTO;
 
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     if (mbar_try_wait(bar, parity)) return true;
@@ -326,28 +359,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         tc_fence_after();
         float y[kTileKeys];
         {
-          uint32_t v0[32], v1[32];
-          tc_ld32(tmem + lane_base + buf * kTileKeys, v0);
-          tc_ld32(tmem + lane_base + buf * kTileKeys + 32, v1);
+          uint32_t v[kTileKeys / 32][32];
+#pragma unroll
+          for (int c = 0; c < kTileKeys / 32; ++c) tc_ld32(tmem + lane_base + buf * kTileKeys + c * 32, v[c]);
           tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            y[e] = __uint_as_float(v0[e]);
-            y[32 + e] = __uint_as_float(v1[e]);
-          }
+          for (int c = 0; c < kTileKeys; ++c) y[c] = __uint_as_float(v[c / 32][c % 32]);
         }
-        const uint32_t hid = *reinterpret_cast<volatile uint32_t*>(s_hidden + (n & 3) * 4);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_empty + buf);
+        const uint2 hid = *reinterpret_cast<const uint2*>(s_hidden + (n & 3) * 8);
 
         const int t0 = (un.kt0 + j) * kTileKeys;
 #pragma unroll
         for (int e = 0; e < kTileKeys; e += 2) mul_f32x2(y[e], y[e + 1], fac);
-        if (t0 < un.all0 || t0 + kTileKeys > un.all1 || hid != 0) {
+        if (t0 < un.all0 || t0 + kTileKeys > un.all1 || (hid.x | hid.y) != 0) {
 #pragma unroll
-          for (int e = 0; e < kTileKeys; ++e)
-            if (t0 + e >= end || t0 + e < beg || (hid >> (e / 16 * 8) & 1)) y[e] = -INFINITY;
+          for (int e = 0; e < kTileKeys; ++e) {
+            const uint32_t gone = (e < 64 ? hid.x : hid.y) >> (e / 16 % 4 * 8) & 1;
+            if (t0 + e >= end || t0 + e < beg || gone) y[e] = -INFINITY;
+          }
         }
         float top = y[0];
 #pragma unroll
@@ -373,26 +402,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             tc_fence_before();
           }
         }
-        // the P buffer is free once P V of the tile two before (one buffer with lo: one before) is done
-        if (!LO) ok = warp_wait(o_done + buf, ph ^ 1);
-        else if (j > 0) ok = warp_wait(o_done + (buf ^ 1), ((n - 1) >> 1) & 1);
-        if (!ok) break;
-        uint32_t w[kTileKeys / 2];
+        // P over the S it comes from
 #pragma unroll
-        for (int e = 0; e < kTileKeys / 2; ++e) {
-          float& a = y[2 * e];
-          float& b = y[2 * e + 1];
-          add_f32x2(a, b, -m, -m);
-          a = ex2(a);
-          b = ex2(b);
-          add_f32x2(l0, l1, a, b);
-          w[e] = pack_h2(a, b);
-        }
-        tc_st<32>(tmem + lane_base + T::kTP + (LO ? 0 : buf * 32), w);
-        if constexpr (LO) {
+        for (int c = 0; c < kTileKeys; c += 64) {
+          uint32_t w[32];
 #pragma unroll
-          for (int e = 0; e < kTileKeys / 2; ++e) w[e] = pack_h2(y[2 * e] - lo_h(w[e]), y[2 * e + 1] - hi_h(w[e]));
-          tc_st<32>(tmem + lane_base + T::kTP + 32, w);
+          for (int e = 0; e < 32; ++e) {
+            float& a = y[c + 2 * e];
+            float& b = y[c + 2 * e + 1];
+            add_f32x2(a, b, -m, -m);
+            a = ex2(a);
+            b = ex2(b);
+            add_f32x2(l0, l1, a, b);
+            w[e] = pack_h2(a, b);
+          }
+          tc_st<32>(tmem + lane_base + buf * kTileKeys + c / 2, w);
+          if constexpr (LO) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = pack_h2(y[c + 2 * e] - lo_h(w[e]), y[c + 2 * e + 1] - hi_h(w[e]));
+            tc_st<32>(tmem + lane_base + buf * kTileKeys + kTileKeys / 2 + c / 2, w);
+          }
         }
         tc_wait_st();
         tc_fence_before();
@@ -452,30 +481,34 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       const int ktok = piece >> 2, kj = piece & 3;    // key piece: a token's words 4 g + kj
       const int vhi = D == 128 ? piece >> 5 : piece & 1, vl = D == 128 ? piece & 31 : piece >> 1;
       const int vi = vl >> 2, vj = vl & 3;            // value piece: tokens 8 vhi + 2 vj, + 1; words W vi ..
-      uint32_t kw[N], ks[N], vw[VW], vs[2];
-      bool there = false;
+      constexpr int H = kTileKeys / kBlkTokens / 4;   // blocks of a thread: bi, bi + 4
+      uint32_t kw[H][N], ks[H][N], vw[H][VW], vs[H][2];
+      uint32_t there = 0;  // a bit per block
       auto load = [&](int j) {  // this thread's pieces of the unit's tile j
-        const int k = (un.kt0 + j) * (kTileKeys / kBlkTokens) + bi;
-        there = false;
-        if (k * kBlkTokens < un.len) {
-          int in_page;
-          const int id = __ldg(p.table + un.b * p.table_stride + page_of(p, k, in_page));
-          if (id >= 0 && id < p.n_pages) {
-            there = true;
-            const uint8_t* blk = p.pages + id * p.page_stride + un.h * p.head_stride + in_page * B::kBytes;
-            auto get = [](const uint8_t* at, auto& v) {
-              if constexpr (sizeof(v) == 16) {
-                const uint4 x = *reinterpret_cast<const uint4*>(at);
-                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(at);
-                v[0] = x.x; v[1] = x.y;
-              }
-            };
-            get(blk + B::key_word(ktok, 0, kj), kw);
-            get(blk + B::key_sz(ktok, 0), ks);
-            get(blk + B::kV + piece * (VW * 4), vw);
-            get(blk + B::value_sz(8 * vhi + 2 * vj, vi * B::W / 4), vs);
+        there = 0;
+#pragma unroll
+        for (int hb = 0; hb < H; ++hb) {
+          const int k = (un.kt0 + j) * (kTileKeys / kBlkTokens) + bi + 4 * hb;
+          if (k * kBlkTokens < un.len) {
+            int in_page;
+            const int id = __ldg(p.table + un.b * p.table_stride + page_of(p, k, in_page));
+            if (id >= 0 && id < p.n_pages) {
+              there |= 1u << hb;
+              const uint8_t* blk = p.pages + id * p.page_stride + un.h * p.head_stride + in_page * B::kBytes;
+              auto get = [](const uint8_t* at, auto& v) {
+                if constexpr (sizeof(v) == 16) {
+                  const uint4 x = *reinterpret_cast<const uint4*>(at);
+                  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                } else {
+                  const uint2 x = *reinterpret_cast<const uint2*>(at);
+                  v[0] = x.x; v[1] = x.y;
+                }
+              };
+              get(blk + B::key_word(ktok, 0, kj), kw[hb]);
+              get(blk + B::key_sz(ktok, 0), ks[hb]);
+              get(blk + B::kV + piece * (VW * 4), vw[hb]);
+              get(blk + B::value_sz(8 * vhi + 2 * vj, vi * B::W / 4), vs[hb]);
+            }
           }
         }
       };
@@ -484,63 +517,66 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
         if (!(ok = warp_wait(s_full + st, ph ^ 1))) break;
         uint8_t* stage = smem + st * T::kStage;
-        const int t0 = (un.kt0 + j) * kTileKeys + bi * kBlkTokens;
-        const bool have = there;
-        // places without a token yet, or without a page: zeros, whatever their bits
-        uint32_t k_w[N], k_s[N], v_w[VW], v_s[2];
+        // values go to registers of their own, so that the next tile's loads start here
+        uint32_t v_w[H][VW], v_s[H][2];
 #pragma unroll
-        for (int g = 0; g < N; ++g) {
-          k_w[g] = kw[g];
-          k_s[g] = have && t0 + ktok < un.len ? ks[g] : 0u;
-        }
+        for (int hb = 0; hb < H; ++hb) {
+          const int t0 = (un.kt0 + j) * kTileKeys + (bi + 4 * hb) * kBlkTokens;
+          const bool have = there >> hb & 1;
+          // places without a token yet, or without a page: zeros, whatever their bits
 #pragma unroll
-        for (int e = 0; e < VW; ++e) v_w[e] = vw[e];
+          for (int e = 0; e < VW; ++e) v_w[hb][e] = vw[hb][e];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) v_s[e] = have && t0 + 8 * vhi + 2 * vj + e < un.len ? vs[e] : 0u;
-        if (j + 1 < nt) load(j + 1);
-
-        const int row = bi * kBlkTokens + ktok;
-        uint8_t* kd = stage + (row >> 3) * 128 + (row & 7) * 16;
+          for (int e = 0; e < 2; ++e) v_s[hb][e] = have && t0 + 8 * vhi + 2 * vj + e < un.len ? vs[hb][e] : 0u;
+          const bool key = have && t0 + ktok < un.len;
+          const int row = (bi + 4 * hb) * kBlkTokens + ktok;
+          uint8_t* kd = stage + (row >> 3) * 128 + (row & 7) * 16;
 #pragma unroll
-        for (int g = 0; g < N; ++g) {
-          const uint32_t s2 = hmul2(__byte_perm(k_s[g], 0, 0x1010), 0x38003800u);  // s / 2
-          uint32_t hi[4], lo[4];
+          for (int g = 0; g < N; ++g) {
+            ks[hb][g] = key ? ks[hb][g] : 0u;
+            const uint32_t s2 = hmul2(__byte_perm(ks[hb][g], 0, 0x1010), 0x38003800u);  // s / 2
+            uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = e < 2 ? k_w[g] : k_w[g] >> 8;
-            const uint32_t c = e & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
-                                     : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
-            hi[e] = hmul2(c, s2);
-            lo[e] = hfms2(c, s2, hi[e]);
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = e < 2 ? kw[hb][g] : kw[hb][g] >> 8;
+              const uint32_t c = e & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
+                                       : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
+              hi[e] = hmul2(c, s2);
+              lo[e] = hfms2(c, s2, hi[e]);
+            }
+            *reinterpret_cast<uint4*>(kd + (4 * g + kj) * T::kChunk) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(kd + T::kKey + (4 * g + kj) * T::kChunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
-          *reinterpret_cast<uint4*>(kd + (4 * g + kj) * T::kChunk) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(kd + T::kKey + (4 * g + kj) * T::kChunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        if (kj < 2) {  // zeros of the token's groups, against the sums' hi and against their lo
-          uint32_t z[4] = {0u, 0u, 0u, 0u};
+          if (kj < 2) {  // zeros of the token's groups, against the sums' hi and against their lo
+            uint32_t z[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-          for (int g = 0; g < N; g += 2) z[g / 2] = __byte_perm(k_s[g], k_s[g + 1], 0x7632);
-          *reinterpret_cast<uint4*>(stage + 2 * T::kKey + kj * (kTileKeys * 16) + row * 16) = make_uint4(z[0], z[1], z[2], z[3]);
+            for (int g = 0; g < N; g += 2) z[g / 2] = __byte_perm(ks[hb][g], ks[hb][g + 1], 0x7632);
+            *reinterpret_cast<uint4*>(stage + 2 * T::kKey + kj * (kTileKeys * 16) + row * 16) = make_uint4(z[0], z[1], z[2], z[3]);
+          }
+          if (piece == 0) s_hidden[(n & 3) * 8 + bi + 4 * hb] = have ? 0 : 1;
         }
-        if (piece == 0) s_hidden[(n & 3) * 4 + bi] = have ? 0 : 1;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full + st);
+        if (j + 1 < nt) load(j + 1);
 
         if (!(ok = warp_wait(o_done + st, ph ^ 1))) break;
-        uint8_t* vd = stage + 2 * T::kKey + T::kZ + (bi * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
 #pragma unroll
-        for (int e = 0; e < VW; ++e) {  // word e: token e / W, dim chunk W vi + e % W
-          const uint32_t s2 = __byte_perm(v_s[e / B::W], 0, 0x1010), z2 = __byte_perm(v_s[e / B::W], 0, 0x3232);
-          uint32_t o[4];
+        for (int hb = 0; hb < H; ++hb) {
+          uint8_t* vd = stage + 2 * T::kKey + T::kZ + ((bi + 4 * hb) * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t x = q < 2 ? v_w[e] : v_w[e] >> 8;
-            const uint32_t c = q & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
-                                     : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
-            o[q] = hfma2(c, s2, z2);
+          for (int e = 0; e < VW; ++e) {  // word e: token e / W, dim chunk W vi + e % W
+            const uint32_t s2 = __byte_perm(v_s[hb][e / B::W], 0, 0x1010), z2 = __byte_perm(v_s[hb][e / B::W], 0, 0x3232);
+            uint32_t o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t x = q < 2 ? v_w[hb][e] : v_w[hb][e] >> 8;
+              const uint32_t c = q & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
+                                       : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
+              o[q] = hfma2(c, s2, z2);
+            }
+            *reinterpret_cast<uint4*>(vd + (B::W * vi + e % B::W) * 128 + e / B::W * 16) = make_uint4(o[0], o[1], o[2], o[3]);
           }
-          *reinterpret_cast<uint4*>(vd + (B::W * vi + e % B::W) * 128 + e / B::W * 16) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -549,9 +585,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       n0 += nt;
     }
   } else {
-    // ================= MMA: one thread issues ====================================
+    // ================= MMA: a thread issues S, another one O =====================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp == kMmaWarp && lane == 0) {
+    // Operands are constants but for the shared memory's base: the instruction takes them from
+    // uniform registers, and values that vary cost more to bring there than the MMA itself.
+    const uint32_t base = smem_u32(smem) >> 4;
+    if (warp == kMmaWarp && lane == 0) {  // S = Q K^T
       uint32_t q_phase = 0;
       while (ok && next_unit(un)) {
         const int nt = un.kt1 - un.kt0;
@@ -559,42 +598,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           ok = wait(q_full, q_phase);
           q_phase ^= 1;
         }
-        const uint32_t id_s = idesc(kTileKeys, false), id_o = idesc(D, true);
-        // B descriptors: start address, bytes between core matrices along K (lbo) and along N (sbo)
-        auto lo_word = [](uint32_t at, uint32_t lbo) { return (at >> 4 & 0x3fff) | (lbo >> 4) << 16; };
-        constexpr uint32_t hi_word = 128 >> 4 | 1u << 14;
-        for (int j = 0; j <= nt && ok; ++j) {
-          if (j < nt) {
-            const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
-            ok = wait(k_full + st, ph) && wait(s_empty + st, ph ^ 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t ka = smem_u32(smem + st * T::kStage), ts = tmem + st * kTileKeys;
-            const uint32_t k_lo = lo_word(ka, T::kChunk), z_lo = lo_word(ka + 2 * T::kKey, kTileKeys * 16);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {  // hi, lo
-#pragma unroll
-              for (int c = 0; c < D / 8; c += 2)
-                tc_mma_ts(ts, tmem + T::kTQ + c * 4, k_lo + (half * T::kKey + c * T::kChunk) / 16, hi_word, id_s, (half | c) != 0);
-            }
-            tc_mma_ts(ts, tmem + T::kTSum, z_lo, hi_word, id_s, true);
-            tc_commit(s_full + st);
-          }
-          if (j > 0) {
-            const uint32_t n = n0 + j - 1, st = n & 1, ph = (n >> 1) & 1;
-            ok = wait(v_full + st, ph) && wait(p_full + st, ph);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t v_lo = lo_word(smem_u32(smem + st * T::kStage + 2 * T::kKey + T::kZ), D / 8 * 128);
-#pragma unroll
-            for (int half = 0; half < (LO ? 2 : 1); ++half) {
-#pragma unroll
-              for (int c = 0; c < kTileKeys / 8; c += 2)
-                tc_mma_ts(t_o, tmem + T::kTP + (LO ? half : st) * 32 + c * 4, v_lo + c * (D / 8 * 128) / 16, hi_word, id_o,
-                          j > 1 || (half | c) != 0);
-            }
-            tc_commit(o_done + st);
-          }
+        for (int j = 0; j < nt && ok; ++j) {
+          const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
+          ok = wait(o_done + st, ph ^ 1) && wait(k_full + st, ph);
+          if (!ok) break;
+          tc_fence_after();
+          if (st == 0) issue_qk<D, 0>(base); else issue_qk<D, 1>(base);
+          tc_commit(s_full + st);
+        }
+        n0 += nt;
+      }
+    } else if (warp == kMmaWarp + 1 && lane == 0) {  // O += P V
+      while (ok && next_unit(un)) {
+        const int nt = un.kt1 - un.kt0;
+        for (int j = 0; j < nt && ok; ++j) {
+          const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
+          ok = wait(v_full + st, ph) && wait(p_full + st, ph);
+          if (!ok) break;
+          tc_fence_after();
+          if (st == 0) issue_pv<D, LO, 0>(base, j > 0); else issue_pv<D, LO, 1>(base, j > 0);
+          tc_commit(o_done + st);
         }
         n0 += nt;
       }
@@ -604,13 +627,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (*s_abort && tid == kMmaWarp * 32) {  // a wait gave up: what was issued must end before the CTA does
+  if (*s_abort && (tid == kMmaWarp * 32 || tid == kMmaWarp * 32 + 32)) {  // a wait gave up: what was issued must end before the CTA does
     tc_commit(bars + 12);
     mbar_wait_bounded(bars + 12, 0, kTileWaitNs);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tc_dealloc(tmem, T::kCols);
+  if (warp == kMmaWarp) tc_dealloc(*s_tmem, T::kCols);
 }
 
 template <int D, bool LO>
