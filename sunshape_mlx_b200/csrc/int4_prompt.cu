@@ -71,6 +71,13 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32])
       "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+// (a, b) = (x, y) * s + (a, b), packed fp32
+__device__ __forceinline__ void fma_f32x2(float& a, float& b, float x, float y, float s) {
+  asm("{\n .reg .b64 t, u, v;\n mov.b64 t, {%0, %1};\n mov.b64 u, {%2, %3};\n mov.b64 v, {%4, %4};\n"
+      " fma.rn.f32x2 t, u, v, t;\n mov.b64 {%0, %1}, t;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y), "f"(s));
+}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -311,7 +318,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         }
         int ex = 0;
         if (big > 0.f && big < INFINITY) ex = 135 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
-        const float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
+        float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
+        // fac > 0, so that the largest product is the largest logit: a negative scale turns the
+        // queries round, a scale of 0 clears them
+        fac = p.scale == 0.f ? 1.f : 2.f * fabsf(p.scale) * kLog2e / up;
+        up = p.scale < 0.f ? -up : p.scale == 0.f ? 0.f : up;
         uint32_t qs[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};  // group sums: 8 hi, 8 lo
         uint32_t qo[D / 2];
         static_assert(B::G <= 8, "group sums fill one chunk");
@@ -343,7 +354,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < D / 2; c += 32) tc_st<32>(tmem + lane_base + T::kTQ + c, qo + c);
         tc_st<8>(tmem + lane_base + T::kTSum, qs);
-        fac = 2.f * p.scale * kLog2e / up;
         tc_wait_st();
         tc_fence_before();
       }
@@ -352,7 +362,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 
       int beg = 0, end = 0;
       if (r < un.rows) row_keys(p, un.nq, un.len, i, beg, end);
-      float m = kLow, l0 = 0.f, l1 = 0.f;
+      float m = kLow, l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
       for (int j = 0; j < nt; ++j) {
         const uint32_t n = n0 + j, buf = n & 1, ph = (n >> 1) & 1;
         if (!(ok = warp_wait(s_full + buf, ph))) break;
@@ -369,8 +379,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         const uint2 hid = *reinterpret_cast<const uint2*>(s_hidden + (n & 3) * 8);
 
         const int t0 = (un.kt0 + j) * kTileKeys;
-#pragma unroll
-        for (int e = 0; e < kTileKeys; e += 2) mul_f32x2(y[e], y[e + 1], fac);
         if (t0 < un.all0 || t0 + kTileKeys > un.all1 || (hid.x | hid.y) != 0) {
 #pragma unroll
           for (int e = 0; e < kTileKeys; ++e) {
@@ -378,14 +386,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             if (t0 + e >= end || t0 + e < beg || gone) y[e] = -INFINITY;
           }
         }
-        float top = y[0];
+        float tops[4] = {y[0], y[1], y[2], y[3]};
 #pragma unroll
-        for (int e = 0; e < kTileKeys; e += 2) top = fmax3(top, y[e], y[e + 1]);
+        for (int e = 4; e < kTileKeys; e += 2) tops[e / 2 % 4] = fmax3(tops[e / 2 % 4], y[e], y[e + 1]);
+        const float top = fmaxf(fmax3(tops[0], tops[1], tops[2]), tops[3]) * fac;  // fac > 0
         if (__any_sync(0xffffffffu, top > m + kSlack)) {
           const float mn = fmaxf(m, top), f = ex2(m - mn);
           m = mn;
           l0 *= f;
           l1 *= f;
+          l2 *= f;
+          l3 *= f;
           if (j > 0) {  // O holds the tiles before: all of them, once the last one's P V is done
             if (!(ok = warp_wait(o_done + (buf ^ 1), ((n - 1) >> 1) & 1))) break;
             tc_fence_after();
@@ -410,10 +421,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           for (int e = 0; e < 32; ++e) {
             float& a = y[c + 2 * e];
             float& b = y[c + 2 * e + 1];
-            add_f32x2(a, b, -m, -m);
-            a = ex2(a);
-            b = ex2(b);
-            add_f32x2(l0, l1, a, b);
+            float x = -m, z = -m;
+            fma_f32x2(x, z, a, b, fac);
+            a = ex2(x);
+            b = ex2(z);
+            add_f32x2(e & 1 ? l2 : l0, e & 1 ? l3 : l1, a, b);
             w[e] = pack_h2(a, b);
           }
           tc_st<32>(tmem + lane_base + buf * kTileKeys + c / 2, w);
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         if (lane == 0) mbar_arrive(p_full + buf);
       }
       // ---- output ----
-      const float l = l0 + l1;
+      const float l = (l0 + l1) + (l2 + l3);
       if (ok && nt > 0) ok = warp_wait(o_done + ((n0 + nt - 1) & 1), ((n0 + nt - 1) >> 1) & 1);
       if (ok) {
         tc_fence_after();
@@ -484,17 +496,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       constexpr int H = kTileKeys / kBlkTokens / 4;   // blocks of a thread: bi, bi + 4
       uint32_t kw[H][N], ks[H][N], vw[H][VW], vs[H][2];
       uint32_t there = 0;  // a bit per block
-      auto load = [&](int j) {  // this thread's pieces of the unit's tile j
-        there = 0;
+      int id[H], in_page[H];
+      auto look_up = [&](int j) {  // pages of the unit's tile j: a tile before they are needed
 #pragma unroll
         for (int hb = 0; hb < H; ++hb) {
           const int k = (un.kt0 + j) * (kTileKeys / kBlkTokens) + bi + 4 * hb;
-          if (k * kBlkTokens < un.len) {
-            int in_page;
-            const int id = __ldg(p.table + un.b * p.table_stride + page_of(p, k, in_page));
-            if (id >= 0 && id < p.n_pages) {
+          id[hb] = -1;
+          if (j < nt && k * kBlkTokens < un.len) id[hb] = __ldg(p.table + un.b * p.table_stride + page_of(p, k, in_page[hb]));
+        }
+      };
+      auto load = [&]() {  // this thread's pieces of the tile that was looked up
+        there = 0;
+#pragma unroll
+        for (int hb = 0; hb < H; ++hb) {
+          if (id[hb] >= 0 && id[hb] < p.n_pages) {
+            {
               there |= 1u << hb;
-              const uint8_t* blk = p.pages + id * p.page_stride + un.h * p.head_stride + in_page * B::kBytes;
+              const uint8_t* blk = p.pages + id[hb] * p.page_stride + un.h * p.head_stride + in_page[hb] * B::kBytes;
               auto get = [](const uint8_t* at, auto& v) {
                 if constexpr (sizeof(v) == 16) {
                   const uint4 x = *reinterpret_cast<const uint4*>(at);
@@ -512,7 +530,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           }
         }
       };
-      if (nt > 0) load(0);
+      look_up(0);
+      load();
+      look_up(1);
       for (int j = 0; j < nt; ++j) {
         const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
         if (!(ok = warp_wait(s_full + st, ph ^ 1))) break;
@@ -558,7 +578,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full + st);
-        if (j + 1 < nt) load(j + 1);
+        load();
+        look_up(j + 2);
 
         if (!(ok = warp_wait(o_done + st, ph ^ 1))) break;
 #pragma unroll
