@@ -34,10 +34,11 @@ namespace ss {
 namespace {
 
 constexpr int kTileRows = 128, kTileKeys = 128;
-constexpr int kSoftWarps = 4, kDecWarps = 8, kMmaWarp = kSoftWarps + kDecWarps;  // two warps issue MMAs
-constexpr int kTileWarps = 16, kTileThreads = kTileWarps * 32;  // whole warpgroups: registers are moved between them
-// Registers of a thread: 128 at launch; 4 * 208 + 8 * 104 + 4 * 64 = 480 * 4 of the 512 * 4 there are.
-constexpr int kSoftRegs = 208, kDecRegs = 104, kMmaRegs = 64;
+constexpr int kMmaWarp = 0, kSoftWarp = 4, kSoftWarps = 8, kDecWarp = kSoftWarp + kSoftWarps, kDecWarps = 8;  // two warps issue MMAs
+constexpr int kTileWarps = 20, kTileThreads = kTileWarps * 32;  // whole warpgroups: registers are moved between them
+// Registers of a thread: 96 at launch; 8 * 120 + 8 * 88 + 4 * 64 = 20 * 96.
+constexpr int kSoftRegs = 120, kDecRegs = 88, kMmaRegs = 64;
+constexpr int kHalfKeys = kTileKeys / 2;  // of a softmax thread: a row is two threads' work
 constexpr uint64_t kTileWaitNs = 2000000000ull;
 constexpr int kTileWaitCode = 32;
 
@@ -49,7 +50,8 @@ struct Tile {
   static constexpr int kVal = kTileKeys * D * 2;    // [8 tokens][dim chunk][token] 16 bytes
   static constexpr int kStage = 2 * kKey + kZ + kVal;
   static constexpr int kOffMisc = 2 * kStage;
-  static constexpr int kSmem = kOffMisc + 512 + kTileThreads * 4;
+  static constexpr int kOffRow = kOffMisc + 512 + kTileThreads * 4;
+  static constexpr int kSmem = kOffRow + 6 * kTileRows * 4;
   // TMEM columns: two S, each overwritten by its P (hi, then lo; two fp16 a column), O, Q, its group sums
   static constexpr int kTO = 2 * kTileKeys, kTQ = kTO + D, kTSum = kTQ + D / 2;
   static constexpr int kCols = 512;
@@ -90,6 +92,12 @@ __device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t* v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) w[i] = v[i];
     tc_st32(taddr, w);
+  } else if constexpr (N == 16) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
   } else {
     static_assert(N == 8, "columns");
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
@@ -177,6 +185,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   uint8_t* s_hidden = reinterpret_cast<uint8_t*>(s_tmem + 2);  // [4][8] blocks of a tile without a page; read before S is freed
   int* s_sum = reinterpret_cast<int*>(smem + T::kOffMisc + 256);      // [16] warps' units
   int* s_cum = reinterpret_cast<int*>(smem + T::kOffMisc + 512);      // [threads] units before a thread's requests
+  float* s_top = reinterpret_cast<float*>(smem + T::kOffRow);         // [2 tiles][2 halves][128] largest logits of a row
+  float* s_fac = s_top + 4 * kTileRows;                               // [128] from logits to base 2
+  float* s_l = s_fac + kTileRows;                                     // [128] a half's sum
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -189,7 +200,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       mbar_init(s_full + s, 1);
       mbar_init(p_full + s, kSoftWarps);
     }
-    mbar_init(q_full, kSoftWarps);
+    mbar_init(q_full, 4);
     mbar_init(bars + 12, 2);  // end of an abandoned unit's MMAs
     *s_abort = 0;
     fence_mbar_init();
@@ -282,22 +293,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   Unit un;
   uint32_t n0 = 0;  // tiles of this CTA's earlier units: the barriers' phases go on
   bool ok = true;   // no wait gave up
-  if (warp < kSoftWarps) {
-    // ================= softmax: a thread per row ================================
+  if (warp >= kSoftWarp && warp < kDecWarp) {
+    // ================= softmax: two threads per row, 64 keys of a tile each =======
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    const int pair = 1 + (warp & 3);  // named barrier of the two warps that share 32 rows
+    // Both warps of a pair come here equally often, or one gives up in a wait: it then arrives
+    // once (below), and its partner finds the flag set.
+    auto pair_sync = [&]() -> bool {
+      named_bar_sync(pair, 64);
+      return __any_sync(0xffffffffu, *s_abort) == 0;
+    };
     while (ok && next_unit(un)) {
       const int nt = un.kt1 - un.kt0;
-      const int r = tid, rr = un.row0 + r, i = rr / p.grp, hd = un.h * p.grp + rr % p.grp;
+      const int half = (warp - kSoftWarp) >> 2, r = tid & (kTileRows - 1), rr = un.row0 + r, i = rr / p.grp, hd = un.h * p.grp + rr % p.grp;
       const int64_t tok = un.tok0 + (int64_t)i;
       const bool live = r < un.rows && tok < p.n_tokens;
-      const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-      float fac;
-      {  // the row's queries, scaled by a power of two into [256, 512), and its group sums
-        uint4 x[D / 8];
+      const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+      if (half == 0) {  // the row's queries, scaled by a power of two into [256, 512), and its group sums
         const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + tok * p.q_st + hd * p.q_sh;
-        float big = 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
+        auto get8 = [&](int c, float (&f)[8]) {
           uint32_t w[4] = {0u, 0u, 0u, 0u};
           if (live) {
             if (p.q_vec) {
@@ -308,42 +322,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
               for (int e = 0; e < 4; ++e) w[e] = qp[c * 8 + 2 * e] | (uint32_t)qp[c * 8 + 2 * e + 1] << 16;
             }
           }
-          x[c] = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float a = p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16);
-            const float b = p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u);
-            big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
+            f[2 * e] = p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16);
+            f[2 * e + 1] = p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u);
           }
+        };
+        float big = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          float f[8];
+          get8(c, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
         }
         int ex = 0;
         if (big > 0.f && big < INFINITY) ex = 135 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
         float up = ex > 126 ? __uint_as_float(253u << 23) : __uint_as_float((uint32_t)(127 + ex) << 23);
         // fac > 0, so that the largest product is the largest logit: a negative scale turns the
         // queries round, a scale of 0 clears them
-        fac = p.scale == 0.f ? 1.f : 2.f * fabsf(p.scale) * kLog2e / up;
+        s_fac[r] = p.scale == 0.f ? 1.f : 2.f * fabsf(p.scale) * kLog2e / up;
         up = p.scale < 0.f ? -up : p.scale == 0.f ? 0.f : up;
         uint32_t qs[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};  // group sums: 8 hi, 8 lo
-        uint32_t qo[D / 2];
         static_assert(B::G <= 8, "group sums fill one chunk");
         float sum[B::G];
 #pragma unroll
-        for (int g = 0; g < B::G; ++g) sum[g] = 0.f;
+        for (int g = 0; g < B::G; ++g) {
+          sum[g] = 0.f;
+          uint32_t qo[16];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-          float f[8];
+          for (int c = 0; c < 4; ++c) {
+            float f[8];
+            get8(g * 4 + c, f);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[2 * e] = (p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16)) * up;
-            f[2 * e + 1] = (p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u)) * up;
+            for (int e = 0; e < 4; ++e) {  // dims (e, e + 4) side by side, as the key words' nibbles come
+              qo[c * 4 + e] = pack_h2(f[e] * up, f[e + 4] * up);
+              sum[g] += lo_h(qo[c * 4 + e]) + hi_h(qo[c * 4 + e]);
+            }
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {  // dims (e, e + 4) side by side, as the key words' nibbles come
-            const uint32_t o = pack_h2(f[e], f[e + 4]);
-            qo[c * 4 + e] = o;
-            sum[c / 4] += lo_h(o) + hi_h(o);
-          }
+          tc_st<16>(tmem + lane_base + T::kTQ + g * 16, qo);
         }
 #pragma unroll
         for (int g = 0; g < B::G; g += 2) {  // halved, as the keys are
@@ -351,14 +368,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           qs[g / 2] = pack_h2(a, b);
           qs[4 + g / 2] = pack_h2(a - lo_h(qs[g / 2]), b - hi_h(qs[g / 2]));
         }
-#pragma unroll
-        for (int c = 0; c < D / 2; c += 32) tc_st<32>(tmem + lane_base + T::kTQ + c, qo + c);
         tc_st<8>(tmem + lane_base + T::kTSum, qs);
         tc_wait_st();
         tc_fence_before();
       }
-      __syncwarp();
-      if (lane == 0 && nt > 0) mbar_arrive(q_full);  // and O of the unit before has been read
+      if (!(ok = pair_sync())) break;
+      const float fac = s_fac[r];
+      if (lane == 0 && half == 0 && nt > 0) mbar_arrive(q_full);  // and O of the unit before has been read
 
       int beg = 0, end = 0;
       if (r < un.rows) row_keys(p, un.nq, un.len, i, beg, end);
@@ -367,29 +383,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         const uint32_t n = n0 + j, buf = n & 1, ph = (n >> 1) & 1;
         if (!(ok = warp_wait(s_full + buf, ph))) break;
         tc_fence_after();
-        float y[kTileKeys];
+        float y[kHalfKeys];
         {
-          uint32_t v[kTileKeys / 32][32];
-#pragma unroll
-          for (int c = 0; c < kTileKeys / 32; ++c) tc_ld32(tmem + lane_base + buf * kTileKeys + c * 32, v[c]);
+          uint32_t v0[32], v1[32];
+          tc_ld32(tmem + lane_base + buf * kTileKeys + half * kHalfKeys, v0);
+          tc_ld32(tmem + lane_base + buf * kTileKeys + half * kHalfKeys + 32, v1);
           tc_wait_ld();
 #pragma unroll
-          for (int c = 0; c < kTileKeys; ++c) y[c] = __uint_as_float(v[c / 32][c % 32]);
-        }
-        const uint2 hid = *reinterpret_cast<const uint2*>(s_hidden + (n & 3) * 8);
-
-        const int t0 = (un.kt0 + j) * kTileKeys;
-        if (t0 < un.all0 || t0 + kTileKeys > un.all1 || (hid.x | hid.y) != 0) {
-#pragma unroll
-          for (int e = 0; e < kTileKeys; ++e) {
-            const uint32_t gone = (e < 64 ? hid.x : hid.y) >> (e / 16 % 4 * 8) & 1;
-            if (t0 + e >= end || t0 + e < beg || gone) y[e] = -INFINITY;
+          for (int e = 0; e < 32; ++e) {
+            y[e] = __uint_as_float(v0[e]);
+            y[32 + e] = __uint_as_float(v1[e]);
           }
+        }
+        const uint32_t hid = *reinterpret_cast<const uint32_t*>(s_hidden + (n & 3) * 8 + half * 4);
+
+        const int t0 = (un.kt0 + j) * kTileKeys + half * kHalfKeys;
+        if (t0 < un.all0 || t0 + kHalfKeys > un.all1 || hid != 0) {
+#pragma unroll
+          for (int e = 0; e < kHalfKeys; ++e)
+            if (t0 + e >= end || t0 + e < beg || (hid >> (e / 16 * 8) & 1)) y[e] = -INFINITY;
         }
         float tops[4] = {y[0], y[1], y[2], y[3]};
 #pragma unroll
-        for (int e = 4; e < kTileKeys; e += 2) tops[e / 2 % 4] = fmax3(tops[e / 2 % 4], y[e], y[e + 1]);
-        const float top = fmaxf(fmax3(tops[0], tops[1], tops[2]), tops[3]) * fac;  // fac > 0
+        for (int e = 4; e < kHalfKeys; e += 2) tops[e / 2 % 4] = fmax3(tops[e / 2 % 4], y[e], y[e + 1]);
+        float top = fmaxf(fmax3(tops[0], tops[1], tops[2]), tops[3]) * fac;  // fac > 0
+        // both halves of a row go by the same reference
+        s_top[(buf * 2 + half) * kTileRows + r] = top;
+        tc_fence_before();
+        if (!(ok = pair_sync())) break;  // and both have read S
+        tc_fence_after();
+        top = fmaxf(top, s_top[(buf * 2 + (half ^ 1)) * kTileRows + r]);
         if (__any_sync(0xffffffffu, top > m + kSlack)) {
           const float mn = fmaxf(m, top), f = ex2(m - mn);
           m = mn;
@@ -400,14 +423,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           if (j > 0) {  // O holds the tiles before: all of them, once the last one's P V is done
             if (!(ok = warp_wait(o_done + (buf ^ 1), ((n - 1) >> 1) & 1))) break;
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 32) {  // a half of the dims each
               uint32_t v[32];
-              tc_ld32(t_o + lane_base + c, v);
+              tc_ld32(t_o + lane_base + half * (D / 2) + c, v);
               tc_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-              tc_st32(t_o + lane_base + c, v);
+              tc_st32(t_o + lane_base + half * (D / 2) + c, v);
             }
             tc_wait_st();
             tc_fence_before();
@@ -415,10 +438,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         }
         // P over the S it comes from
 #pragma unroll
-        for (int c = 0; c < kTileKeys; c += 64) {
-          uint32_t w[32];
+        for (int c = 0; c < kHalfKeys; c += 32) {
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < 16; ++e) {
             float& a = y[c + 2 * e];
             float& b = y[c + 2 * e + 1];
             float x = -m, z = -m;
@@ -428,11 +451,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             add_f32x2(e & 1 ? l2 : l0, e & 1 ? l3 : l1, a, b);
             w[e] = pack_h2(a, b);
           }
-          tc_st<32>(tmem + lane_base + buf * kTileKeys + c / 2, w);
+          const uint32_t at = tmem + lane_base + buf * kTileKeys + (half * kHalfKeys + c) / 2;
+          tc_st<16>(at, w);
           if constexpr (LO) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = pack_h2(y[c + 2 * e] - lo_h(w[e]), y[c + 2 * e + 1] - hi_h(w[e]));
-            tc_st<32>(tmem + lane_base + buf * kTileKeys + kTileKeys / 2 + c / 2, w);
+            for (int e = 0; e < 16; ++e) w[e] = pack_h2(y[c + 2 * e] - lo_h(w[e]), y[c + 2 * e + 1] - hi_h(w[e]));
+            tc_st<16>(at + kTileKeys / 2, w);
           }
         }
         tc_wait_st();
@@ -441,17 +465,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         if (lane == 0) mbar_arrive(p_full + buf);
       }
       // ---- output ----
-      const float l = (l0 + l1) + (l2 + l3);
+      float l = (l0 + l1) + (l2 + l3);
+      if (half == 1) s_l[r] = l;
+      ok = ok && pair_sync();
+      if (half == 0) s_top[r] = l += s_l[r];
+      ok = ok && pair_sync();
+      l = s_top[r];
       if (ok && nt > 0) ok = warp_wait(o_done + ((n0 + nt - 1) & 1), ((n0 + nt - 1) >> 1) & 1);
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (tok * p.hq + hd) * D;
+        uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (tok * p.hq + hd) * D + half * (D / 2);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < D / 2; c += 32) {
           uint32_t v[32];
           if (nt > 0) {
-            tc_ld32(t_o + lane_base + c, v);
+            tc_ld32(t_o + lane_base + half * (D / 2) + c, v);
             tc_wait_ld();
           } else {
 #pragma unroll
@@ -477,30 +506,31 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             }
           }
         }
-        if (live && p.lse) p.lse[tok * p.hq + hd] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+        if (live && p.lse && half == 0) p.lse[tok * p.hq + hd] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
         tc_fence_before();
       }
       n0 += nt;
     }
-  } else if (warp < kMmaWarp) {
+    if (!ok) asm volatile("bar.arrive %0, 64;" ::"r"(pair) : "memory");
+  } else if (warp >= kDecWarp) {
     // ================= decode: 64 threads per block of 16 tokens ================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecRegs));
     while (ok && next_unit(un)) {
       const int nt = un.kt1 - un.kt0;
-      const int d = tid - kSoftWarps * 32, bi = d >> 6, piece = d & 63;
+      const int d = tid - kDecWarp * 32, bi = d >> 6, piece = d & 63;
       constexpr int N = B::N, VW = 2 * B::W;          // key words and value words of a thread
       static_assert(B::G == N, "one key piece per token and lane");
       const int ktok = piece >> 2, kj = piece & 3;    // key piece: a token's words 4 g + kj
       const int vhi = D == 128 ? piece >> 5 : piece & 1, vl = D == 128 ? piece & 31 : piece >> 1;
       const int vi = vl >> 2, vj = vl & 3;            // value piece: tokens 8 vhi + 2 vj, + 1; words W vi ..
-      constexpr int H = kTileKeys / kBlkTokens / 4;   // blocks of a thread: bi, bi + 4
+      constexpr int DB = kDecWarps / 2, H = kTileKeys / kBlkTokens / DB;  // blocks of a thread: bi, bi + DB, ..
       uint32_t kw[H][N], ks[H][N], vw[H][VW], vs[H][2];
       uint32_t there = 0;  // a bit per block
       int id[H], in_page[H];
       auto look_up = [&](int j) {  // pages of the unit's tile j: a tile before they are needed
 #pragma unroll
         for (int hb = 0; hb < H; ++hb) {
-          const int k = (un.kt0 + j) * (kTileKeys / kBlkTokens) + bi + 4 * hb;
+          const int k = (un.kt0 + j) * (kTileKeys / kBlkTokens) + bi + DB * hb;
           id[hb] = -1;
           if (j < nt && k * kBlkTokens < un.len) id[hb] = __ldg(p.table + un.b * p.table_stride + page_of(p, k, in_page[hb]));
         }
@@ -541,7 +571,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         uint32_t v_w[H][VW], v_s[H][2];
 #pragma unroll
         for (int hb = 0; hb < H; ++hb) {
-          const int t0 = (un.kt0 + j) * kTileKeys + (bi + 4 * hb) * kBlkTokens;
+          const int t0 = (un.kt0 + j) * kTileKeys + (bi + DB * hb) * kBlkTokens;
           const bool have = there >> hb & 1;
           // places without a token yet, or without a page: zeros, whatever their bits
 #pragma unroll
@@ -549,7 +579,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < 2; ++e) v_s[hb][e] = have && t0 + 8 * vhi + 2 * vj + e < un.len ? vs[hb][e] : 0u;
           const bool key = have && t0 + ktok < un.len;
-          const int row = (bi + 4 * hb) * kBlkTokens + ktok;
+          const int row = (bi + DB * hb) * kBlkTokens + ktok;
           uint8_t* kd = stage + (row >> 3) * 128 + (row & 7) * 16;
 #pragma unroll
           for (int g = 0; g < N; ++g) {
@@ -573,7 +603,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             for (int g = 0; g < N; g += 2) z[g / 2] = __byte_perm(ks[hb][g], ks[hb][g + 1], 0x7632);
             *reinterpret_cast<uint4*>(stage + 2 * T::kKey + kj * (kTileKeys * 16) + row * 16) = make_uint4(z[0], z[1], z[2], z[3]);
           }
-          if (piece == 0) s_hidden[(n & 3) * 8 + bi + 4 * hb] = have ? 0 : 1;
+          if (piece == 0) s_hidden[(n & 3) * 8 + bi + DB * hb] = have ? 0 : 1;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -584,7 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         if (!(ok = warp_wait(o_done + st, ph ^ 1))) break;
 #pragma unroll
         for (int hb = 0; hb < H; ++hb) {
-          uint8_t* vd = stage + 2 * T::kKey + T::kZ + ((bi + 4 * hb) * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
+          uint8_t* vd = stage + 2 * T::kKey + T::kZ + ((bi + DB * hb) * 2 + vhi) * (D / 8 * 128) + 2 * vj * 16;
 #pragma unroll
           for (int e = 0; e < VW; ++e) {  // word e: token e / W, dim chunk W vi + e % W
             const uint32_t s2 = __byte_perm(v_s[hb][e / B::W], 0, 0x1010), z2 = __byte_perm(v_s[hb][e / B::W], 0, 0x3232);
