@@ -256,22 +256,35 @@ def stream_ptr(device: torch.device | None = None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-class _Here:
-    """A context that does nothing: the tensors are on the current device."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_CTX = _Here()
+# ------------------------------------------------------------------ short calls
+# A serving step makes many calls whose kernels take a few microseconds, so
+# what a wrapper does besides checking and launching is kept short: entry
+# points are looked up once, and device and stream come from torch's raw
+# getters (no Device or Stream objects).
+_FNS: dict = {}
+current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def on_device(device: torch.device):
-    """Makes `device` current for a launch (free where it is already)."""
-    return _HERE_CTX if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def entry(fn: str):
+    """C entry point `fn` (a bound ctypes function)."""
+    f = _FNS.get(fn)
+    if f is None:
+        f = _FNS[fn] = getattr(load(), fn)
+    return f
+
+
+def launch(fn: str, index: int, *args) -> None:
+    """Calls entry point `fn` with `args` and the current stream of CUDA device
+    `index`, which is made current for the launch if it is not."""
+    f = _FNS.get(fn) or entry(fn)
+    if current_device() == index:
+        rc = f(*args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, raw_stream(index))
+    if rc:
+        raise SunShapeCudaError(fn, rc, last_error())
 
 
 def dtype_code(dt: torch.dtype) -> int:

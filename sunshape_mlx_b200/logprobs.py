@@ -35,23 +35,25 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     nothing else gives -inf and entropy 0. A row with NaN or +inf gives NaN
     everywhere and ids of -1.
     """
-    L.require_cuda(logits, targets)
-    if logits.dim() != 2 or not logits.shape[1]:
+    if not (logits.is_cuda and targets.is_cuda):
+        L.require_cuda(logits, targets)
+    if logits.dim() != 2 or not logits.size(1):
         raise ValueError("logits must be (rows, vocab)")
     n, vocab = logits.shape
-    if logits.stride(1) != 1 and vocab > 1:
+    row_stride, stride = logits.stride()
+    if stride != 1 and vocab > 1:
         raise ValueError("logits must be contiguous in vocab")
-    dev = logits.device
-    if targets.dtype != torch.int64 or targets.shape != (n,) or targets.device != dev or not targets.is_contiguous():
+    index = logits.get_device()
+    if (targets.dtype is not torch.int64 or targets.dim() != 1 or targets.size(0) != n
+            or targets.get_device() != index or not targets.is_contiguous()):
         raise ValueError("targets must be a contiguous int64 tensor with one element per row, on the logits' device")
     if not 0 <= top_k <= _MAX_TOP:
         raise ValueError(f"top_k must be in [0, {_MAX_TOP}], got {top_k}")
     dt = L.dtype_code(logits.dtype)
-    out = torch.empty((2 + top_k) * n, dtype=torch.float32, device=dev)
-    lp, ent, top = out.split((n, n, top_k * n))
-    ids = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-    with L.on_device(dev):
-        L.call("ss_token_logprobs", logits.data_ptr(), dt, n, logits.stride(0), vocab,
-               targets.data_ptr(), top_k, lp.data_ptr(), ent.data_ptr(), ids.data_ptr(),
-               top.data_ptr(), L.stream_ptr(dev))
+    out = torch.empty((2 + top_k) * n, dtype=torch.float32, device=logits.device)
+    lp, ent, top = out.split_with_sizes((n, n, top_k * n))
+    ids = torch.empty((n, top_k), dtype=torch.int32, device=logits.device)
+    at = out.data_ptr()
+    L.launch("ss_token_logprobs", index, logits.data_ptr(), dt, n, row_stride, vocab, targets.data_ptr(),
+             top_k, at, at + 4 * n, ids.data_ptr(), at + 8 * n)
     return TokenLogprobs(lp, ent, ids, top.view(n, top_k))

@@ -51,24 +51,30 @@ class StepPlan(NamedTuple):
     status: torch.Tensor
 
 
-def _int32(name: str, t: torch.Tensor, dims: int, device) -> None:
-    if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.numel() and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be a contiguous {dims}-D int32 tensor on {device}")
+_I32, _I64, _U8 = torch.int32, torch.int64, torch.uint8
 
 
-def _check_tables(seq_lens, block_table, free_pages, n_free, page_size) -> None:
-    L.require_cuda(seq_lens)
-    dev = seq_lens.device
-    _int32("seq_lens", seq_lens, 1, dev)
-    _int32("block_table", block_table, 2, dev)
-    _int32("free_pages", free_pages, 1, dev)
-    _int32("n_free", n_free, 1, dev)
-    if block_table.shape[0] != seq_lens.shape[0] or n_free.shape[0] != 1:
+def _int32(name: str, t: torch.Tensor, dims: int, index: int) -> None:
+    if t.dtype is not _I32 or t.dim() != dims or t.get_device() != index or (t.stride(-1) != 1 and t.numel()):
+        raise ValueError(f"{name} must be a contiguous {dims}-D int32 tensor on CUDA device {index}")
+
+
+def _check_tables(seq_lens, block_table, free_pages, n_free, page_size) -> int:
+    """Checks what a step's tables share; returns the index of their device."""
+    if not seq_lens.is_cuda:
+        L.require_cuda(seq_lens)
+    index = seq_lens.get_device()
+    _int32("seq_lens", seq_lens, 1, index)
+    _int32("block_table", block_table, 2, index)
+    _int32("free_pages", free_pages, 1, index)
+    _int32("n_free", n_free, 1, index)
+    if block_table.size(0) != seq_lens.size(0) or n_free.size(0) != 1:
         raise ValueError("block_table needs a row per request, n_free one element")
-    if block_table.stride(0) < block_table.shape[1]:
+    if block_table.stride(0) < block_table.size(1):
         raise ValueError("the rows of block_table must not overlap")
     if page_size < 16 or page_size % 16:
         raise ValueError(f"page_size must be a multiple of 16, got {page_size}")
+    return index
 
 
 def plan_step(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_table: torch.Tensor,
@@ -84,23 +90,24 @@ def plan_step(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_table: torch.T
     step of fewer tokens leaves slots of -1 at the end). If the step does not
     fit, nothing is allocated and ``status`` says why.
     """
-    _check_tables(seq_lens, block_table, free_pages, n_free, page_size)
-    dev = seq_lens.device
-    _int32("q_lens", q_lens, 1, dev)
-    n = seq_lens.shape[0]
-    if q_lens.shape[0] != n:
+    index = _check_tables(seq_lens, block_table, free_pages, n_free, page_size)
+    _int32("q_lens", q_lens, 1, index)
+    n = seq_lens.size(0)
+    if q_lens.size(0) != n:
         raise ValueError("q_lens and seq_lens must have one element per request")
     if n_tokens < 0:
         raise ValueError("n_tokens must not be negative")
-    slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
-    cu, pos, req, lens, left, status = torch.empty(
-        2 * n + 3 + 2 * n_tokens, dtype=torch.int32, device=dev).split((n + 1, n_tokens, n_tokens, n, 1, 1))
-    with L.on_device(dev):
-        L.call("ss_plan_step", seq_lens.data_ptr(), q_lens.data_ptr(), n, block_table.data_ptr(),
-               block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0],
-               n_free.data_ptr(), page_size, n_tokens, cu.data_ptr(), pos.data_ptr(), req.data_ptr(),
-               slots.data_ptr(), lens.data_ptr(), left.data_ptr(), status.data_ptr(),
-               L.stream_ptr(dev))
+    slots = torch.empty(n_tokens, dtype=_I64, device=seq_lens.device)
+    out = torch.empty(2 * n + 3 + 2 * n_tokens, dtype=_I32, device=seq_lens.device)
+    cu, pos, req, lens, left, status = out.split_with_sizes((n + 1, n_tokens, n_tokens, n, 1, 1))
+    at = out.data_ptr()
+    at_pos = at + 4 * (n + 1)
+    at_req = at_pos + 4 * n_tokens
+    at_lens = at_req + 4 * n_tokens
+    L.launch("ss_plan_step", index, seq_lens.data_ptr(), q_lens.data_ptr(), n, block_table.data_ptr(),
+             block_table.stride(0), block_table.size(1), free_pages.data_ptr(), free_pages.size(0),
+             n_free.data_ptr(), page_size, n_tokens, at, at_pos, at_req, slots.data_ptr(), at_lens,
+             at_lens + 4 * n, at_lens + 4 * n + 4)
     return StepPlan(cu, pos, req, slots, lens, left, status)
 
 
@@ -109,16 +116,14 @@ def release_pages(seq_lens: torch.Tensor, done: torch.Tensor, block_table: torch
     """Pushes the pages of every request with ``done`` (n,) bool back onto the
     stack ``free_pages`` and clears its table row (-1). Returns (seq_lens,
     n_free, status) after it."""
-    _check_tables(seq_lens, block_table, free_pages, n_free, page_size)
-    dev, n = seq_lens.device, seq_lens.shape[0]
-    if done.dtype != torch.bool or done.shape != (n,) or done.device != dev or not done.is_contiguous():
+    index = _check_tables(seq_lens, block_table, free_pages, n_free, page_size)
+    n = seq_lens.size(0)
+    if done.dtype is not torch.bool or done.shape != (n,) or done.get_device() != index or not done.is_contiguous():
         raise ValueError("done must be a contiguous bool tensor with one element per request")
-    lens, left, status = torch.empty(n + 2, dtype=torch.int32, device=dev).split((n, 1, 1))
-    with L.on_device(dev):
-        L.call("ss_release_pages", seq_lens.data_ptr(), done.data_ptr(), n, block_table.data_ptr(),
-               block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0],
-               n_free.data_ptr(), page_size, lens.data_ptr(), left.data_ptr(), status.data_ptr(),
-               L.stream_ptr(dev))
+    lens, left, status = torch.empty(n + 2, dtype=_I32, device=seq_lens.device).split_with_sizes((n, 1, 1))
+    L.launch("ss_release_pages", index, seq_lens.data_ptr(), done.data_ptr(), n, block_table.data_ptr(),
+             block_table.stride(0), block_table.size(1), free_pages.data_ptr(), free_pages.size(0),
+             n_free.data_ptr(), page_size, lens.data_ptr(), left.data_ptr(), status.data_ptr())
     return lens, left, status
 
 
@@ -141,14 +146,15 @@ def _page_tokens(nbytes: int, head_dim: int) -> int:
 
 
 def _check_pool(pages: torch.Tensor, head_dim: int) -> int:
-    L.require_cuda(pages)
-    if pages.dtype != torch.uint8 or pages.dim() != 3 or pages.stride(2) != 1 or not pages.shape[0]:
+    if not pages.is_cuda:
+        L.require_cuda(pages)
+    if pages.dtype is not _U8 or pages.dim() != 3 or pages.stride(2) != 1 or not pages.size(0):
         raise ValueError("pages must be uint8 (n_pages, n_kv_heads, bytes), contiguous in the last dim")
-    return _page_tokens(pages.shape[2], head_dim)
+    return _page_tokens(pages.size(2), head_dim)
 
 
-def _check_slots(slots: torch.Tensor, n: int, device) -> None:
-    if slots.dtype != torch.int64 or slots.shape != (n,) or slots.device != device or not slots.is_contiguous():
+def _check_slots(slots: torch.Tensor, n: int, index: int) -> None:
+    if slots.dtype is not _I64 or slots.dim() != 1 or slots.size(0) != n or slots.get_device() != index or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int64 tensor with one element per token, on the pages' device")
 
 
@@ -157,23 +163,24 @@ def int4_append(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor, p
     bf16, into the pages at ``slots`` (n,) int64; -1 skips a token. Slots of
     one call must differ. Magnitudes above 2^15 saturate; a NaN makes its
     group of 32 dims read as NaN."""
-    L.require_cuda(keys, values)
-    if keys.dim() != 3 or keys.shape != values.shape or keys.dtype != values.dtype:
+    if not (keys.is_cuda and values.is_cuda):
+        L.require_cuda(keys, values)
+    if keys.dim() != 3 or keys.shape != values.shape or keys.dtype is not values.dtype:
         raise ValueError("keys and values must be (n, n_kv_heads, head_dim) of one shape and dtype")
     n, h, d = keys.shape
     page = _check_pool(pages, d)
-    if pages.shape[1] != h:
-        raise ValueError(f"the pages hold {pages.shape[1]} kv heads, got {h}")
-    if keys.device != pages.device or values.device != pages.device:
+    index = pages.get_device()
+    if pages.size(1) != h:
+        raise ValueError(f"the pages hold {pages.size(1)} kv heads, got {h}")
+    if keys.get_device() != index or values.get_device() != index:
         raise ValueError("keys, values and pages must be on one device")
-    if n and (keys.stride(2) != 1 or values.stride(2) != 1):
+    ks, vs = keys.stride(), values.stride()
+    if n and (ks[2] != 1 or vs[2] != 1):
         raise ValueError("keys and values must be contiguous in head_dim")
-    _check_slots(slots, n, pages.device)
-    dt = L.dtype_code(keys.dtype)
-    with L.on_device(pages.device):
-        L.call("ss_int4_append", keys.data_ptr(), values.data_ptr(), dt, keys.stride(0), keys.stride(1),
-               values.stride(0), values.stride(1), slots.data_ptr(), n, h, d, pages.data_ptr(),
-               pages.shape[0], pages.stride(0), pages.stride(1), page, L.stream_ptr(pages.device))
+    _check_slots(slots, n, index)
+    L.launch("ss_int4_append", index, keys.data_ptr(), values.data_ptr(), L.dtype_code(keys.dtype), ks[0], ks[1],
+             vs[0], vs[1], slots.data_ptr(), n, h, d, pages.data_ptr(), pages.size(0), pages.stride(0),
+             pages.stride(1), page)
 
 
 def int4_fetch(slots: torch.Tensor, pages: torch.Tensor, head_dim: int, *,
@@ -181,14 +188,13 @@ def int4_fetch(slots: torch.Tensor, pages: torch.Tensor, head_dim: int, *,
     """Keys and values (n, n_kv_heads, head_dim) as the pages hold them at
     ``slots``; zeros where a slot is -1."""
     page = _check_pool(pages, head_dim)
-    n, h = slots.shape[0], pages.shape[1]
-    _check_slots(slots, n, pages.device)
+    index, n, h = pages.get_device(), slots.numel(), pages.size(1)
+    _check_slots(slots, n, index)
     dt = L.dtype_code(dtype)
-    k, v = (torch.empty((n, h, head_dim), dtype=dtype, device=pages.device) for _ in range(2))
-    with L.on_device(pages.device):
-        L.call("ss_int4_fetch", slots.data_ptr(), n, h, head_dim, pages.data_ptr(), pages.shape[0],
-               pages.stride(0), pages.stride(1), page, k.data_ptr(), v.data_ptr(), dt,
-               L.stream_ptr(pages.device))
+    k = torch.empty((n, h, head_dim), dtype=dtype, device=pages.device)
+    v = torch.empty_like(k)
+    L.launch("ss_int4_fetch", index, slots.data_ptr(), n, h, head_dim, pages.data_ptr(), pages.size(0),
+             pages.stride(0), pages.stride(1), page, k.data_ptr(), v.data_ptr(), dt)
     return k, v
 
 
@@ -210,42 +216,55 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     row that sees no key gives 0 and -inf, as does a token outside ``cu_q``.
     """
     L.poll_device_errors()
-    L.require_cuda(queries, pages)
+    if not queries.is_cuda:
+        L.require_cuda(queries)
     if queries.dim() != 3:
         raise ValueError("queries must be (n_tokens, n_q_heads, head_dim)")
     n, hq, d = queries.shape
     page = _check_pool(pages, d)
-    dev = pages.device
-    hkv = pages.shape[1]
-    if queries.dtype not in (torch.float16, torch.bfloat16):
+    index, hkv = pages.get_device(), pages.size(1)
+    if queries.dtype is not torch.float16 and queries.dtype is not torch.bfloat16:
         raise TypeError(f"queries must be fp16 or bf16, got {queries.dtype}")
-    if queries.device != dev:
+    if queries.get_device() != index:
         raise ValueError("queries and pages must be on one device")
     if hq < 1 or hq % hkv:
         raise ValueError("n_q_heads must be a multiple of n_kv_heads")
     if n and queries.stride(2) != 1:
         raise ValueError("queries must be contiguous in head_dim")
-    _int32("block_table", block_table, 2, dev)
-    _int32("seq_lens", seq_lens, 1, dev)
-    _int32("cu_q", cu_q, 1, dev)
-    b = seq_lens.shape[0]
-    if not b or block_table.shape[0] != b or cu_q.shape[0] != b + 1 or not block_table.shape[1]:
+    _int32("block_table", block_table, 2, index)
+    _int32("seq_lens", seq_lens, 1, index)
+    _int32("cu_q", cu_q, 1, index)
+    b = seq_lens.size(0)
+    if not b or block_table.size(0) != b or cu_q.size(0) != b + 1 or not block_table.size(1):
         raise ValueError("block_table and seq_lens need a row per request, cu_q one element more")
     if max_q < 1 or window < 0:
         raise ValueError("max_q must be positive and window not negative")
-    out = torch.empty((n, hq, d), dtype=queries.dtype, device=dev)
-    lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if return_lse else None
+    out = torch.empty((n, hq, d), dtype=queries.dtype, device=pages.device)
+    lse = torch.empty((n, hq), dtype=torch.float32, device=pages.device) if return_lse else None
     if n:
-        ws = workspace_for(dev, L.load().ss_int4_attention_workspace(d), "int4")
+        ws = _workspace(pages.device, index, d)
         a = L.Int4AttnArgs(queries.data_ptr(), L.dtype_code(queries.dtype), queries.stride(0),
-                           queries.stride(1), n, hq, hkv, d, pages.data_ptr(), pages.shape[0],
+                           queries.stride(1), n, hq, hkv, d, pages.data_ptr(), pages.size(0),
                            pages.stride(0), pages.stride(1), page, block_table.data_ptr(),
-                           block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+                           block_table.stride(0), block_table.size(1), seq_lens.data_ptr(),
                            cu_q.data_ptr(), b, max_q, scale, 1 if causal else 0, window,
                            out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel())
-        with L.on_device(dev):
-            L.call("ss_int4_attention", C.byref(a), L.stream_ptr(dev))
+        L.launch("ss_int4_attention", index, C.byref(a))
     return (out, lse) if return_lse else out
+
+
+# The kernels' scratch belongs to a stream: (device, stream, head_dim) -> workspace.
+_WS: dict[tuple, torch.Tensor] = {}
+
+
+def _workspace(device: torch.device, index: int, head_dim: int) -> torch.Tensor:
+    key = (index, L.raw_stream(index), head_dim)
+    ws = _WS.get(key)
+    if ws is None:
+        with torch.cuda.device(index):
+            ws = workspace_for(device, L.entry("ss_int4_attention_workspace")(head_dim), f"int4-{head_dim}")
+        _WS[key] = ws
+    return ws
 
 
 # ------------------------------------------------------------------ a server's state
