@@ -20,11 +20,36 @@ struct RowsParams {
   const int64_t* slots;
   int64_t n;
   int h;
+  uint32_t h_inv;      // 2^32 / h, rounded up
   uint8_t* pages;
   int64_t page_stride, head_stride;  // bytes
-  int page;
+  int page_blocks;     // 16-token blocks of a page
+  uint32_t page_inv;   // 2^32 / page_blocks, rounded up
   int64_t n_slots;
 };
+
+// x / d for d >= 2 with inv = ceil(2^32 / d); the quotient of the product is x / d or one more.
+__device__ __forceinline__ uint32_t quick_div(uint32_t x, uint32_t d, uint32_t inv, uint32_t& rem) {
+  if (d == 1) {
+    rem = 0;
+    return x;
+  }
+  uint32_t q = __umulhi(x, inv);
+  int r = (int)(x - q * d);
+  if (r < 0) { --q; r += (int)d; }
+  rem = (uint32_t)r;
+  return q;
+}
+
+// Block of a slot in the pool and the token's place in it; null if the slot is outside the pool.
+template <int D>
+__device__ __forceinline__ uint8_t* block_of(const RowsParams& p, int64_t slot, uint32_t head, int& tok) {
+  if (slot < 0 || slot >= p.n_slots) return nullptr;
+  tok = (int)slot & 15;
+  uint32_t in_page;
+  const uint32_t page = quick_div((uint32_t)(slot >> 4), p.page_blocks, p.page_inv, in_page);
+  return p.pages + page * p.page_stride + head * p.head_stride + (int64_t)in_page * Int4Blk<D>::kBytes;
+}
 
 // 8 consecutive elements as fp32.
 template <int DT, bool VEC>
@@ -103,41 +128,50 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], uint32_t& sz) {
   const float s = h2f(sh), z = h2f(zh);
   uint32_t w = 0;
   if (s > 0.f) {  // false for NaN
+    // (x - z) / s by a reciprocal: off by at most 2 ulp of 16, 4e-6, so the nearest integer is the
+    // division's unless the quotient comes that near to a half; then it is divided.
+    const float r = __frcp_rn(s);
+    bool close = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
-      w |= (uint32_t)c << (4 * i);
+      const float q = fminf(fmaxf(__fsub_rn(x[i], z) * r, 0.f), 15.f);
+      const float t = q + 12582912.f;  // 1.5 * 2^23: the integer is in the low bits, ties to even
+      close |= fabsf(q - (t - 12582912.f)) > 0.49999f;
+      w |= (__float_as_uint(t) & 15u) << (4 * i);
+    }
+    if (close) {
+      w = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
+        w |= (uint32_t)c << (4 * i);
+      }
     }
   }
   return w;
 }
 
 template <int D, int DT, bool VEC>
-__global__ void __launch_bounds__(256) append_kernel(RowsParams p) {
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ RowsParams p) {
   using B = Int4Blk<D>;
   constexpr int X = D / 8;  // words of a row
-  const int64_t total = p.n * p.h * X;
-  for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = i0 + threadIdx.x;  // whole groups of 4 lanes are in or out: X is a multiple of 8
-    const bool in = i < total;
-    const int x = (int)(i % X);
-    const int64_t row = i / X;
-    const int64_t t = row / p.h;
-    const int hd = (int)(row - t * p.h);
-    const int64_t slot = in ? p.slots[t] : -1;
-    const bool live = slot >= 0 && slot < p.n_slots;
+  const int x = threadIdx.x % X;
+  const uint32_t rows = (uint32_t)p.n * p.h, per = 256 / X, step = gridDim.x * per;
+  // whole rows are in or out for a group of 4 lanes: X is a multiple of 8
+  for (uint32_t row0 = blockIdx.x * per; row0 < rows; row0 += step) {
+    const uint32_t row = row0 + threadIdx.x / X;
+    uint32_t hd;
+    const uint32_t t = quick_div(row, p.h, p.h_inv, hd);
+    int tok;
+    uint8_t* blk = row < rows ? block_of<D>(p, p.slots[t], hd, tok) : nullptr;
     float a[8] = {}, b[8] = {};
-    if (live) {
+    if (blk) {
       load8<DT, VEC>(p.k, t * p.k_st + hd * p.k_sh + x * 8, a);
       load8<DT, VEC>(p.v, t * p.v_st + hd * p.v_sh + x * 8, b);
     }
     uint32_t ksz, vsz;
     const uint32_t kw = quantise8(a, ksz), vw = quantise8(b, vsz);
-    if (!live) continue;
-    const int64_t page = slot / p.page;
-    const int in_page = (int)(slot - page * p.page);
-    uint8_t* blk = p.pages + page * p.page_stride + hd * p.head_stride + (int64_t)(in_page >> 4) * B::kBytes;
-    const int tok = in_page & 15;
+    if (!blk) continue;
     *reinterpret_cast<uint32_t*>(blk + B::key_word(tok, x >> 2, x & 3)) = kw;
     *reinterpret_cast<uint32_t*>(blk + B::value_word(tok, x)) = vw;
     if ((x & 3) == 0) {
@@ -154,35 +188,43 @@ __device__ __forceinline__ void dequant8(uint32_t w, uint32_t sz, float (&x)[8])
 }
 
 template <int D, int DT>
-__global__ void __launch_bounds__(256) fetch_kernel(RowsParams p) {
+__global__ void __launch_bounds__(256) fetch_kernel(const __grid_constant__ RowsParams p) {
   using B = Int4Blk<D>;
   constexpr int X = D / 8;
-  const int64_t total = p.n * p.h * X;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int x = (int)(i % X);
-    const int64_t row = i / X;
-    const int64_t t = row / p.h;
-    const int hd = (int)(row - t * p.h);
-    const int64_t slot = p.slots[t];
+  const int x = threadIdx.x % X;
+  const uint32_t rows = (uint32_t)p.n * p.h, per = 256 / X, step = gridDim.x * per;
+  for (uint32_t row = blockIdx.x * per + threadIdx.x / X; row < rows; row += step) {
+    uint32_t hd;
+    const uint32_t t = quick_div(row, p.h, p.h_inv, hd);
+    int tok;
+    const uint8_t* blk = block_of<D>(p, p.slots[t], hd, tok);
     float a[8] = {}, b[8] = {};
-    if (slot >= 0 && slot < p.n_slots) {
-      const int64_t page = slot / p.page;
-      const int in_page = (int)(slot - page * p.page);
-      const uint8_t* blk = p.pages + page * p.page_stride + hd * p.head_stride + (int64_t)(in_page >> 4) * B::kBytes;
-      const int tok = in_page & 15;
+    if (blk) {
       dequant8(*reinterpret_cast<const uint32_t*>(blk + B::key_word(tok, x >> 2, x & 3)),
                *reinterpret_cast<const uint32_t*>(blk + B::key_sz(tok, x >> 2)), a);
       dequant8(*reinterpret_cast<const uint32_t*>(blk + B::value_word(tok, x)),
                *reinterpret_cast<const uint32_t*>(blk + B::value_sz(tok, x >> 2)), b);
     }
-    store8<DT>(p.ko, i * 8, a);
-    store8<DT>(p.vo, i * 8, b);
+    const int64_t at = ((int64_t)row * X + x) * 8;
+    store8<DT>(p.ko, at, a);
+    store8<DT>(p.vo, at, b);
   }
 }
 
-int rows_grid(int64_t total) {
-  const int64_t want = (total + 255) / 256, cap = 8LL * sm_count();
+int rows_grid(int64_t threads) {
+  const int64_t want = (threads + 255) / 256, cap = 16LL * sm_count();
   return (int)(want < cap ? want : cap);
+}
+
+// Sizes that the two entry points share.
+void set_sizes(RowsParams& p, int64_t n, int h, int64_t n_pages, int page_size) {
+  auto inv = [](int d) { return d < 2 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); };
+  p.n = n;
+  p.h = h;
+  p.h_inv = inv(h);
+  p.page_blocks = page_size / kBlkTokens;
+  p.page_inv = inv(p.page_blocks);
+  p.n_slots = n_pages * page_size;
 }
 
 template <int D>
@@ -207,12 +249,14 @@ int launch_fetch(const RowsParams& p, cudaStream_t st) {
   return check_launch("ss_int4_fetch");
 }
 
-int check_pool(const void* pages, int64_t n_pages, int64_t page_stride, int64_t head_stride, int h,
+int check_pool(const void* pages, int64_t n_pages, int64_t page_stride, int64_t head_stride, int64_t n, int h,
                int page_size, int d) {
   SS_REQUIRE(pages, "int4 pages: null pointer");
   SS_REQUIRE(int4_head_dim_ok(d), "int4 pages: head_dim must be 64, 128 or 256");
   SS_REQUIRE(page_size >= 16 && page_size % 16 == 0, "int4 pages: page_size must be a multiple of 16");
   SS_REQUIRE(n_pages >= 1 && h >= 1, "int4 pages: empty pool");
+  SS_REQUIRE(n <= 0x7fffffff / h && n_pages <= (int64_t)0x7fffffff / (page_size / kBlkTokens),
+             "int4 pages: 2^31 rows or blocks or more");
   SS_REQUIRE(((reinterpret_cast<uintptr_t>(pages) | (uintptr_t)page_stride | (uintptr_t)head_stride) & 15) == 0,
              "int4 pages: the pool and its strides must be multiples of 16 bytes");
   return SS_OK;
@@ -234,15 +278,15 @@ int ss_int4_append(const void* k, const void* v, int dtype, int64_t k_token_stri
     if (n == 0) return SS_OK;
     SS_REQUIRE(k && v && slots && n > 0, "ss_int4_append: null pointer or negative count");
     SS_REQUIRE(dtype >= SS_F32 && dtype <= SS_BF16, "ss_int4_append: bad dtype");
-    if (int rc = check_pool(pages, n_pages, page_stride, head_stride, n_heads, page_size, d)) return rc;
+    if (int rc = check_pool(pages, n_pages, page_stride, head_stride, n, n_heads, page_size, d)) return rc;
     count_dispatch("ss_int4_append");
     RowsParams p{};
     p.k = k; p.v = v; p.dtype = dtype;
     p.k_st = k_token_stride; p.k_sh = k_head_stride; p.v_st = v_token_stride; p.v_sh = v_head_stride;
-    p.slots = slots; p.n = n; p.h = n_heads;
+    p.slots = slots;
     p.pages = static_cast<uint8_t*>(pages);
-    p.page_stride = page_stride; p.head_stride = head_stride; p.page = page_size;
-    p.n_slots = n_pages * page_size;
+    p.page_stride = page_stride; p.head_stride = head_stride;
+    set_sizes(p, n, n_heads, n_pages, page_size);
     const int es = dtype == SS_F32 ? 4 : 2;
     const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                        (uintptr_t)((k_token_stride | k_head_stride | v_token_stride | v_head_stride) * es)) & 15) == 0;
@@ -261,14 +305,14 @@ int ss_int4_fetch(const int64_t* slots, int64_t n, int n_heads, int d, const voi
     SS_REQUIRE(dtype >= SS_F32 && dtype <= SS_BF16, "ss_int4_fetch: bad dtype");
     SS_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0,
                "ss_int4_fetch: outputs must be 16-byte aligned");
-    if (int rc = check_pool(pages, n_pages, page_stride, head_stride, n_heads, page_size, d)) return rc;
+    if (int rc = check_pool(pages, n_pages, page_stride, head_stride, n, n_heads, page_size, d)) return rc;
     count_dispatch("ss_int4_fetch");
     RowsParams p{};
     p.ko = k_out; p.vo = v_out; p.dtype = dtype;
-    p.slots = slots; p.n = n; p.h = n_heads;
+    p.slots = slots;
     p.pages = static_cast<uint8_t*>(const_cast<void*>(pages));
-    p.page_stride = page_stride; p.head_stride = head_stride; p.page = page_size;
-    p.n_slots = n_pages * page_size;
+    p.page_stride = page_stride; p.head_stride = head_stride;
+    set_sizes(p, n, n_heads, n_pages, page_size);
     cudaStream_t st = as_stream(stream);
     return d == 64 ? launch_fetch<64>(p, st) : d == 128 ? launch_fetch<128>(p, st) : launch_fetch<256>(p, st);
   });
