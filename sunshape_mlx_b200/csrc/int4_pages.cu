@@ -103,50 +103,78 @@ __device__ __forceinline__ void store8(void* base, int64_t at, const float (&x)[
   }
 }
 
+// min / max of three that keep NaN.
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// (a, b) = (a, b) * s + (c, d), packed fp32
+__device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float c, float d) {
+  asm("{\n .reg .b64 t, u, v;\n mov.b64 t, {%0, %1};\n mov.b64 u, {%2, %2};\n mov.b64 v, {%3, %4};\n"
+      " fma.rn.f32x2 t, t, u, v;\n mov.b64 {%0, %1}, t;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(s), "f"(c), "f"(d));
+}
+__device__ __forceinline__ float mul_sat(float a, float b) {
+  float r;
+  asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The 4 lanes of a group hold 8 values each: this lane's code word and the group's (s, z).
-__device__ __forceinline__ uint32_t quantise8(float (&x)[8], uint32_t& sz) {
-  float lo = x[0], hi = x[0];
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    nan |= x[i] != x[i];
-    x[i] = fminf(fmaxf(x[i], -kInt4Max), kInt4Max);
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-  lo = fminf(fmaxf(lo, -kInt4Max), kInt4Max);
-  hi = fminf(fmaxf(hi, -kInt4Max), kInt4Max);
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& sz) {
+  float lo = min3_nan(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
+  lo = min3_nan(min3_nan(lo, x[3], x[4]), min3_nan(x[5], x[6], x[7]), x[7]);
+  hi = max3_nan(max3_nan(hi, x[3], x[4]), max3_nan(x[5], x[6], x[7]), x[7]);
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+    const float l2 = __shfl_xor_sync(0xffffffffu, lo, o), h2 = __shfl_xor_sync(0xffffffffu, hi, o);
+    lo = min3_nan(lo, l2, l2);
+    hi = max3_nan(hi, h2, h2);
   }
+  const bool nan = lo != lo;
+  // the ends saturate; values beyond them go to the end codes by themselves
+  lo = fminf(fmaxf(lo, -kInt4Max), kInt4Max);
+  hi = fminf(fmaxf(hi, -kInt4Max), kInt4Max);
   const uint16_t sh = nan ? 0x7fff : f2h(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
   const uint16_t zh = nan ? 0x7fff : f2h(lo);
   sz = sh | (uint32_t)zh << 16;
   const float s = h2f(sh), z = h2f(zh);
   uint32_t w = 0;
   if (s > 0.f) {  // false for NaN
-    // (x - z) / s by a reciprocal: off by at most 2 ulp of 16, 4e-6, so the nearest integer is the
-    // division's unless the quotient comes that near to a half; then it is divided.
-    const float r = __frcp_rn(s);
-    bool close = false;
+    // (x - z) / s by a reciprocal, clamped as a share of 15: off by less than 1e-5, so the nearest
+    // integer is the division's unless the quotient comes that near to a half; then it is divided.
+    const float r = __frcp_rn(s) * (1.f / 15.f);
+    const float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to integers, ties to even
+    float c[8], off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = fminf(fmaxf(__fsub_rn(x[i], z) * r, 0.f), 15.f);
-      const float t = q + 12582912.f;  // 1.5 * 2^23: the integer is in the low bits, ties to even
-      close |= fabsf(q - (t - 12582912.f)) > 0.49999f;
-      w |= (__float_as_uint(t) & 15u) << (4 * i);
+    for (int i = 0; i < 8; i += 2) {
+      float a = x[i], b = x[i + 1];
+      add_f32x2(a, b, -z, -z);
+      a = mul_sat(a, r);
+      b = mul_sat(b, r);
+      float t = a, u = b;
+      fma_f32x2(t, u, 15.f, kMagic, kMagic);
+      add_f32x2(t, u, -kMagic, -kMagic);
+      c[i] = t;
+      c[i + 1] = u;
+      fma_f32x2(a, b, 15.f, -t, -u);
+      off = fmaxf(off, fmaxf(fabsf(a), fabsf(b)));
     }
-    if (close) {
-      w = 0;
+    if (off > 0.49998f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
-        w |= (uint32_t)c << (4 * i);
-      }
+      for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
     }
+    // four codes make an integer below 2^16, exact in fp32 and in the low bits of 2^23 + it
+    const float w0 = fmaf(fmaf(c[3], 16.f, c[2]), 256.f, fmaf(c[1], 16.f, c[0])) + 8388608.f;
+    const float w1 = fmaf(fmaf(c[7], 16.f, c[6]), 256.f, fmaf(c[5], 16.f, c[4])) + 8388608.f;
+    w = __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
   }
   return w;
 }
