@@ -6,7 +6,14 @@
 //   c = clamp(rint((x' - z) / s), 0, 15), 0 where s = 0;   value = c * s + z
 // (fp32 arithmetic, IEEE division, ties to even). A NaN makes its group's s
 // and z NaN, so readers see NaN for the group and nothing else.
-// Bound by HBM: a row is read once and 5 bits per value are written.
+//
+// A row is read once and 5 bits per value are written: HBM is the floor, but
+// quantising costs about 10 instructions a value, so a write of 16-bit rows is
+// bound by issue (70 % of the slots): two lanes a group, 16 keys and 16 values
+// a thread, so that what a row costs once (slot, page, addresses) is shared by
+// 32 values. 49999 tokens x 8 heads x 128: write 72 us from fp16 (3.7 TB/s), 80
+// us from fp32 (5.9 TB/s); with 8 + 8 values a thread it was 96 us. Read back
+// 55 us to fp16 (4.9 TB/s).
 #include "int4_pages.cuh"
 
 namespace ss {
@@ -51,36 +58,46 @@ __device__ __forceinline__ uint8_t* block_of(const RowsParams& p, int64_t slot, 
   return p.pages + page * p.page_stride + head * p.head_stride + (int64_t)in_page * Int4Blk<D>::kBytes;
 }
 
-// 8 consecutive elements as fp32.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8]) {
-  if constexpr (DT == SS_F32) {
-    const float* p = reinterpret_cast<const float*>(base) + at;
+// 16 consecutive elements as they are stored.
+template <int DT>
+struct Raw {
+  static constexpr int N = DT == SS_F32 ? 16 : 8;
+  uint32_t u[N];
+
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
     if constexpr (VEC) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(base) + at * (DT == SS_F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        const uint4 a = __ldcs(p + i);
+        u[4 * i] = a.x; u[4 * i + 1] = a.y; u[4 * i + 2] = a.z; u[4 * i + 3] = a.w;
+      }
+    } else if constexpr (DT == SS_F32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = reinterpret_cast<const uint32_t*>(base)[at + i];
     } else {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = p[i];
-    }
-  } else {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
-    uint32_t u[4];
-    if constexpr (VEC) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-      u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = DT == SS_F16 ? h2f(u[i] & 0xffff) : bf2f(u[i] & 0xffff);
-      x[2 * i + 1] = DT == SS_F16 ? h2f(u[i] >> 16) : bf2f(u[i] >> 16);
+      for (int i = 0; i < N; ++i) u[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
     }
   }
-}
+  __device__ __forceinline__ void get(float (&x)[16]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (DT == SS_F32) {
+        x[i] = __uint_as_float(u[i]);
+      } else if constexpr (DT == SS_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      } else {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    }
+  }
+};
 
 template <int DT>
 __device__ __forceinline__ void store8(void* base, int64_t at, const float (&x)[8]) {
@@ -114,30 +131,27 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// (a, b) = (a, b) * s + (c, d), packed fp32
-__device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float c, float d) {
-  asm("{\n .reg .b64 t, u, v;\n mov.b64 t, {%0, %1};\n mov.b64 u, {%2, %2};\n mov.b64 v, {%3, %4};\n"
-      " fma.rn.f32x2 t, t, u, v;\n mov.b64 {%0, %1}, t;\n}"
-      : "+f"(a), "+f"(b)
-      : "f"(s), "f"(c), "f"(d));
-}
 __device__ __forceinline__ float mul_sat(float a, float b) {
   float r;
   asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// The 4 lanes of a group hold 8 values each: this lane's code word and the group's (s, z).
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& sz) {
-  float lo = min3_nan(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
-  lo = min3_nan(min3_nan(lo, x[3], x[4]), min3_nan(x[5], x[6], x[7]), x[7]);
-  hi = max3_nan(max3_nan(hi, x[3], x[4]), max3_nan(x[5], x[6], x[7]), x[7]);
+// The two lanes of a group hold 16 values each: this lane's two code words and the group's (s, z).
+__device__ __forceinline__ void quantise16(const float (&x)[16], uint32_t (&w)[2], uint32_t& sz) {
+  float lo = x[0], hi = x[0], lo2 = x[1], hi2 = x[1];
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    const float l2 = __shfl_xor_sync(0xffffffffu, lo, o), h2 = __shfl_xor_sync(0xffffffffu, hi, o);
-    lo = min3_nan(lo, l2, l2);
-    hi = max3_nan(hi, h2, h2);
+  for (int i = 2; i < 14; i += 4) {
+    lo = min3_nan(lo, x[i], x[i + 1]);
+    hi = max3_nan(hi, x[i], x[i + 1]);
+    lo2 = min3_nan(lo2, x[i + 2], x[i + 3]);
+    hi2 = max3_nan(hi2, x[i + 2], x[i + 3]);
   }
+  lo = min3_nan(min3_nan(lo, x[14], x[15]), lo2, lo2);
+  hi = max3_nan(max3_nan(hi, x[14], x[15]), hi2, hi2);
+  const float lo3 = __shfl_xor_sync(0xffffffffu, lo, 1), hi3 = __shfl_xor_sync(0xffffffffu, hi, 1);
+  lo = min3_nan(lo, lo3, lo3);
+  hi = max3_nan(hi, hi3, hi3);
   const bool nan = lo != lo;
   // the ends saturate; values beyond them go to the end codes by themselves
   lo = fminf(fmaxf(lo, -kInt4Max), kInt4Max);
@@ -146,65 +160,73 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& sz)
   const uint16_t zh = nan ? 0x7fff : f2h(lo);
   sz = sh | (uint32_t)zh << 16;
   const float s = h2f(sh), z = h2f(zh);
-  uint32_t w = 0;
+  w[0] = w[1] = 0u;
   if (s > 0.f) {  // false for NaN
     // (x - z) / s by a reciprocal, clamped as a share of 15: off by less than 1e-5, so the nearest
     // integer is the division's unless the quotient comes that near to a half; then it is divided.
     const float r = __frcp_rn(s) * (1.f / 15.f);
     const float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to integers, ties to even
-    float c[8], off = 0.f;
+    float c[16], off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      float a = x[i], b = x[i + 1];
-      add_f32x2(a, b, -z, -z);
-      a = mul_sat(a, r);
-      b = mul_sat(b, r);
-      float t = a, u = b;
-      fma_f32x2(t, u, 15.f, kMagic, kMagic);
-      add_f32x2(t, u, -kMagic, -kMagic);
-      c[i] = t;
-      c[i + 1] = u;
-      fma_f32x2(a, b, 15.f, -t, -u);
-      off = fmaxf(off, fmaxf(fabsf(a), fabsf(b)));
+    for (int i = 0; i < 16; ++i) {
+      const float q = mul_sat(x[i] - z, r);
+      c[i] = fmaf(q, 15.f, kMagic) - kMagic;
+      off = fmaxf(off, fabsf(fmaf(q, 15.f, -c[i])));
     }
     if (off > 0.49998f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
+      for (int i = 0; i < 16; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
     }
-    // four codes make an integer below 2^16, exact in fp32 and in the low bits of 2^23 + it
-    const float w0 = fmaf(fmaf(c[3], 16.f, c[2]), 256.f, fmaf(c[1], 16.f, c[0])) + 8388608.f;
-    const float w1 = fmaf(fmaf(c[7], 16.f, c[6]), 256.f, fmaf(c[5], 16.f, c[4])) + 8388608.f;
-    w = __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {  // four codes make an integer below 2^16, exact in the low bits of 2^23 + it
+      const float* e = c + 8 * v;
+      const float w0 = fmaf(fmaf(e[3], 16.f, e[2]), 256.f, fmaf(e[1], 16.f, e[0])) + 8388608.f;
+      const float w1 = fmaf(fmaf(e[7], 16.f, e[6]), 256.f, fmaf(e[5], 16.f, e[4])) + 8388608.f;
+      w[v] = __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
+    }
   }
-  return w;
 }
 
 template <int D, int DT, bool VEC>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(256, 4) append_kernel(const __grid_constant__ RowsParams p) {
   using B = Int4Blk<D>;
-  constexpr int X = D / 8;  // words of a row
-  const int x = threadIdx.x % X;
+  constexpr int X = D / 16;  // threads of a row: 16 dims of its key and of its value each
+  const int y = threadIdx.x % X;
   const uint32_t rows = (uint32_t)p.n * p.h, per = 256 / X, step = gridDim.x * per;
-  // whole rows are in or out for a group of 4 lanes: X is a multiple of 8
+  // whole rows are in or out for the two lanes of a group
   for (uint32_t row0 = blockIdx.x * per; row0 < rows; row0 += step) {
     const uint32_t row = row0 + threadIdx.x / X;
     uint32_t hd;
     const uint32_t t = quick_div(row, p.h, p.h_inv, hd);
     int tok;
-    uint8_t* blk = row < rows ? block_of<D>(p, p.slots[t], hd, tok) : nullptr;
-    float a[8] = {}, b[8] = {};
+    uint8_t* blk = row < rows ? block_of<D>(p, __ldg(p.slots + t), hd, tok) : nullptr;
+    Raw<DT> k{}, v{};
     if (blk) {
-      load8<DT, VEC>(p.k, t * p.k_st + hd * p.k_sh + x * 8, a);
-      load8<DT, VEC>(p.v, t * p.v_st + hd * p.v_sh + x * 8, b);
+      k.template load<VEC>(p.k, t * p.k_st + hd * p.k_sh + y * 16);
+      v.template load<VEC>(p.v, t * p.v_st + hd * p.v_sh + y * 16);
     }
-    uint32_t ksz, vsz;
-    const uint32_t kw = quantise8(a, ksz), vw = quantise8(b, vsz);
-    if (!blk) continue;
-    *reinterpret_cast<uint32_t*>(blk + B::key_word(tok, x >> 2, x & 3)) = kw;
-    *reinterpret_cast<uint32_t*>(blk + B::value_word(tok, x)) = vw;
-    if ((x & 3) == 0) {
-      *reinterpret_cast<uint32_t*>(blk + B::key_sz(tok, x >> 2)) = ksz;
-      *reinterpret_cast<uint32_t*>(blk + B::value_sz(tok, x >> 2)) = vsz;
+    uint32_t w[2], ksz, vsz;
+    float x[16];
+    k.get(x);
+    quantise16(x, w, ksz);
+    if (blk) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<uint32_t*>(blk + B::key_word(tok, y >> 1, 2 * (y & 1) + e)) = w[e];
+    }
+    v.get(x);
+    quantise16(x, w, vsz);
+    if (blk) {
+      if constexpr (B::W > 1) {  // two words of one piece
+        *reinterpret_cast<uint2*>(blk + B::value_word(tok, 2 * y)) = make_uint2(w[0], w[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(blk + B::value_word(tok, 2 * y)) = w[0];
+        *reinterpret_cast<uint32_t*>(blk + B::value_word(tok, 2 * y + 1)) = w[1];
+      }
+      if ((y & 1) == 0) {
+        *reinterpret_cast<uint32_t*>(blk + B::key_sz(tok, y >> 1)) = ksz;
+        *reinterpret_cast<uint32_t*>(blk + B::value_sz(tok, y >> 1)) = vsz;
+      }
     }
   }
 }
@@ -257,7 +279,7 @@ void set_sizes(RowsParams& p, int64_t n, int h, int64_t n_pages, int page_size) 
 
 template <int D>
 int launch_append(const RowsParams& p, bool vec, cudaStream_t st) {
-  const int g = rows_grid(p.n * p.h * (D / 8));
+  const int g = rows_grid(p.n * p.h * (D / 16));
 #define SS_APPEND(DT)                                                     \
   if (vec) append_kernel<D, DT, true><<<g, 256, 0, st>>>(p);              \
   else append_kernel<D, DT, false><<<g, 256, 0, st>>>(p)
