@@ -32,7 +32,7 @@ struct AttnParams {
   int* sink;    // process error sink (host word) or null
 };
 
-constexpr float kLow = -1e30f;   // softmax reference before any key
+constexpr float kLow = -3e38f;   // softmax reference before any key
 constexpr float kSlack = 8.f;    // a logit may exceed the reference by this (base 2)
 constexpr float kLog2e = 1.4426950408889634f;
 

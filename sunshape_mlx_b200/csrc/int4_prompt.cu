@@ -436,6 +436,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             tc_fence_before();
           }
         }
+        // The exponent is one FMA; from 2^22 on its unrounded product strays from the reference by
+        // whole units, so products are rounded before the difference there.
+        float fac_x = fac, m_x = m;
+        if (__any_sync(0xffffffffu, fabsf(m) > 0x1p22f && m != kLow)) {
+#pragma unroll
+          for (int e = 0; e < kHalfKeys; ++e) y[e] = __fadd_rn(__fmul_rn(y[e], fac), -m);
+          fac_x = 1.f;
+          m_x = 0.f;
+        }
         // P over the S it comes from
 #pragma unroll
         for (int c = 0; c < kHalfKeys; c += 32) {
@@ -444,8 +453,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
           for (int e = 0; e < 16; ++e) {
             float& a = y[c + 2 * e];
             float& b = y[c + 2 * e + 1];
-            float x = -m, z = -m;
-            fma_f32x2(x, z, a, b, fac);
+            float x = -m_x, z = -m_x;
+            fma_f32x2(x, z, a, b, fac_x);
             a = ex2(x);
             b = ex2(z);
             add_f32x2(e & 1 ? l2 : l0, e & 1 ? l3 : l1, a, b);

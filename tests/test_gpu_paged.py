@@ -394,6 +394,65 @@ def test_attention_scales_of_tiny_and_large_values(ss):
             assert ((o.double() - want).abs() <= 2.0 ** -11 * want.abs() + (4 * 2.0 ** -11 + 2 * dz) * pv + 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+def test_attention_any_scale(ss, scale):
+    for old, new, d in (([200, 30], [1, 1], 128), ([0, 60], [400, 300], 64)):
+        pool, table, lens, cu, q, kv = _setup(ss, old, new, 2, d, 16, 11, torch.bfloat16, 4)
+        o, lse = ss.int4_attention(q, pool, table, lens, cu, scale, max_q=max(new), return_lse=True)
+        _check(o, lse, q, kv, old, new, scale, True, 0)
+
+
+def test_attention_tiles_and_units_share_a_batch(ss):
+    # requests on both sides of the rule that sends rows to the tile kernel, empty ones, and wrong pages
+    old, new = [0, 3000, 17, 0, 64, 500], [700, 1, 0, 300, 2, 36]
+    for dtype, window in ((torch.float16, 0), (torch.bfloat16, 130)):
+        pool, table, lens, cu, q, kv = _setup(ss, old, new, 8, 128, 64, 12, dtype, 4, pad=7)
+        o, lse = ss.int4_attention(q, pool, table, lens, cu, 0.088, max_q=700, window=window, return_lse=True)
+        _check(o, lse, q, kv, old, new, 0.088, True, window)
+    t = table.clone()
+    t[0, 3] = -1  # keys 192 .. 255 of the first request disappear
+    o = ss.int4_attention(q, pool, t, lens, cu, 0.088, max_q=700)
+    (k, v) = kv[0]
+    for row in (100, 300, 699):
+        keep = torch.tensor([i for i in range(row + 1) if not 192 <= i < 256], device="cuda")
+        want, _, _, _ = R.attention(q[row:row + 1], k[keep], v[keep], len(keep), 0.088, causal=False)
+        assert (o[row].double() - want[0]).abs().max() < 2.0 ** -7 * (1 + want.abs().max())
+
+
+def test_attention_tiles_special_values(ss):
+    d = 128
+    pool, table, lens, cu, q, kv = _setup(ss, [0, 0], [300, 300], 2, d, 16, 13, torch.bfloat16, 4)
+    q2 = q.clone()
+    q2[5, 1] = math.nan
+    q2[7] = 0
+    q2[8] = (q2[8].float() * 1e30).to(q.dtype)   # one key takes all the weight
+    q2[9] = (q2[9].float() * 1e-37).to(q.dtype)
+    o, lse = ss.int4_attention(q2, pool, table, lens, cu, 1.0, max_q=300, return_lse=True)
+    assert o[5, 1].isnan().all() and torch.isfinite(o[5, [0] + list(range(2, 8))]).all()
+    keep = [i for i in range(600) if i != 5]
+    assert torch.isfinite(o[keep]).all()
+    (k, v), _ = kv
+    for h in range(8):
+        z = torch.einsum("d,td->t", q2[8, h].double(), k[:9, h // 4].double())
+        want = v[z.argmax(), h // 4].double()
+        assert ((o[8, h].double() - want).abs() <= (2.0 ** -8 + 4 * 2.0 ** -11) * want.abs()).all()
+    for row in (7, 9):  # the mean of the values
+        want = v[:row + 1].double().mean(0).repeat_interleave(4, 0)
+        pv = v[:row + 1].double().abs().mean(0).repeat_interleave(4, 0)
+        assert ((o[row].double() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * 2.0 ** -11 * pv).all()
+        assert (lse[row] - math.log(row + 1)).abs().max() < 1e-5
+    # the widest groups that pages hold: codes times scales reach fp16's largest
+    pool2 = ss.int4_pool(4, 1, 64, d).fill_(255)
+    x = torch.zeros((200, 1, d), device="cuda")
+    x[:, 0, ::2], x[:, 0, 1::2] = 32768.0, -32768.0
+    ss.int4_append(x, x * 1e-3, torch.arange(200, device="cuda"), pool2)
+    kr, vr = ss.int4_fetch(torch.arange(200, device="cuda"), pool2, d)
+    qq = torch.randn((200, 16, d), generator=_gen(3), device="cuda").half()
+    t = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    o, lse = ss.int4_attention(qq, pool2, t, _i32([200]), _i32([0, 200]), 1e-6, max_q=200, return_lse=True)
+    _check(o, lse, qq, [(kr, vr)], [0], [200], 1e-6, True, 0)
+
+
 def test_attention_strided_queries_other_stream_and_pool_view(ss):
     old, new = [200, 31], [2, 1]
     pool, table, lens, cu, q, kv = _setup(ss, old, new, 2, 128, 16, 9, torch.float16, 4)
