@@ -57,7 +57,7 @@ struct Shape {
   static constexpr int S = D == 64 ? 4 : D == 256 ? 3 : U == 2 ? 2 : 4;  // ring stages of a warp
   static constexpr int kRing = W * S * U * Int4Blk<D>::kBytes;
   static constexpr int kMerge = W * R * (D + 4) * 4;  // rows padded by 4 floats
-  static constexpr int kSmem = kRing + kMerge + 2 * W * R * 4 + (W * 32 + 1) * 8;
+  static constexpr int kSmem = kRing + kMerge + 2 * W * R * 4 + (W * 32 + 1) * 8 + W * 32 * (int)sizeof(Req);
 };
 
 // One CTA's walk over its range: unit after unit.
@@ -68,21 +68,22 @@ struct Walk {
   Req r{};
 
   __device__ __forceinline__ int64_t cost() const { return r.nblk + kSegCost; }
-  __device__ void skip_empty(const AttnParams& p) {
+  // reqs: the requests, in shared memory, or null where there are more than threads
+  __device__ void skip_empty(const AttnParams& p, const Req* reqs) {
     while (b < p.n) {
-      r = load_req<R>(p, b);
+      r = reqs ? reqs[b] : load_req<R>(p, b);
       if (r.rbs > 0) break;
       ++b;
     }
   }
-  __device__ void next(const AttnParams& p) {
+  __device__ void next(const AttnParams& p, const Req* reqs) {
     at += cost();
     if (++rb < r.rbs) return;
     rb = 0;
     if (++h < p.hkv) return;
     h = 0;
     ++b;
-    skip_empty(p);
+    skip_empty(p, reqs);
   }
 };
 
@@ -129,29 +130,21 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas)
   float* s_l = s_m + W * R;                                           // [W][R]
   int64_t* s_cum = reinterpret_cast<int64_t*>(s_l + W * R);           // [T]
   int* s_last = reinterpret_cast<int*>(s_cum + T);                    // this CTA joins the unit's parts
+  Req* s_req = reinterpret_cast<Req*>(s_last + 2);                    // [T] the requests, if there are no more
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gi = lane >> 2, gj = lane & 3;
   uint8_t* ring = smem + warp * S * U * B::kBytes;
 
-  // tokens outside cu_q: zero rows
-  {
-    const int64_t first = min((int64_t)max(p.cu_q[0], 0), p.n_tokens), last = min((int64_t)max(p.cu_q[p.n], 0), p.n_tokens);
-    const int64_t none = first + p.n_tokens - last, row = (int64_t)p.hq * D / 8;
-    for (int64_t i = (int64_t)blockIdx.x * T + tid; i < none * row; i += (int64_t)gridDim.x * T) {
-      int64_t t = i / row;
-      t = t < first ? t : last + t - first;
-      reinterpret_cast<uint4*>(p.out)[t * row + i % row] = make_uint4(0, 0, 0, 0);
-      if (p.lse && i % row < p.hq) p.lse[t * p.hq + i % row] = -INFINITY;
-    }
-  }
-
   // ---- schedule: costs of the requests, thread by thread, then a scan -------
   const int per = (p.n + T - 1) / T;
   const int rb0 = min(p.n, tid * per), rb1 = min(p.n, rb0 + per);
   int64_t cost = 0, units = 0;
+  const Req* reqs = per == 1 ? s_req : nullptr;
+  const int cq0 = p.cu_q[0], cqn = p.cu_q[p.n];
   for (int b = rb0; b < rb1; ++b) {
     const Req r = load_req<R>(p, b);
+    if (per == 1) s_req[b] = r;
     cost += (int64_t)r.rbs * p.hkv * (r.nblk + kSegCost);
     units += (int64_t)r.rbs * p.hkv;
   }
@@ -176,13 +169,31 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas)
   }
   s_cum[tid] = before + inc - cost;  // cost of the requests before this thread's
   __syncthreads();
+  // tokens outside cu_q: zero rows
+  {
+    const int64_t first = min((int64_t)max(cq0, 0), p.n_tokens), last = min((int64_t)max(cqn, 0), p.n_tokens);
+    const int64_t none = first + p.n_tokens - last, row = (int64_t)p.hq * D / 8;
+    for (int64_t i = (int64_t)blockIdx.x * T + tid; i < none * row; i += (int64_t)gridDim.x * T) {
+      int64_t t = i / row;
+      t = t < first ? t : last + t - first;
+      reinterpret_cast<uint4*>(p.out)[t * row + i % row] = make_uint4(0, 0, 0, 0);
+      if (p.lse && i % row < p.hq) p.lse[t * p.hq + i % row] = -INFINITY;
+    }
+  }
   // as many ranges as SMs, but none smaller than a unit or kMinCost
-  int64_t want = (total + kMinCost + kSegCost - 1) / (kMinCost + kSegCost);
+  int64_t want = total < (1 << 22) ? (int64_t)(((uint32_t)total + kMinCost + kSegCost - 1) / (uint32_t)(kMinCost + kSegCost))
+                                   : (total + kMinCost + kSegCost - 1) / (kMinCost + kSegCost);
   want = want < units ? units : want;
   const int nc = (int)(want < gridDim.x ? want : (int64_t)gridDim.x);
   if ((int)blockIdx.x >= nc) return;
-  auto range_start = [&](int64_t i) { return i * total / nc; };
-  auto cta_of = [&](int64_t c) { return (int)(((c + 1) * nc - 1) / total); };  // the range that holds c
+  // (64-bit divisions take some 100 cycles each, and these stand before the first copy)
+  const bool small = total < (1 << 22);  // products with nc + 1 <= 2 * 148 + 1 stay below 2^31
+  auto range_start = [&](int i) -> int64_t {
+    return small ? (int64_t)((uint32_t)i * (uint32_t)total / (uint32_t)nc) : i * total / nc;
+  };
+  auto cta_of = [&](int64_t c) {  // the range that holds c
+    return small ? (int)(((uint32_t)(c + 1) * (uint32_t)nc - 1) / (uint32_t)total) : (int)(((c + 1) * nc - 1) / total);
+  };
   const int64_t lo = range_start(blockIdx.x), hi = range_start(blockIdx.x + 1);
 
   Walk<R> walk;
@@ -194,19 +205,19 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas)
     }
     walk.b = min(p.n, a * per);
     walk.at = s_cum[a];
-    walk.skip_empty(p);
+    walk.skip_empty(p, reqs);
     for (;;) {
       const int64_t one = walk.cost(), all = one * walk.r.rbs * p.hkv;
       if (walk.at + all > lo) {
-        const int64_t u = (lo - walk.at) / one;
-        walk.h = (int)(u / walk.r.rbs);
+        const int64_t u = small ? (int64_t)((uint32_t)(lo - walk.at) / (uint32_t)one) : (lo - walk.at) / one;
+        walk.h = (int)((uint32_t)u / (uint32_t)walk.r.rbs);
         walk.rb = (int)(u - (int64_t)walk.h * walk.r.rbs);
         walk.at += u * one;
         break;
       }
       walk.at += all;
       ++walk.b;
-      walk.skip_empty(p);
+      walk.skip_empty(p, reqs);
     }
   }
 
@@ -238,7 +249,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas)
       pk += warp * U;
       pn = 32;
       if (pk < pk1) return;
-      pw.next(p);
+      pw.next(p, reqs);
     }
   };
   open();
@@ -273,7 +284,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas)
       }
       pk += W * U;
       if (pk >= pk1) {
-        pw.next(p);
+        pw.next(p, reqs);
         open();
       }
     } else {
@@ -286,7 +297,7 @@ __global__ void __launch_bounds__(Shape<D, MODE>::W * 32, Shape<D, MODE>::kCtas)
   int stage = 0;
 
   // ---- unit after unit --------------------------------------------------------
-  for (; walk.b < p.n && walk.at < hi; walk.next(p)) {
+  for (; walk.b < p.n && walk.at < hi; walk.next(p, reqs)) {
     int k0, k1;
     const bool part = blocks(walk, k0, k1);
     const Req r = walk.r;
