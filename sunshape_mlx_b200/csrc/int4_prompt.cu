@@ -311,30 +311,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
       if (half == 0) {  // the row's queries, scaled by a power of two into [256, 512), and its group sums
         const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + tok * p.q_st + hd * p.q_sh;
-        auto get8 = [&](int c, float (&f)[8]) {
-          uint32_t w[4] = {0u, 0u, 0u, 0u};
+        uint32_t w[D / 8][4];  // all of the row in flight
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          w[c][0] = w[c][1] = w[c][2] = w[c][3] = 0u;
           if (live) {
             if (p.q_vec) {
               const uint4 v = __ldg(reinterpret_cast<const uint4*>(qp) + c);
-              w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+              w[c][0] = v.x; w[c][1] = v.y; w[c][2] = v.z; w[c][3] = v.w;
             } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = qp[c * 8 + 2 * e] | (uint32_t)qp[c * 8 + 2 * e + 1] << 16;
+              for (int e = 0; e < 4; ++e) w[c][e] = qp[c * 8 + 2 * e] | (uint32_t)qp[c * 8 + 2 * e + 1] << 16;
             }
           }
+        }
+        const bool f16 = p.dtype == SS_F16;
+        float big = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            f[2 * e] = p.dtype == SS_F16 ? lo_h(w[e]) : __uint_as_float(w[e] << 16);
-            f[2 * e + 1] = p.dtype == SS_F16 ? hi_h(w[e]) : __uint_as_float(w[e] & 0xffff0000u);
+            const float a = f16 ? lo_h(w[c][e]) : __uint_as_float(w[c][e] << 16);
+            const float b = f16 ? hi_h(w[c][e]) : __uint_as_float(w[c][e] & 0xffff0000u);
+            big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
           }
-        };
-        float big = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          float f[8];
-          get8(c, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
         }
         int ex = 0;
         if (big > 0.f && big < INFINITY) ex = 135 - (int)(__float_as_uint(fmaxf(big, 1.2e-38f)) >> 23);
@@ -353,7 +353,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float f[8];
-            get8(g * 4 + c, f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = w[g * 4 + c][e];
+              f[2 * e] = f16 ? lo_h(x) : __uint_as_float(x << 16);
+              f[2 * e + 1] = f16 ? hi_h(x) : __uint_as_float(x & 0xffff0000u);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // dims (e, e + 4) side by side, as the key words' nibbles come
               qo[c * 4 + e] = pack_h2(f[e] * up, f[e + 4] * up);
