@@ -9,6 +9,7 @@ pointers plus the current CUDA stream.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 import os
 import threading
 
@@ -264,6 +265,20 @@ def stream_ptr(device: torch.device | None = None):
 _FNS: dict = {}
 current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+_fast = None
+
+
+def fast():
+    """The native lane (csrc/binding.cpp): functions that do an ordinary call's
+    checks, allocations and launch, and return None where the wrapper has to
+    look closer. Built beside the library."""
+    global _fast
+    if _fast is None:
+        load()
+        _fast = importlib.import_module("._fast", __package__)
+    return _fast
 
 
 def entry(fn: str):

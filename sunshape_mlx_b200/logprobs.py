@@ -35,6 +35,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     nothing else gives -inf and entropy 0. A row with NaN or +inf gives NaN
     everywhere and ids of -1.
     """
+    t = (L._fast or L.fast()).logprobs(logits, targets, top_k)
+    if t is not None:
+        return TokenLogprobs._make(t)
     if not (logits.is_cuda and targets.is_cuda):
         L.require_cuda(logits, targets)
     if logits.dim() != 2 or not logits.size(1):

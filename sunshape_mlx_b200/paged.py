@@ -90,6 +90,9 @@ def plan_step(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_table: torch.T
     step of fewer tokens leaves slots of -1 at the end). If the step does not
     fit, nothing is allocated and ``status`` says why.
     """
+    t = (L._fast or L.fast()).plan_step(seq_lens, q_lens, block_table, free_pages, n_free, page_size, n_tokens)
+    if t is not None:
+        return StepPlan._make(t)
     index = _check_tables(seq_lens, block_table, free_pages, n_free, page_size)
     _int32("q_lens", q_lens, 1, index)
     n = seq_lens.size(0)
@@ -163,6 +166,8 @@ def int4_append(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor, p
     bf16, into the pages at ``slots`` (n,) int64; -1 skips a token. Slots of
     one call must differ. Magnitudes above 2^15 saturate; a NaN makes its
     group of 32 dims read as NaN."""
+    if (L._fast or L.fast()).append(keys, values, slots, pages):
+        return
     if not (keys.is_cuda and values.is_cuda):
         L.require_cuda(keys, values)
     if keys.dim() != 3 or keys.shape != values.shape or keys.dtype is not values.dtype:
@@ -187,10 +192,13 @@ def int4_fetch(slots: torch.Tensor, pages: torch.Tensor, head_dim: int, *,
                dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values (n, n_kv_heads, head_dim) as the pages hold them at
     ``slots``; zeros where a slot is -1."""
+    dt = L.dtype_code(dtype)
+    kv = (L._fast or L.fast()).fetch(slots, pages, head_dim, dt)
+    if kv is not None:
+        return kv
     page = _check_pool(pages, head_dim)
     index, n, h = pages.get_device(), slots.numel(), pages.size(1)
     _check_slots(slots, n, index)
-    dt = L.dtype_code(dtype)
     k = torch.empty((n, h, head_dim), dtype=dtype, device=pages.device)
     v = torch.empty_like(k)
     L.launch("ss_int4_fetch", index, slots.data_ptr(), n, h, head_dim, pages.data_ptr(), pages.size(0),
@@ -216,6 +224,11 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     row that sees no key gives 0 and -inf, as does a token outside ``cu_q``.
     """
     L.poll_device_errors()
+    if queries.is_cuda and pages.is_cuda and queries.dim() == 3:
+        t = (L._fast or L.fast()).attention(queries, pages, block_table, seq_lens, cu_q, scale, max_q, causal, window, return_lse,
+                                            _workspace(pages, queries.size(2)))
+        if t is not None:
+            return t if return_lse else t[0]
     if not queries.is_cuda:
         L.require_cuda(queries)
     if queries.dim() != 3:
@@ -242,7 +255,7 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     out = torch.empty((n, hq, d), dtype=queries.dtype, device=pages.device)
     lse = torch.empty((n, hq), dtype=torch.float32, device=pages.device) if return_lse else None
     if n:
-        ws = _workspace(pages.device, index, d)
+        ws = _workspace(pages, d)
         a = L.Int4AttnArgs(queries.data_ptr(), L.dtype_code(queries.dtype), queries.stride(0),
                            queries.stride(1), n, hq, hkv, d, pages.data_ptr(), pages.size(0),
                            pages.stride(0), pages.stride(1), page, block_table.data_ptr(),
@@ -257,12 +270,13 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
 _WS: dict[tuple, torch.Tensor] = {}
 
 
-def _workspace(device: torch.device, index: int, head_dim: int) -> torch.Tensor:
+def _workspace(pages: torch.Tensor, head_dim: int) -> torch.Tensor:
+    index = pages.get_device()
     key = (index, L.raw_stream(index), head_dim)
     ws = _WS.get(key)
     if ws is None:
         with torch.cuda.device(index):
-            ws = workspace_for(device, L.entry("ss_int4_attention_workspace")(head_dim), f"int4-{head_dim}")
+            ws = workspace_for(pages.device, L.entry("ss_int4_attention_workspace")(head_dim), f"int4-{head_dim}")
         _WS[key] = ws
     return ws
 
