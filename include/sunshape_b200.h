@@ -428,7 +428,10 @@ int ss_int4_fetch(const int64_t* slots, int64_t n, int n_heads, int d, const voi
  * > 0: so are keys at position - window and before. A row that sees no key
  * gives 0 and lse -inf; so does a token outside cu_q. Keys on a table entry
  * outside the pool are hidden. Bits of a page past a request's length are
- * never used. */
+ * never used. A value with NaN reaches the rows of its request that share its
+ * MMA, those that do not see it among them: 0 * NaN.
+ * Batches with many query rows launch two kernels; the one for many rows has
+ * bounded waits and ORs 32 into the error sink when one gives up. */
 typedef struct ss_int4_attn_args {
   const void* q;                  /* (n_tokens, hq, d), dims contiguous */
   int dtype;                      /* SS_F16 or SS_BF16, of q and out */
@@ -452,6 +455,9 @@ typedef struct ss_int4_attn_args {
   float* lse;                     /* (n_tokens, hq) natural logarithm, or NULL */
   void* workspace;                /* ss_int4_attention_workspace(d) bytes, zeroed once */
   size_t workspace_bytes;
+  int64_t wait_limit_ns;          /* bound of the tile kernel's waits (<= 0: 2 s) */
+  int64_t test_skip_tile;         /* test hook (> 0): tile test_skip_tile - 1 of every CTA of the
+                                     tile kernel waits for keys that never come */
 } ss_int4_attn_args;
 
 /* Bytes of scratch on the current device. The caller zeroes it once and keeps

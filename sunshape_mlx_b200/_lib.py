@@ -109,6 +109,7 @@ class Int4AttnArgs(C.Structure):
         ("scale", f32), ("causal", i32), ("window", i32),
         ("out", vp), ("lse", vp),
         ("workspace", vp), ("workspace_bytes", C.c_size_t),
+        ("wait_limit_ns", i64), ("test_skip_tile", i64),
     ]
 
 

@@ -796,6 +796,8 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     const int rows = most > 16 ? 16 : (int)most;
     p.tiles = most > 16 && a->d != 256;
     p.sink = error_sink();
+    p.wait_ns = a->wait_limit_ns > 0 ? (uint64_t)a->wait_limit_ns : 2000000000ull;
+    p.skip_tile = a->test_skip_tile > 0 ? (uint32_t)(a->test_skip_tile - 1) : 0xffffffffu;
     cudaStream_t st = as_stream(stream);
     if (p.tiles) {
       if (int rc = launch_tiles(p, a->d, st)) return rc;

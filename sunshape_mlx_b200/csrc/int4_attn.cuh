@@ -29,6 +29,8 @@ struct AttnParams {
   uint8_t* ws;
   int n_slots;  // CTAs of the warp-MMA kernel
   int tiles;    // the tile kernel runs too
+  uint64_t wait_ns;   // bound of its waits
+  uint32_t skip_tile; // test hook: tile of a CTA whose keys are never seen (all ones: none)
   int* sink;    // process error sink (host word) or null
 };
 

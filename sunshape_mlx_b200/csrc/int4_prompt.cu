@@ -39,7 +39,6 @@ constexpr int kTileWarps = 20, kTileThreads = kTileWarps * 32;  // whole warpgro
 // Registers of a thread: 96 at launch; 8 * 120 + 8 * 88 + 4 * 64 = 20 * 96.
 constexpr int kSoftRegs = 120, kDecRegs = 88, kMmaRegs = 64;
 constexpr int kHalfKeys = kTileKeys / 2;  // of a softmax thread: a row is two threads' work
-constexpr uint64_t kTileWaitNs = 2000000000ull;
 constexpr int kTileWaitCode = 32;
 
 template <int D>
@@ -242,7 +241,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     for (;;) {
       if (mbar_try_wait(bar, parity)) return true;
       if (*s_abort) return false;
-      if (global_ns() - t0 > kTileWaitNs) {
+      if (global_ns() - t0 > p.wait_ns) {
         if (!*s_abort) report_wait_failure(nullptr, p.sink, kTileWaitCode);
         *s_abort = 1;
         return false;
@@ -665,7 +664,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         }
         for (int j = 0; j < nt && ok; ++j) {
           const uint32_t n = n0 + j, st = n & 1, ph = (n >> 1) & 1;
-          ok = wait(o_done + st, ph ^ 1) && wait(k_full + st, ph);
+          ok = wait(o_done + st, ph ^ 1) && (n != p.skip_tile ? wait(k_full + st, ph) : wait(bars + 12, 0));
           if (!ok) break;
           tc_fence_after();
           if (st == 0) issue_qk<D, 0>(base); else issue_qk<D, 1>(base);
@@ -694,7 +693,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   tc_fence_after();
   if (*s_abort && (tid == kMmaWarp * 32 || tid == kMmaWarp * 32 + 32)) {  // a wait gave up: what was issued must end before the CTA does
     tc_commit(bars + 12);
-    mbar_wait_bounded(bars + 12, 0, kTileWaitNs);
+    mbar_wait_bounded(bars + 12, 0, 2000000000ull);
   }
   tc_fence_before();
   __syncthreads();

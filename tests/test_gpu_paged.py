@@ -499,6 +499,33 @@ def test_attention_in_a_cuda_graph(ss):
     assert torch.equal(out, want)
 
 
+def test_attention_wait_that_runs_out_is_reported_then_recovers(ss):
+    """The tile kernel's waits are bounded: with one tile never announced and a
+    bound of 1 ms the launch gives up, the next call says so, and the one
+    after is right."""
+    import ctypes as C
+
+    from sunshape_mlx_b200 import _lib as L
+    from sunshape_mlx_b200.paged import _workspace
+
+    L.check_device_errors()
+    old, new = [0, 100], [900, 400]
+    pool, table, lens, cu, q, kv = _setup(ss, old, new, 4, 128, 16, 14, torch.float16, 4)
+    out, ws = torch.empty_like(q), _workspace(pool, 128)
+    a = L.Int4AttnArgs(q.data_ptr(), L.SS_F16, q.stride(0), q.stride(1), q.shape[0], 16, 4, 128, pool.data_ptr(), pool.shape[0],
+                       pool.stride(0), pool.stride(1), 16, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(),
+                       cu.data_ptr(), 2, 900, 0.09, 1, 0, out.data_ptr(), None, ws.data_ptr(), ws.numel(), 1_000_000, 2 + 1)
+    L.call("ss_int4_attention", C.byref(a), L.stream_ptr(q.device))
+    torch.cuda.synchronize()
+    args = (q, pool, table, lens, cu, 0.09)
+    with pytest.raises(L.SunShapeCudaError, match="int4_attention tile wait") as e:
+        ss.int4_attention(*args, max_q=900)
+    assert e.value.code == L.SS_ERR_TIMEOUT
+    o, lse = ss.int4_attention(*args, max_q=900, return_lse=True)
+    _check(o, lse, q, kv, old, new, 0.09, True, 0)
+    L.check_device_errors()
+
+
 def test_no_queries(ss):
     pool = ss.int4_pool(1, 2, 16, 64)
     q = torch.empty((0, 4, 64), dtype=torch.float16, device="cuda")
