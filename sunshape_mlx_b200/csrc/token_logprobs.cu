@@ -11,8 +11,8 @@
 // entropy 0. A row that holds NaN or +inf gives NaN, and ids -1.
 // A target < 0 gives 0 (padding), one >= vocab NaN.
 //
-// One pass over a row, by a CTA or, for few rows, by a cluster whose first
-// CTA joins the others' results out of their shared memory. A thread keeps
+// One pass over a row, by a CTA or, for few rows, by a cluster whose CTAs push
+// their results into the first one's shared memory. A thread keeps
 // (M, l, A) of its own elements in fp32 and rescales only when 16 new ones
 // raise its maximum. The k-th largest of the threads' maxima bounds the k-th
 // largest element from below, so only the few threads whose maximum reaches it
@@ -151,6 +151,10 @@ struct LpShared {
   uint32_t tau;
   int hot[kLpThreads];
   int n_hot, n_cand, n_top;
+  // what the parts of a row push to the first one's shared memory
+  uint32_t all_key[kLpMaxSplit * kLpMaxTop];
+  int all_idx[kLpMaxSplit * kLpMaxTop];
+  Sums all_sums[kLpMaxSplit];
   int wsum[kLpWarps];
 };
 
@@ -187,6 +191,8 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
   const int per = (vecs + split - 1) / split, v0 = min(vecs, part * per), v1 = min(vecs, v0 + per);
   const uint4* body = reinterpret_cast<const uint4*>(base + head * ES);
   if (tid == 0) s.n_hot = s.n_cand = 0;
+  // the first part's shared memory is there once every CTA of the cluster has started
+  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   // ---- sums ----
   float m = -INFINITY, l[2] = {0.f, 0.f}, a[2] = {0.f, 0.f};
@@ -439,34 +445,28 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
   const int* ti = s.top_idx;
   if (split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    if (part == 0) {
-      int n = 0;
-      for (int c = 0; c < split; ++c) {
-        const LpShared* o = cluster.map_shared_rank(&s, c);
-        const int oc = o->n_top;
-        for (int i = tid; i < oc; i += kLpThreads) {
-          s.key[n + i] = o->top_key[i];
-          s.idx[n + i] = o->top_idx[i];
-        }
-        n += oc;
-        if (c > 0) {
-          const Sums y = o->sums;
-          const float w = max_nan(sum.m, y.m);
-          sum = merge(sum, y);
-          sum.m = w;
-        }
-      }
-      __syncthreads();
-      // the places 8 * 32 .. of the lists are free
-      rank_candidates(s.key, s.idx, n, k, s.key + kLpMaxSplit * kLpMaxTop, s.idx + kLpMaxSplit * kLpMaxTop);
-      __syncthreads();
-      tk = s.key + kLpMaxSplit * kLpMaxTop;
-      ti = s.idx + kLpMaxSplit * kLpMaxTop;
-      n_top = min(n, k);
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    LpShared* first = cluster.map_shared_rank(&s, 0);
+    if (tid < k) {  // past this part's elements: what ranks behind everything
+      first->all_key[part * k + tid] = tid < n_top ? s.top_key[tid] : 0u;
+      first->all_idx[part * k + tid] = tid < n_top ? s.top_idx[tid] : 0x7fffffff - part * kLpMaxTop - tid;
     }
-    cluster.sync();  // nobody leaves while its shared memory is read
+    if (tid == 0) first->all_sums[part] = sum;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (part != 0) return;
+    float worst_m = -INFINITY;
+    sum = s.all_sums[0];
+    for (int c = 0; c < split; ++c) {
+      worst_m = max_nan(worst_m, s.all_sums[c].m);
+      if (c > 0) sum = merge(sum, s.all_sums[c]);
+    }
+    sum.m = worst_m;
+    rank_candidates(s.all_key, s.all_idx, split * k, k, s.key, s.idx);
+    __syncthreads();
+    tk = s.key;
+    ti = s.idx;
+    n_top = min(k, p.vocab);
   }
 
   const bool bad = !(sum.m < INFINITY), none = sum.m == -INFINITY;
