@@ -186,7 +186,10 @@ __global__ void __launch_bounds__(Shape<D, MODE, WIDE>::W * 32, Shape<D, MODE, W
                                    : (total + kMinCost + kSegCost - 1) / (kMinCost + kSegCost);
   want = want < units ? units : want;
   const int nc = (int)(want < gridDim.x ? want : (int64_t)gridDim.x);
-  if ((int)blockIdx.x >= nc) return;
+  if ((int)blockIdx.x >= nc) {
+    grid_dependency_wait();
+    return;
+  }
   // (64-bit divisions take some 100 cycles each, and these stand before the first copy)
   const bool small = total < (1 << 22);  // products with nc + 1 <= 2 * 148 + 1 stay below 2^31
   auto range_start = [&](int i) -> int64_t {
@@ -719,6 +722,9 @@ __global__ void __launch_bounds__(Shape<D, MODE, WIDE>::W * 32, Shape<D, MODE, W
     __syncthreads();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  // The tile kernel of the same call may still run beside this one (programmatic dependent launch):
+  // this grid ends after it, so that what follows on the stream finds both results.
+  grid_dependency_wait();
 }
 
 // Workspace: a counter per CTA, then two parts per CTA of R rows of D + 2 floats
@@ -734,7 +740,21 @@ int launch_shape(AttnParams& p, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, MODE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   if (e != cudaSuccess) return fail(SS_ERR_CUDA, std::string("ss_int4_attention: ") + cudaGetErrorString(e));
   p.n_slots = sm_count() * Sh::kCtas;
-  attn_decode_kernel<D, MODE, WIDE><<<p.n_slots, Sh::W * 32, Sh::kSmem, st>>>(p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.n_slots);
+  cfg.blockDim = dim3(Sh::W * 32);
+  cfg.dynamicSmemBytes = Sh::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.tiles ? 1 : 0;  // beside the tile kernel: the two write different rows
+  const cudaError_t e2 = cudaLaunchKernelEx(&cfg, attn_decode_kernel<D, MODE, WIDE>, p);
+  if (e2 != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SS_ERR_CUDA, std::string("ss_int4_attention: ") + cudaGetErrorString(e2));
+  }
   return check_launch("ss_int4_attention");
 }
 

@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   // ---- setup ---------------------------------------------------------------
+  grid_launch_dependents();  // the warp-MMA kernel of the same call: other rows, its own workspace
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(k_full + s, kDecWarps);
