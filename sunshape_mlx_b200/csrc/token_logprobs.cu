@@ -39,7 +39,7 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxSplit = 8;
 constexpr int kLpCap = 1024;     // candidates of a CTA
-constexpr int kLpVecs = 2;       // 16-byte loads of a thread in flight
+constexpr int kLpVec = 32;       // bytes of a load: a whole sector, so that reading elements again wastes none
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -1e30f;   // stands for -inf in differences: its exponential is 0, times it is 0
 
@@ -91,27 +91,34 @@ __device__ __forceinline__ bool before(uint32_t k, int i, uint32_t k2, int i2) {
   return k > k2 || (k == k2 && i < i2);
 }
 
+struct Words {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Words load32(const void* p) {
+  Words r;
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+               : "l"(p));
+  return r;
+}
+
 template <int DT>
 struct Vec {
-  static constexpr int E = DT == SS_F32 ? 4 : 8;  // elements of 16 bytes
-  static __device__ __forceinline__ void get(const uint4& u, float (&x)[E]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  static constexpr int E = DT == SS_F32 ? 8 : 16;  // elements of a load
+  static __device__ __forceinline__ void get(const Words& u, float (&x)[E]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       if constexpr (DT == SS_F32) {
-        x[i] = __uint_as_float(w[i]);
+        x[i] = __uint_as_float(u.w[i]);
       } else if constexpr (DT == SS_BF16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        x[2 * i] = __uint_as_float(u.w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u.w[i] & 0xffff0000u);
       } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u.w[i]));
         x[2 * i] = f.x;
         x[2 * i + 1] = f.y;
       }
     }
-  }
-  static __device__ __forceinline__ uint32_t low() {  // two (one) elements of -inf
-    return DT == SS_F32 ? 0xff800000u : DT == SS_F16 ? 0xfc00fc00u : 0xff80ff80u;
   }
 };
 
@@ -184,12 +191,12 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
   const int part = blockIdx.x % split;
   constexpr int ES = DT == SS_F32 ? 4 : 2;
   const char* base = reinterpret_cast<const char*>(p.x) + row * p.row_stride * ES;
-  // elements before the first 16-byte boundary, then vectors, then the rest
-  int head = (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / ES;
+  // elements before the first 32-byte boundary, then whole loads, then the rest
+  int head = (int)((kLpVec - (reinterpret_cast<uintptr_t>(base) & (kLpVec - 1))) & (kLpVec - 1)) / ES;
   head = min(head, p.vocab);
   const int vecs = (p.vocab - head) / E, tail0 = head + vecs * E;
   const int per = (vecs + split - 1) / split, v0 = min(vecs, part * per), v1 = min(vecs, v0 + per);
-  const uint4* body = reinterpret_cast<const uint4*>(base + head * ES);
+  const char* body = base + head * ES;
   if (tid == 0) s.n_hot = s.n_cand = 0;
   // the first part's shared memory is there once every CTA of the cluster has started
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -206,29 +213,17 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
     }
     m = max_nan(m, lm);
   };
-  uint4 buf[kLpVecs];
-  auto load = [&](int v) {
+  Words buf;
+  if (v0 + tid < v1) buf = load32(body + (int64_t)(v0 + tid) * kLpVec);
+  for (int v = v0 + tid; v < v1; v += kLpThreads) {
+    float x[E];
+    Vec<DT>::get(buf, x);
+    if (v + kLpThreads < v1) buf = load32(body + (int64_t)(v + kLpThreads) * kLpVec);
+    float lm = x[0];
 #pragma unroll
-    for (int u = 0; u < kLpVecs; ++u) {
-      const int at = v + u * kLpThreads;
-      buf[u] = at < v1 ? __ldcs(body + at) : make_uint4(Vec<DT>::low(), Vec<DT>::low(), Vec<DT>::low(), Vec<DT>::low());
-    }
-  };
-  if (v0 + tid < v1) load(v0 + tid);
-  for (int v = v0 + tid; v < v1; v += kLpVecs * kLpThreads) {
-    float x[kLpVecs][E];
-#pragma unroll
-    for (int u = 0; u < kLpVecs; ++u) Vec<DT>::get(buf[u], x[u]);
-    if (v + kLpVecs * kLpThreads < v1) load(v + kLpVecs * kLpThreads);
-    float lm = x[0][0];
-#pragma unroll
-    for (int u = 0; u < kLpVecs; ++u) {
-#pragma unroll
-      for (int i = 0; i < E; i += 2) lm = max3_nan(lm, x[u][i], x[u][i + 1]);
-    }
+    for (int i = 0; i < E; i += 2) lm = max3_nan(lm, x[i], x[i + 1]);
     raise(lm);
-#pragma unroll
-    for (int u = 0; u < kLpVecs; ++u) add_up(x[u], m, l, a);
+    add_up(x, m, l, a);
   }
   // the ragged ends belong to the first part: a thread takes at most one element of each
   const int n_ends = part == 0 ? head + p.vocab - tail0 : 0;
@@ -302,7 +297,7 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
         const int v = v0 + w / n_hot * kLpThreads + s.hot[w % n_hot];
         if (v < v1) {
           float x[E];
-          Vec<DT>::get(body[v], x);
+          Vec<DT>::get(load32(body + (int64_t)v * kLpVec), x);
 #pragma unroll
           for (int i = 0; i < E; ++i) offer(x[i], head + v * E + i);
         }
@@ -336,7 +331,7 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
         const int v = v0 + w / n_above * kLpThreads + s.hot[w % n_above];
         if (v < v1) {
           float x[E];
-          Vec<DT>::get(body[v], x);
+          Vec<DT>::get(load32(body + (int64_t)v * kLpVec), x);
 #pragma unroll
           for (int i = 0; i < E; ++i) list(x[i], head + v * E + i);
         }
@@ -355,7 +350,7 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
           x[0] = end_x;
         } else if (v0 + st * kLpThreads + tid < v1) {
           const int v = v0 + st * kLpThreads + tid;
-          Vec<DT>::get(body[v], x);
+          Vec<DT>::get(load32(body + (int64_t)v * kLpVec), x);
           at = head + v * E;
           n = E;
         }
@@ -407,7 +402,7 @@ __global__ void __launch_bounds__(kLpThreads, 5) logprobs_kernel(const __grid_co
         };
         for (int v = v0 + tid; v < v1; v += kLpThreads) {
           float x[E];
-          Vec<DT>::get(body[v], x);
+          Vec<DT>::get(load32(body + (int64_t)v * kLpVec), x);
 #pragma unroll
           for (int i = 0; i < E; ++i) look(x[i], head + v * E + i);
         }
