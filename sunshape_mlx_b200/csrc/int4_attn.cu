@@ -640,11 +640,10 @@ __global__ void __launch_bounds__(Shape<D, MODE, WIDE>::W * 32, Shape<D, MODE, W
     const int c_first = cta_of(body), c_last = cta_of(body + r.nblk - 1);
     const bool whole = c_first == c_last;
     constexpr int kPart = R * (D + 2);
-    float* parts = reinterpret_cast<float*>(p.ws + ((size_t)p.n_slots * 4 + 15) / 16 * 16);
     // a CTA leaves at most two parts: of the unit it starts in (the first slot), and of the one it
     // ends in; only a unit's first CTA can have started in another one
     const int first_slot = range_start(c_first) >= walk.at ? 0 : 1;
-    auto slot_of = [&](int c) { return parts + (size_t)(2 * c + (c == c_first ? first_slot : 0)) * kPart; };
+    auto slot_of = [&](int c) { return p.parts + (size_t)(2 * c + (c == c_first ? first_slot : 0)) * kPart; };
     float* mine = whole ? nullptr : slot_of(blockIdx.x);
     auto finish = [&](int row, int dim, float4 v, float mm, float ll) {  // 4 dims of a row
       const int rr = row0 + row, hd = walk.h * p.grp + rr % p.grp;
@@ -728,9 +727,11 @@ __global__ void __launch_bounds__(Shape<D, MODE, WIDE>::W * 32, Shape<D, MODE, W
 }
 
 // Workspace: a counter per CTA, then two parts per CTA of R rows of D + 2 floats
-// (up to 16 rows for one CTA on an SM, up to 8 for two).
+// (up to 16 rows for one CTA on an SM, up to 8 for two). Launches of every shape share it, so the
+// counters' room is that of the most CTAs: a part never lies over a counter.
+size_t attn_counter_bytes(int sms) { return ((size_t)sms * 2 * 4 + 15) / 16 * 16; }
 size_t attn_ws_bytes(int d, int sms) {
-  return ((size_t)sms * 2 * 4 + 15) / 16 * 16 + (size_t)sms * 2 * 16 * (d + 2) * 4;
+  return attn_counter_bytes(sms) + (size_t)sms * 2 * 16 * (d + 2) * 4;
 }
 
 template <int D, int MODE, bool WIDE>
@@ -822,7 +823,8 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.seq_lens = a->seq_lens; p.cu_q = a->cu_q; p.n = a->n_requests;
     p.scale = a->scale; p.causal = a->causal; p.window = a->window;
     p.out = a->out; p.lse = a->lse;
-    p.ws = static_cast<uint8_t*>(a->workspace); p.n_slots = 0;
+    p.ws = static_cast<uint8_t*>(a->workspace);
+    p.parts = reinterpret_cast<float*>(p.ws + attn_counter_bytes(ctas));
     const int64_t most = (int64_t)a->max_q * p.grp;
     const int rows = most > 16 ? 16 : (int)most;
     p.tiles = most > 16 && a->d != 256;

@@ -26,7 +26,8 @@ struct AttnParams {
   int causal, window;
   void* out;
   float* lse;
-  uint8_t* ws;
+  uint8_t* ws;    // counters of the warp-MMA kernel's CTAs
+  float* parts;   // and their parts: a place that does not depend on the kernel's shape
   int n_slots;  // CTAs of the warp-MMA kernel
   int tiles;    // the tile kernel runs too
   uint64_t wait_ns;   // bound of its waits

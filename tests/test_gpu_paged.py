@@ -394,6 +394,25 @@ def test_attention_scales_of_tiny_and_large_values(ss):
             assert ((o.double() - want).abs() <= 2.0 ** -11 * want.abs() + (4 * 2.0 ** -11 + 2 * dz) * pv + 2.0 ** -24).all()
 
 
+def test_attention_launches_of_every_shape_share_a_workspace(ss):
+    """Units cut into parts, by launches with one and two CTAs on an SM and
+    units of 4, 8 and 16 rows, in turn on one stream: every one finds its
+    counters at zero."""
+    cases = []
+    for i, (old, new, grp) in enumerate([([40000], [1], 4), ([3000] * 24, [1] * 24, 4), ([20000, 9000], [2, 2], 8), ([50000], [1], 8),
+                                         ([2500] * 40, [1] * 40, 8), ([30000], [4], 4)]):
+        cases.append((_setup(ss, old, new, 8, 128, 64, 20 + i, torch.bfloat16, grp), old, new))
+    first = None
+    for _ in range(3):
+        out = [ss.int4_attention(q, pool, t, ln, cu, 0.09, max_q=max(new), return_lse=True) for (pool, t, ln, cu, q, kv), old, new in cases]
+        if first is None:
+            first = out
+            for ((pool, t, ln, cu, q, kv), old, new), (o, lse) in zip(cases, out):
+                _check(o, lse, q, kv, old, new, 0.09, True, 0)
+        for (o, lse), (o1, lse1) in zip(out, first):
+            assert torch.equal(o, o1) and torch.equal(lse, lse1)
+
+
 @pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
 def test_attention_any_scale(ss, scale):
     for old, new, d in (([200, 30], [1, 1], 128), ([0, 60], [400, 300], 64)):
