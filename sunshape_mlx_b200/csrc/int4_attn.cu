@@ -8,15 +8,17 @@
 //
 // Split. A unit is (request, kv-head, up to R query rows): the rows share its
 // keys, so a block is read once for all of them. The blocks of all units in a
-// row are cut into ranges of equal cost, one per CTA (persistent, one CTA per
-// SM); a unit cut by a range boundary leaves partial (o, m, l) rows in the
+// row are cut into ranges of equal cost, one per CTA (persistent, one or two CTAs
+// on an SM); a unit cut by a range boundary leaves partial (o, m, l) rows in the
 // workspace and the last CTA to arrive joins them in the order of the ranges,
 // so results do not depend on timing. Lengths are read on the GPU: nothing
 // waits for the host.
 //
-// One warp takes a 16-token block at a time, with its own ring of cp.async
-// copies (20 D contiguous bytes a block) and its own softmax state; the warps
-// meet at the end of a unit only.
+// One warp takes two 16-token blocks at a time (one for D = 256 and for 16 rows,
+// whose state fills the registers), with its own ring of cp.async copies (20 D
+// contiguous bytes a block) and its own softmax state; the warps meet at the end
+// of a unit only. Two CTAs of 6 warps share an SM, so that one joins its warps
+// while the other streams; with no more units than SMs it is one of 12.
 //   S^T (16 tokens x 8 rows) by warp MMAs. With code c, scale s and zero z of
 //   a (token, group): q . k = sum_g s_g (sum_d q_d c_d) + sum_g z_g (sum_d q_d).
 //   A nibble masked out of its word is, read as fp16, the subnormal c 2^-24 or
@@ -34,6 +36,14 @@
 //   the output's); for up to 4 rows lo uses the columns that are free anyway.
 // The softmax reference of a row moves only when a logit exceeds it by 2^8:
 // the usual block needs one vote and no shuffles.
+//
+// Measured (D = 128, 8 kv heads): 1 request of 524288 tokens, 64 heads, fp16 149 us
+// (4.5 TB/s); 32 requests of 500 to 16384 tokens, bf16 87 us (4.1 TB/s); 1 of 777
+// tokens 12 us. HBM would allow 103 and 55 us: a block costs about 340 warp
+// instructions, 57 % of the issue slots at that rate, and what is left is
+// latency within a warp's block (the registers hold 12 warps an SM). One block at
+// a time took 163 and 123 us; keys rounded from nibbles to fp16 by conversions
+// 179 and 129 us.
 #include "int4_attn.cuh"
 
 namespace ss {

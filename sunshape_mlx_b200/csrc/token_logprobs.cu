@@ -17,14 +17,16 @@
 // raise its maximum. The k-th largest of the threads' maxima bounds the k-th
 // largest element from below, so only the few threads whose maximum reaches it
 // hold candidates: their elements alone are read again (3 % of a row at k =
-// 8), by all threads together, and ranked against each other. Where more
+// 8, in whole sectors), by all threads together, and ranked against each other. Where more
 // elements reach the bound than are listed (a constant row), those above it are
 // listed and the first equal ones taken in order.
 //
 // Bound by HBM; an element costs about 5.5 issue slots, one of them exp2, at
 // half of what an SM can issue at full bandwidth. 256 threads and five CTAs an
 // SM, so that rows in their last phase overlap rows that stream: 2047 x 128256
-// bf16, top 8: 109 us (4.8 TB/s), 112 us with 512 threads and two CTAs.
+// bf16, top 8: 103.5 us (5.1 TB/s); with loads of 16 bytes, of whose sectors the
+// second reading used half, 109 us, and then 112 with 512 threads and two CTAs.
+// 333 x 50257 fp32, top 5: 16 us; one row of 128256: 9.5 us, latency.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
