@@ -44,6 +44,8 @@
 // latency within a warp's block (the registers hold 12 warps an SM). One block at
 // a time took 163 and 123 us; keys rounded from nibbles to fp16 by conversions
 // 179 and 129 us.
+#include <algorithm>
+
 #include "int4_attn.cuh"
 
 namespace ss {
@@ -737,11 +739,13 @@ __global__ void __launch_bounds__(Shape<D, MODE, WIDE>::W * 32, Shape<D, MODE, W
 }
 
 // Workspace: a counter per CTA, then two parts per CTA of R rows of D + 2 floats
-// (up to 16 rows for one CTA on an SM, up to 8 for two). Launches of every shape share it, so the
-// counters' room is that of the most CTAs: a part never lies over a counter.
+// (up to 16 rows for one CTA on an SM, up to 8 for two), and the same again for the tile kernel,
+// which may run beside. Launches of every shape share it, so the counters' room is that of the
+// most CTAs: a part never lies over a counter.
 size_t attn_counter_bytes(int sms) { return ((size_t)sms * 2 * 4 + 15) / 16 * 16; }
+size_t attn_part_bytes(int d, int sms) { return (size_t)sms * 2 * 16 * (d + 2) * 4; }
 size_t attn_ws_bytes(int d, int sms) {
-  return attn_counter_bytes(sms) + (size_t)sms * 2 * 16 * (d + 2) * 4;
+  return 2 * attn_counter_bytes(sms) + attn_part_bytes(d, sms) + (d == 256 ? 0 : (size_t)sms * tile_part_floats(d) * 4);
 }
 
 template <int D, int MODE, bool WIDE>
@@ -834,10 +838,16 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.scale = a->scale; p.causal = a->causal; p.window = a->window;
     p.out = a->out; p.lse = a->lse;
     p.ws = static_cast<uint8_t*>(a->workspace);
-    p.parts = reinterpret_cast<float*>(p.ws + attn_counter_bytes(ctas));
+    p.tile_ws = reinterpret_cast<uint32_t*>(p.ws + attn_counter_bytes(ctas));
+    p.parts = reinterpret_cast<float*>(p.ws + 2 * attn_counter_bytes(ctas));
+    p.tile_parts = reinterpret_cast<float*>(p.ws + 2 * attn_counter_bytes(ctas) + attn_part_bytes(a->d, ctas));
     const int64_t most = (int64_t)a->max_q * p.grp;
     const int rows = most > 16 ? 16 : (int)most;
     p.tiles = most > 16 && a->d != 256;
+    // The host does not know the lengths: a request's rows over 128, and one more for each request
+    // with enough rows, or max_q's tiles for each. The hint may be wrong: it chooses a variant.
+    const int64_t all_rows = p.n_tokens * p.grp;
+    p.tile_units = std::min(all_rows / 128 + std::min<int64_t>(p.n, all_rows / 17), (most + 127) / 128 * p.n) * p.hkv;
     p.sink = error_sink();
     p.wait_ns = a->wait_limit_ns > 0 ? (uint64_t)a->wait_limit_ns : 2000000000ull;
     p.skip_tile = a->test_skip_tile > 0 ? (uint32_t)(a->test_skip_tile - 1) : 0xffffffffu;

@@ -28,8 +28,11 @@ struct AttnParams {
   float* lse;
   uint8_t* ws;    // counters of the warp-MMA kernel's CTAs
   float* parts;   // and their parts: a place that does not depend on the kernel's shape
+  uint32_t* tile_ws;  // the tile kernel's counters, 4 per unit
+  float* tile_parts;  // and its parts, one per CTA
   int n_slots;  // CTAs of the warp-MMA kernel
   int tiles;    // the tile kernel runs too
+  int64_t tile_units;  // about how many units it has at most
   uint64_t wait_ns;   // bound of its waits
   uint32_t skip_tile; // test hook: tile of a CTA whose keys are never seen (all ones: none)
   int* sink;    // process error sink (host word) or null
@@ -40,12 +43,19 @@ constexpr float kSlack = 8.f;    // a logit may exceed the reference by this (ba
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Rows (query tokens times heads of a group) from which a request's queries go to the tiles of
-// 128 rows of the tcgen05 kernel instead of the 16-row units of the warp-MMA kernel. A tile is a
-// CTA's work alone, the units of a request are spread over all SMs: the tiles win once about nine
-// CTAs' worth of full tiles run at once.
-__device__ __forceinline__ bool to_tiles(const AttnParams& p, int nq) {
-  const int64_t rows = (int64_t)nq * p.grp;
-  return p.tiles && rows > 16 && rows * p.hkv >= 1152;
+// 128 rows of the tcgen05 kernel instead of the 16-row units of the warp-MMA kernel. A tile is one
+// CTA's work, or a few CTAs' where there are few tiles; the units of a request are spread over all
+// SMs, but read and decode the keys once per 16 rows. The tiles win once about nine full tiles run
+// at once, whatever the keys, and from 48 rows where rows times heads times keys reach 2^21 (8 kv
+// heads, 128 dims, units against tiles: 68 rows over 4017 keys 37 and 35 us, over 517 keys 18 and 28;
+// 128 rows over 30000 keys 125 and 65; 8 requests of 36 rows over 4009 keys 69 and 68, 8 of 128
+// rows over 4032 152 and 52).
+constexpr float kTilesFrom = 1152.f, kTileRowsFrom = 48.f, kTileWorkFrom = 0x1p21f;
+
+__device__ __forceinline__ bool to_tiles(const AttnParams& p, int nq, int len) {
+  const float rows = (float)nq * p.grp, all = rows * p.hkv;
+  const float keys = p.window > 0 ? fminf((float)len, (float)p.window + nq) : (float)len;
+  return p.tiles && rows > 16.f && (all >= kTilesFrom || (rows >= kTileRowsFrom && all * keys >= kTileWorkFrom));
 }
 
 // What a request contributes to the schedule of the warp-MMA kernel.
@@ -59,7 +69,7 @@ __device__ __forceinline__ Req load_req(const AttnParams& p, int b) {
   const int c0 = max(p.cu_q[b], 0);
   r.nq = max(p.cu_q[b + 1] - c0, 0);
   r.len = min(max(p.seq_lens[b], 0), p.width * p.page);
-  r.rbs = to_tiles(p, r.nq) ? 0 : (int)(((int64_t)r.nq * p.grp + R - 1) / R);
+  r.rbs = to_tiles(p, r.nq, r.len) ? 0 : (int)(((int64_t)r.nq * p.grp + R - 1) / R);
   r.blk0 = p.window > 0 ? max(0, r.len - r.nq - p.window + 1) / kBlkTokens : 0;
   r.nblk = max(1, (r.len + kBlkTokens - 1) / kBlkTokens - r.blk0);
   return r;
@@ -106,6 +116,9 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float lo_h(uint32_t x) { return __low2float(*reinterpret_cast<__half2*>(&x)); }
 __device__ __forceinline__ float hi_h(uint32_t x) { return __high2float(*reinterpret_cast<__half2*>(&x)); }
 
+
+// Floats of a CTA's part in the tile kernel: 128 rows of D dims, reference and sum.
+__host__ __device__ constexpr int tile_part_floats(int d) { return 128 * (d + 2); }
 
 // The requests of a batch that have query rows for the tiles, see int4_prompt.cu.
 int launch_tiles(AttnParams& p, int d, cudaStream_t st);

@@ -413,6 +413,51 @@ def test_attention_launches_of_every_shape_share_a_workspace(ss):
             assert torch.equal(o, o1) and torch.equal(lse, lse1)
 
 
+@pytest.mark.parametrize("old,new,hkv,grp,d,dtype,causal,window", [
+    ([4000], [64], 8, 4, 128, torch.bfloat16, True, 0),        # 16 units of 32 tiles
+    ([5001], [37], 8, 4, 128, torch.float16, True, 0),         # ragged rows and keys
+    ([3000, 900, 0], [40, 50, 130], 4, 8, 64, torch.float16, True, 0),  # units of 1 to 24 tiles
+    ([2500, 2500], [40, 1], 8, 4, 64, torch.bfloat16, True, 1300),      # a window, and a decoding request
+    ([2000], [200], 2, 3, 128, torch.float16, False, 0),
+    ([20000], [1200], 1, 1, 128, torch.bfloat16, True, 0),
+    ([3000] * 4, [32] * 4, 8, 4, 128, torch.float16, True, 0),  # tiles for the length of their keys
+    ([3000, 70, 3000], [12, 12, 11], 8, 4, 64, torch.bfloat16, True, 0),  # and just not
+])
+def test_attention_few_tiles_are_cut_along_the_keys(ss, old, new, hkv, grp, d, dtype, causal, window):
+    pool, table, lens, cu, q, kv = _setup(ss, old, new, hkv, d, 64, sum(old) + d, dtype, grp, pad=3)
+    first = None
+    for _ in range(3):  # the order of arrival does not matter, and counters are left as they were found
+        o, lse = ss.int4_attention(q, pool, table, lens, cu, 0.09, max_q=max(new), causal=causal, window=window, return_lse=True)
+        if first is None:
+            first = o, lse
+            _check(o, lse, q, kv, old, new, 0.09, causal, window)
+        assert torch.equal(o, first[0]) and torch.equal(lse, first[1])
+
+
+def test_attention_cut_tiles_wait_that_runs_out_then_recovers(ss):
+    """Parts that give up still arrive: the counters of their units end at zero."""
+    import ctypes as C
+
+    from sunshape_mlx_b200 import _lib as L
+    from sunshape_mlx_b200.paged import _workspace
+
+    L.check_device_errors()
+    old, new = [4000], [64]
+    pool, table, lens, cu, q, kv = _setup(ss, old, new, 8, 128, 16, 15, torch.bfloat16, 4)
+    out, ws = torch.empty_like(q), _workspace(pool, 128)
+    a = L.Int4AttnArgs(q.data_ptr(), L.SS_BF16, q.stride(0), q.stride(1), q.shape[0], 32, 8, 128, pool.data_ptr(), pool.shape[0],
+                       pool.stride(0), pool.stride(1), 16, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(),
+                       cu.data_ptr(), 1, 64, 0.09, 1, 0, out.data_ptr(), None, ws.data_ptr(), ws.numel(), 1_000_000, 2 + 1)
+    L.call("ss_int4_attention", C.byref(a), L.stream_ptr(q.device))
+    torch.cuda.synchronize()
+    args = (q, pool, table, lens, cu, 0.09)
+    with pytest.raises(L.SunShapeCudaError, match="int4_attention tile wait"):
+        ss.int4_attention(*args, max_q=64)
+    o, lse = ss.int4_attention(*args, max_q=64, return_lse=True)
+    _check(o, lse, q, kv, old, new, 0.09, True, 0)
+    L.check_device_errors()
+
+
 @pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
 def test_attention_any_scale(ss, scale):
     for old, new, d in (([200, 30], [1, 1], 128), ([0, 60], [400, 300], 64)):
