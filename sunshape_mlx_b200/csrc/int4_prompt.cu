@@ -4,7 +4,9 @@
 // A unit is (request, kv-head, 128 query rows); the rows of a group's heads and
 // of consecutive tokens share a tile, so keys and values are decoded once for
 // all of them. CTAs (one an SM) take units in turn, those with most keys of a
-// request first, rounds in alternating direction. Per tile of 128 tokens:
+// request first, rounds in alternating direction; where there are few units their
+// keys are cut into parts (fp32 rows of O, reference and sum in the workspace,
+// joined by the last of them to arrive, in order). Per tile of 128 tokens:
 //   decode    (8 warps)  codes -> fp16 operands in shared memory
 //   S = Q K^T (1 thread) M = 128, N = 128, fp32 in TMEM, two buffers
 //   softmax   (8 warps)  two threads a row, P as fp16 over its S in TMEM
@@ -27,8 +29,8 @@
 // logits exceed its reference by 2^8.
 //
 // Measured: one causal prompt of 8192 tokens, 32 query heads on 8, D = 128: bf16
-// 865 us (635 TFLOP/s of the formula's 4 D a pair; the tensor cores do half as
-// much again for lo), fp16 1017 us, D = 64 680 us. A tile of 128 keys takes
+// 860 us (640 TFLOP/s of the formula's 4 D a pair; the tensor cores do half as
+// much again for lo), fp16 1013 us, D = 64 685 us. A tile of 128 keys takes
 // 1.9 us: the tensor pipe is busy 40 % of the time, issue slots 55 %, shared
 // memory 46 %; no one of them is full, the chain decode - S - softmax - O of two
 // tiles in flight is (a third tile has no room: two stages take 205 KB, and S, P,
@@ -165,7 +167,9 @@ struct Unit {
 
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
   const int nq = max(p.cu_q[b + 1] - max(p.cu_q[b], 0), 0);
-  return to_tiles(p, nq, min(max(p.seq_lens[b], 0), p.width * p.page)) ? (int)(((int64_t)nq * p.grp + kTileRows - 1) / kTileRows) : 0;
+  int len = 0;
+  if ((float)nq * p.grp * p.hkv < kTilesFrom) len = min(max(p.seq_lens[b], 0), p.width * p.page);
+  return to_tiles(p, nq, len) ? (int)(((int64_t)nq * p.grp + kTileRows - 1) / kTileRows) : 0;
 }
 // Keys [beg, end) that the row of query token i sees.
 __device__ __forceinline__ void row_keys(const AttnParams& p, int nq, int len, int i, int& beg, int& end) {
@@ -286,6 +290,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
       if (s_cum[mid] <= u) a = mid; else e = mid;
     }
     int at = s_cum[a], b = a * per, tiles = 0;
+#pragma unroll 1
     for (;; ++b) {
       tiles = tiles_of(p, b);
       if (at + tiles * p.hkv > u) break;
@@ -405,6 +410,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         tc_fence_before();
       }
       ok = pair_sync();
+      if (!SPLIT && !ok) break;  // parts arrive all the same
       const float fac = s_fac[r];
       if (ok && lane == 0 && half == 0 && nt > 0) mbar_arrive(q_full);  // and O of the unit before has been read
 
@@ -799,8 +805,8 @@ int launch_kernel(AttnParams& p, cudaStream_t st) {
 template <int D, bool LO>
 int launch(AttnParams& p, cudaStream_t st) {
   // Both variants are right for any number of units; the one that can cut them along the keys takes
-  // 1 to 8 % more time where it cannot (a prompt of 8192: 871 against 865 us bf16, 1066 against 1020
-  // fp16), and where it can, 64 query tokens over 30000 keys, 32 heads on 8, take 81 instead of 389 us.
+  // 1 to 8 % more time where it cannot (a prompt of 8192: 871 against 860 us bf16, 1066 against 1020
+  // fp16), and where it can, 64 query tokens over 30000 keys, 32 heads on 8, take 78 instead of 389 us.
   if (2 * p.tile_units <= sm_count()) return launch_kernel<D, LO, true>(p, st);
   return launch_kernel<D, LO, false>(p, st);
 }
