@@ -17,8 +17,8 @@
 // One warp takes two 16-token blocks at a time (one for D = 256 and for 16 rows,
 // whose state fills the registers), with its own ring of cp.async copies (20 D
 // contiguous bytes a block) and its own softmax state; the warps meet at the end
-// of a unit only. Two CTAs of 6 warps share an SM, so that one joins its warps
-// while the other streams; with no more units than SMs it is one of 12.
+// of a unit only. Two CTAs of 6 warps (D = 256: 4) share an SM, so that one joins
+// its warps while the other streams; with no more units than SMs it is one of 12 (8).
 //   S^T (16 tokens x 8 rows) by warp MMAs. With code c, scale s and zero z of
 //   a (token, group): q . k = sum_g s_g (sum_d q_d c_d) + sum_g z_g (sum_d q_d).
 //   A nibble masked out of its word is, read as fp16, the subnormal c 2^-24 or
@@ -58,15 +58,15 @@ constexpr int kMinCost = 96;     // a range is not cut below this many blocks' w
 enum { kRows4, kRows8, kRows8Lo, kRows16, kRows16Lo };
 __host__ __device__ constexpr int mode_rows(int m) { return m == kRows4 ? 4 : m <= kRows8Lo ? 8 : 16; }
 
-// WIDE: one CTA of 12 warps on an SM instead of two of 6.
+// WIDE: one CTA of 12 warps on an SM instead of two of 6 (D = 256: of 8 instead of two of 4).
 template <int D, int MODE, bool WIDE>
 struct Shape {
   static constexpr int R = mode_rows(MODE);
   static constexpr int NR = R == 16 ? 2 : 1;       // 8-column tiles
   static constexpr bool LO = MODE == kRows8Lo || MODE == kRows16Lo;  // a second MMA for lo
   static constexpr int U = D == 256 || NR == 2 ? 1 : 2;  // blocks a warp takes at a time
-  static constexpr int kCtas = U == 2 && !WIDE ? 2 : 1;  // CTAs on an SM: one joins its warps while the other streams
-  static constexpr int W = U == 1 ? 8 : WIDE ? 12 : 6;   // warps
+  static constexpr int kCtas = (U == 2 || D == 256) && !WIDE ? 2 : 1;  // CTAs on an SM: one joins its warps while the other streams
+  static constexpr int W = D == 256 ? (WIDE ? 8 : 4) : U == 1 ? 8 : WIDE ? 12 : 6;   // warps
   static constexpr int S = D == 64 ? 4 : D == 256 ? 3 : U == 2 ? 2 : 4;  // ring stages of a warp
   static constexpr int kRing = W * S * U * Int4Blk<D>::kBytes;
   static constexpr int kMerge = W * R * (D + 4) * 4;  // rows padded by 4 floats
@@ -774,21 +774,25 @@ int launch_shape(AttnParams& p, cudaStream_t st) {
 }
 
 template <int D, int MODE>
-int launch_decode(AttnParams& p, cudaStream_t st) {
-  if constexpr (Shape<D, MODE, false>::U == 2) {
+int launch_decode(AttnParams& p, int64_t most, cudaStream_t st) {
+  if constexpr (Shape<D, MODE, false>::kCtas == 2) {
     // No more units than SMs: nothing to overlap the joins with, and a short unit is done in fewer
-    // rounds by 12 warps (one request of 777 tokens 13.0 -> 12.2 us, one of 524288 156 -> 149 us).
-    if ((int64_t)p.n * p.hkv <= sm_count()) return launch_shape<D, MODE, true>(p, st);
+    // rounds by all warps (one request of 777 tokens 13.0 -> 12.2 us, one of 524288 156 -> 149 us; D =
+    // 256, 32 heads on 8: 17 query tokens over 4000 keys 50 -> 35 us). With more it is the other way
+    // round: D = 256, a prompt of 1000 tokens 412 -> 314 us, 8 of 180 tokens 323 -> 203 us.
+    constexpr int R = mode_rows(MODE);
+    if (std::min(p.n_tokens * p.grp / R + p.n, (most + R - 1) / R * p.n) * p.hkv <= sm_count()) return launch_shape<D, MODE, true>(p, st);
   }
   return launch_shape<D, MODE, false>(p, st);
 }
 
 template <int D>
-int launch_mode(AttnParams& p, int rows, cudaStream_t st) {
+int launch_mode(AttnParams& p, int64_t most, cudaStream_t st) {  // most: rows of a request
   const bool lo = p.dtype == SS_F16;
-  if (rows <= 4) return launch_decode<D, kRows4>(p, st);
-  if (rows <= 8 || D == 256) return lo ? launch_decode<D, kRows8Lo>(p, st) : launch_decode<D, kRows8>(p, st);
-  if constexpr (D != 256) return lo ? launch_decode<D, kRows16Lo>(p, st) : launch_decode<D, kRows16>(p, st);
+  if (most <= 4) return launch_decode<D, kRows4>(p, most, st);
+  // D = 256: 16 rows spill (a prompt of 1000 tokens 427 us where 8 took 412, 17 query tokens 63 and 35)
+  if (most <= 8 || D == 256) return lo ? launch_decode<D, kRows8Lo>(p, most, st) : launch_decode<D, kRows8>(p, most, st);
+  if constexpr (D != 256) return lo ? launch_decode<D, kRows16Lo>(p, most, st) : launch_decode<D, kRows16>(p, most, st);
   return SS_OK;
 }
 
@@ -842,7 +846,6 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.parts = reinterpret_cast<float*>(p.ws + 2 * attn_counter_bytes(ctas));
     p.tile_parts = reinterpret_cast<float*>(p.ws + 2 * attn_counter_bytes(ctas) + attn_part_bytes(a->d, ctas));
     const int64_t most = (int64_t)a->max_q * p.grp;
-    const int rows = most > 16 ? 16 : (int)most;
     p.tiles = most > 16 && a->d != 256;
     // The host does not know the lengths: a request's rows over 128, and one more for each request
     // with enough rows, or max_q's tiles for each. The hint may be wrong: it chooses a variant.
@@ -855,7 +858,7 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     if (p.tiles) {
       if (int rc = launch_tiles(p, a->d, st)) return rc;
     }
-    return a->d == 64 ? launch_mode<64>(p, rows, st) : a->d == 128 ? launch_mode<128>(p, rows, st) : launch_mode<256>(p, rows, st);
+    return a->d == 64 ? launch_mode<64>(p, most, st) : a->d == 128 ? launch_mode<128>(p, most, st) : launch_mode<256>(p, most, st);
   });
 }
 

@@ -394,6 +394,19 @@ def test_attention_scales_of_tiny_and_large_values(ss):
             assert ((o.double() - want).abs() <= 2.0 ** -11 * want.abs() + (4 * 2.0 ** -11 + 2 * dz) * pv + 2.0 ** -24).all()
 
 
+def test_attention_wide_heads_with_few_and_many_units(ss):
+    # 256 dims: units of 8 rows, one or two CTAs on an SM, and in turn on one workspace
+    cases = []
+    for i, (old, new, hkv, grp, window) in enumerate([([2000], [5], 8, 4, 0), ([0, 30, 200], [150, 90, 1], 8, 4, 0),
+                                                      ([900] * 40, [1] * 40, 8, 2, 300), ([4000], [1], 4, 8, 0)]):
+        for dtype in (torch.float16, torch.bfloat16):
+            cases.append((_setup(ss, old, new, hkv, 256, 32, 40 + i, dtype, grp, pad=2), old, new, window))
+    for _ in range(2):
+        for (pool, table, lens, cu, q, kv), old, new, window in cases:
+            o, lse = ss.int4_attention(q, pool, table, lens, cu, 0.06, max_q=max(new), window=window, return_lse=True)
+            _check(o, lse, q, kv, old, new, 0.06, True, window)
+
+
 def test_attention_launches_of_every_shape_share_a_workspace(ss):
     """Units cut into parts, by launches with one and two CTAs on an SM and
     units of 4, 8 and 16 rows, in turn on one stream: every one finds its
