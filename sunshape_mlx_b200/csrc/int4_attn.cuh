@@ -45,11 +45,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Rows (query tokens times heads of a group) from which a request's queries go to the tiles of
 // 128 rows of the tcgen05 kernel instead of the 16-row units of the warp-MMA kernel. A tile is one
 // CTA's work, or a few CTAs' where there are few tiles; the units of a request are spread over all
-// SMs, but read and decode the keys once per 16 rows. The tiles win once about nine full tiles run
-// at once, whatever the keys, and from 48 rows where rows times heads times keys reach 2^21 (8 kv
-// heads, 128 dims, units against tiles: 68 rows over 4017 keys 37 and 35 us, over 517 keys 18 and 28;
-// 128 rows over 30000 keys 125 and 65; 8 requests of 36 rows over 4009 keys 69 and 68, 8 of 128
-// rows over 4032 152 and 52).
+// SMs, but read and decode the keys once per 16 rows. The tiles win from about nine full tiles on,
+// whatever the keys, and from 48 rows where rows times heads times keys reach 2^21 (8 kv heads of 128
+// dims, groups of 4, units against tiles: 32 prompts of 40 tokens 139 and 49 us, though one alone 17
+// and 21; 68 rows over 4017 keys 37 and 35 us, over 517 keys 18 and 28; 128 rows over 30000 keys 125
+// and 65; 8 requests of 36 rows over 4009 keys 69 and 68, 8 of 128 rows over 4032 152 and 52). The
+// rule is a request's own: how many others there are is not known where it is asked.
 constexpr float kTilesFrom = 1152.f, kTileRowsFrom = 48.f, kTileWorkFrom = 0x1p21f;
 
 __device__ __forceinline__ bool to_tiles(const AttnParams& p, int nq, int len) {
