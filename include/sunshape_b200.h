@@ -43,6 +43,8 @@ int ss_abi_version(void);
 const char* ss_last_error(void);
 /* Number of SMs of the current device (used to size persistent grids). */
 int ss_device_sm_count(void);
+/* *id: which CUDA-graph capture the stream is in, 0 if none. */
+int ss_stream_capture_id(void* stream, unsigned long long* id);
 
 /* Dispatch counters (reference: kernels.py:33-47 _KERNEL_STATS). Names are
  * the C entry points; counting is always on and costs one host increment. */
@@ -453,17 +455,20 @@ typedef struct ss_int4_attn_args {
   int causal, window;
   void* out;                      /* (n_tokens, hq, d) dense, 16-byte aligned */
   float* lse;                     /* (n_tokens, hq) natural logarithm, or NULL */
-  void* workspace;                /* ss_int4_attention_workspace(d) bytes, zeroed once */
+  void* workspace;                /* ss_int4_attention_workspace(d) bytes, counters zeroed once */
   size_t workspace_bytes;
   int64_t wait_limit_ns;          /* bound of the tile kernel's waits (<= 0: 2 s) */
   int64_t test_skip_tile;         /* test hook (> 0): tile test_skip_tile - 1 of every CTA of the
                                      tile kernel waits for keys that never come */
 } ss_int4_attn_args;
 
-/* Bytes of scratch on the current device. The caller zeroes it once and keeps
- * it: every launch leaves its counters at zero. Launches that may overlap on
- * the GPU must not share it. */
+/* Bytes of scratch on the current device. The caller zeroes its first
+ * ss_int4_attention_counters() bytes once and keeps it: every launch leaves
+ * its counters at zero. Launches that may overlap on the GPU must not share
+ * it; those of a CUDA graph need one of the graph's own, or replays must be
+ * in order with all that uses it. */
 size_t ss_int4_attention_workspace(int d);
+size_t ss_int4_attention_counters(void);
 int ss_int4_attention(const ss_int4_attn_args* a, void* stream);
 
 /* Log probability of targets[r] (int64; < 0: 0, >= vocab: NaN; NULL: all 0),

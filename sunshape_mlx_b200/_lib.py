@@ -117,6 +117,7 @@ _SIGS = {
     "ss_abi_version": ([], i32),
     "ss_last_error": ([], C.c_char_p),
     "ss_device_sm_count": ([], i32),
+    "ss_stream_capture_id": ([vp, C.POINTER(C.c_ulonglong)], i32),
     "ss_kernel_stats": ([C.c_char_p, C.c_size_t], i32),
     "ss_reset_kernel_stats": ([], None),
     "ss_vq_assign": ([vp, i32, i64, i64, i64, i64, i32, vp, vp, i32, i32, vp, vp, i64, i64,
@@ -156,6 +157,7 @@ _SIGS = {
                         i32, vp], i32),
     "ss_int4_fetch": ([vp, i64, i32, i32, vp, i64, i64, i64, i32, vp, vp, i32, vp], i32),
     "ss_int4_attention_workspace": ([i32], C.c_size_t),
+    "ss_int4_attention_counters": ([], C.c_size_t),
     "ss_int4_attention": ([C.POINTER(Int4AttnArgs), vp], i32),
     "ss_token_logprobs": ([vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp, vp], i32),
 }
@@ -266,6 +268,7 @@ def stream_ptr(device: torch.device | None = None):
 _FNS: dict = {}
 current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else None
 
 
 _fast = None

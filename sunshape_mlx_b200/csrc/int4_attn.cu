@@ -805,6 +805,8 @@ extern "C" {
 
 size_t ss_int4_attention_workspace(int d) { return attn_ws_bytes(d, sm_count()); }
 
+size_t ss_int4_attention_counters(void) { return 2 * attn_counter_bytes(sm_count()); }
+
 int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
   return c_entry([&]() -> int {
     SS_REQUIRE(a, "ss_int4_attention: null pointer");

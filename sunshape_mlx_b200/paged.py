@@ -268,17 +268,38 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
 
 # The kernels' scratch belongs to a stream: (device, stream, head_dim) -> workspace.
 _WS: dict[tuple, torch.Tensor] = {}
+# That of captured calls to their graph, which may run on any stream and at any time: the same
+# key -> (capture, workspace) of the last capture.
+_GRAPH_WS: dict[tuple, tuple] = {}
 
 
 def _workspace(pages: torch.Tensor, head_dim: int) -> torch.Tensor:
     index = pages.get_device()
+    if L.current_device() != index:
+        with torch.cuda.device(index):
+            return _workspace(pages, head_dim)
     key = (index, L.raw_stream(index), head_dim)
+    if L.capturing():
+        return _graph_workspace(pages.device, key)
     ws = _WS.get(key)
     if ws is None:
-        with torch.cuda.device(index):
-            ws = workspace_for(pages.device, L.entry("ss_int4_attention_workspace")(head_dim), f"int4-{head_dim}")
+        ws = workspace_for(pages.device, L.entry("ss_int4_attention_workspace")(head_dim), f"int4-{head_dim}")
         _WS[key] = ws
     return ws
+
+
+def _graph_workspace(device: torch.device, key: tuple) -> torch.Tensor:
+    """Scratch of the calls that one capture has on this stream, in the graph's own
+    memory, its counters cleared by the graph before the first of them."""
+    now = C.c_ulonglong()
+    L.call("ss_stream_capture_id", key[1], C.byref(now))
+    held = _GRAPH_WS.get(key)
+    if held is None or held[0] != now.value:
+        ws = torch.empty(L.entry("ss_int4_attention_workspace")(key[2]), dtype=torch.uint8, device=device)
+        ws[:L.entry("ss_int4_attention_counters")()].zero_()
+        # kept while the capture goes on; afterwards the graph's memory stays the graph's
+        held = _GRAPH_WS[key] = now.value, ws
+    return held[1]
 
 
 # ------------------------------------------------------------------ a server's state

@@ -62,3 +62,91 @@ def test_attention_one_key_above_a_long_context(ss, n_req, nq, grp, d, keys, dty
     sums = keys / 4 * 2.0 ** -24
     assert ((o.double() - want).abs() <= u_out * want.abs() + (4 * u + sums) * pv + keys * 2.0 ** -37 * vr.abs().max()).all()
     assert ((lse.double() - wl).abs() <= sums + 1e-5 * (1 + wl.abs())).all()
+
+
+# ------------------------------------------------------------------ launches inside graphs
+
+def _batch(ss, old, new, d, grp, seed, dtype=torch.bfloat16):
+    lens = [a + b for a, b in zip(old, new)]
+    need = [-(-x // 64) for x in lens]
+    k = torch.randn((sum(need) * 64, 8, d), generator=_gen(seed), device="cuda")
+    v = torch.randn((sum(need) * 64, 8, d), generator=_gen(seed + 1), device="cuda")
+    pool, row = _filled(ss, k, v)
+    table = torch.full((len(old), max(need)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, x in enumerate(need):
+        table[b, :x] = row[at:at + x]
+        at += x
+    cu = [0]
+    for x in new:
+        cu.append(cu[-1] + x)
+    q = torch.randn((cu[-1], 8 * grp, d), generator=_gen(seed + 2), device="cuda").to(dtype)
+    return (q, pool, table, _i32(lens), _i32(cu), 0.09), max(new)
+
+
+def _stale_memory(pool, stream, nbytes):
+    """Leaves nbytes of ones in the free memory that a graph pool has for a stream."""
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, pool=pool, stream=stream):
+        x = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")
+    g.replay()
+    torch.cuda.synchronize()
+    del x
+    return g
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_captured_without_a_call_before(ss, d):
+    """Two graphs whose first call is the captured one, replayed in the other
+    order, in memory that held something else: units are cut into parts, so
+    every output waits on counters that must start at zero."""
+    decode, m1 = _batch(ss, [3000, 9000], [1, 1], d, 4, 1)
+    mixed, m2 = _batch(ss, [3000, 20, 4000], [1, 300, 40], d, 4, 2)  # both kernels, one launch beside the other
+    want = [ss.int4_attention(*decode, max_q=m1), ss.int4_attention(*mixed, max_q=m2)]
+    mem = torch.cuda.graph_pool_handle()
+    stream = torch.cuda.Stream()  # no call ran on it
+    keep = _stale_memory(mem, stream, 128 << 20)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, pool=mem, stream=stream):
+        a = [ss.int4_attention(*decode, max_q=m1), ss.int4_attention(*mixed, max_q=m2)]
+    with torch.cuda.graph(second, pool=mem, stream=stream):
+        b = [ss.int4_attention(*mixed, max_q=m2), ss.int4_attention(*decode, max_q=m1)]
+    second.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(b[0], want[1]) and torch.equal(b[1], want[0])
+    for _ in range(2):
+        first.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a[0], want[0]) and torch.equal(a[1], want[1])
+    # a call on that stream, outside any graph, before and after
+    with torch.cuda.stream(stream):
+        c = ss.int4_attention(*decode, max_q=m1)
+    stream.synchronize()
+    assert torch.equal(c, want[0])
+    del keep
+
+
+def test_attention_graphs_of_one_stream_replayed_side_by_side(ss):
+    """Graphs captured on one stream, and calls on it, may run at the same time: each has counters of its own."""
+    calls = [_batch(ss, [20000, 9000], [1, 1], 128, 4, 3), _batch(ss, [3000, 20, 4000], [1, 300, 40], 128, 4, 4)]
+    want = [ss.int4_attention(*x, max_q=m) for x, m in calls]
+    s = torch.cuda.Stream()
+    graphs, outs = [], []
+    for x, m in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(ss.int4_attention(*x, max_q=m))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(30):
+        for o in outs:
+            o.fill_(math.nan)
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+                g.replay()
+        with torch.cuda.stream(s):
+            eager = ss.int4_attention(*calls[0][0], max_q=1)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[0])
