@@ -153,7 +153,9 @@ __device__ __forceinline__ void quantise16(const float (&x)[16], uint32_t (&w)[2
   lo = min3_nan(lo, lo3, lo3);
   hi = max3_nan(hi, hi3, hi3);
   const bool nan = lo != lo;
-  // the ends saturate; values beyond them go to the end codes by themselves
+  // The ends saturate. Values below go to code 0 by themselves (z = -2^15 then); values above do not
+  // always go to the code of 2^15, where z or s is rounded up: such a group is divided, see below.
+  const bool above = hi > kInt4Max;
   lo = fminf(fmaxf(lo, -kInt4Max), kInt4Max);
   hi = fminf(fmaxf(hi, -kInt4Max), kInt4Max);
   const uint16_t sh = nan ? 0x7fff : f2h(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
@@ -173,9 +175,9 @@ __device__ __forceinline__ void quantise16(const float (&x)[16], uint32_t (&w)[2
       c[i] = fmaf(q, 15.f, kMagic) - kMagic;
       off = fmaxf(off, fabsf(fmaf(q, 15.f, -c[i])));
     }
-    if (off > 0.49998f) {
+    if (off > 0.49998f || above) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], z), s)), 0.f), 15.f);
+      for (int i = 0; i < 16; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(fminf(x[i], kInt4Max), z), s)), 0.f), 15.f);
     }
 #pragma unroll
     for (int v = 0; v < 2; ++v) {  // four codes make an integer below 2^16, exact in the low bits of 2^23 + it

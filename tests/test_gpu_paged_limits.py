@@ -150,3 +150,26 @@ def test_attention_graphs_of_one_stream_replayed_side_by_side(ss):
             eager = ss.int4_attention(*calls[0][0], max_q=1)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[0])
+
+
+# ------------------------------------------------------------------ written values
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_append_groups_across_the_largest_magnitude(ss, d, dtype):
+    """Codes are those of the clamped values, also where others of the group
+    lie so near 2^15 that its zero is rounded up to it."""
+    g = _gen(d)
+    n = 500
+    near = 32768.0 - torch.rand((n, 2, d), generator=g, device="cuda") * torch.rand((n, 2, 1), generator=g, device="cuda") * 300
+    x = torch.where(torch.rand((n, 2, d), generator=g, device="cuda") < 0.1, 33000 + torch.rand((n, 2, d), generator=g, device="cuda") * 20000, near)
+    x[0, 0] = 32760.0
+    x[0, 0, 7::32] = 40000.0
+    x[1, 0, 3::32] = math.inf
+    x[2, 0] = 65000.0
+    x[3, 0, 5::32] = -math.inf
+    k, v = x.to(dtype), (-x).to(dtype)
+    pool, slots = ss.int4_pool(-(-n // 16), 2, 16, d), torch.arange(n, device="cuda")
+    ss.int4_append(k, v, slots, pool)
+    kr, vr = ss.int4_fetch(slots, pool, d)
+    assert torch.equal(kr, R.stored(k).float()) and torch.equal(vr, R.stored(v).float())
