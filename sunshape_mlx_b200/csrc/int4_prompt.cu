@@ -17,12 +17,13 @@
 // MMA takes the thread about 75 cycles beside the other warps' work, a tile of
 // 64 tokens as long as one of 128.
 //
-// Keys enter exactly: c s is the pair of fp16 values hi = fp16(c s) and
-// lo = c s - hi (15 bits in all, so lo is exact), and q . z is one more K step
-// of 16, z as stored against the row's group sums in two fp16 terms. One
-// rounded fp16 key would move a logit by 3e-4, which rows with few keys show
-// in their log-sum-exp; the second product costs 136 / 264 of the tensor time
-// of a tile. s enters halved: 15 s can be one place above fp16's largest.
+// Keys enter as pairs of fp16 values, hi = fp16(c s) and lo = c s - hi (15 bits
+// in all, so lo is exact), and q . z is one more K step of 16, z as stored
+// against the row's group sums in two fp16 terms. One rounded fp16 key would
+// move a logit by 3e-4, which rows with few keys show in their log-sum-exp; the
+// second product costs 136 / 264 of the tensor time of a tile. Codes enter
+// halved, since 15 s can be one place above fp16's largest: exact but where c and
+// s / 2^-24 are odd and s is below 2^-13; there a key is off by 2^-24.
 // Values are fp16(c s + z), probabilities fp16, or hi + lo (a second pass of
 // P V) where the output is fp16 and the rounding would show. Row statistics
 // and both products accumulate in fp32. O in TMEM is rescaled only when a logit
@@ -690,13 +691,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
 #pragma unroll
           for (int g = 0; g < N; ++g) {
             ks[hb][g] = key ? ks[hb][g] : 0u;
-            const uint32_t s2 = hmul2(__byte_perm(ks[hb][g], 0, 0x1010), 0x38003800u);  // s / 2
+            const uint32_t s2 = __byte_perm(ks[hb][g], 0, 0x1010);
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t x = e < 2 ? kw[hb][g] : kw[hb][g] >> 8;
-              const uint32_t c = e & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x54005400u), 0x54005400u)
-                                       : hsub2(lop_or(x, 0x000f000fu, 0x64006400u), 0x64006400u);
+              const uint32_t c = e & 1 ? hsub2(lop_or(x, 0x00f000f0u, 0x50005000u), 0x50005000u)
+                                       : hsub2(lop_or(x, 0x000f000fu, 0x60006000u), 0x60006000u);  // c / 2
               hi[e] = hmul2(c, s2);
               lo[e] = hfms2(c, s2, hi[e]);
             }

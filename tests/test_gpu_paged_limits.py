@@ -173,3 +173,28 @@ def test_append_groups_across_the_largest_magnitude(ss, d, dtype):
     ss.int4_append(k, v, slots, pool)
     kr, vr = ss.int4_fetch(slots, pool, d)
     assert torch.equal(kr, R.stored(k).float()) and torch.equal(vr, R.stored(v).float())
+
+
+# ------------------------------------------------------------------ small keys
+
+@pytest.mark.parametrize("nq", [1, 60])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("steps", [1, 3, 1025])
+def test_attention_keys_of_the_smallest_scales(ss, steps, d, nq):
+    """Scales of `steps` times fp16's smallest: units of few rows take such
+    keys exactly, tiles to 2^-24 where code and scale are both odd."""
+    s = steps * 2.0 ** -24
+    t = 200
+    codes = (torch.arange(t, device="cuda") % 8 * 2)[:, None].expand(t, 32).clone().float()
+    codes[:, 0], codes[:, 1] = 0.0, 15.0
+    k = (codes * s)[:, None].repeat(1, 1, d // 32).contiguous()
+    pool, row = _filled(ss, k, torch.randn((t, 1, d), generator=_gen(1), device="cuda"))
+    kr, vr = ss.int4_fetch(torch.arange(t, device="cuda"), pool, d)
+    assert torch.equal(kr, k)
+    size = 2.0 ** 17 / steps
+    size = 2.0 ** math.floor(math.log2(size))
+    q = torch.full((nq, 32, d), size, dtype=torch.bfloat16, device="cuda")
+    o, lse = ss.int4_attention(q, pool, row[None], _i32([t]), _i32([0, nq]), 128 / d, max_q=nq, causal=False, return_lse=True)
+    _, wl, _, _ = R.attention(q, kr, vr, t, 128 / d, causal=False)
+    odd = d // 32 if nq > 1 and steps % 2 else 0
+    assert ((lse.double() - wl).abs() <= 128 / d * odd * size * 2.0 ** -24 + 1e-5 * (1 + wl.abs())).all()
