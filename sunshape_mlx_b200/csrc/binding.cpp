@@ -66,9 +66,9 @@ struct Call {
     if (ok) want(t.scalar_type() == at::kInt && t.dim() == dims && t.numel() > 0 && t.stride(dims - 1) == 1);
     return t;
   }
-  // Pages of head_dim d; returns the tokens of a page.
+  // Pages of head_dim d; returns the tokens of a page. The pool has pages and kv heads then.
   int64_t pool(const Tensor& t, int64_t d) {
-    if (!ok || !want(t.scalar_type() == at::kByte && t.dim() == 3 && t.stride(2) == 1 && t.size(0) > 0 &&
+    if (!ok || !want(t.scalar_type() == at::kByte && t.dim() == 3 && t.stride(2) == 1 && t.size(0) > 0 && t.size(1) > 0 &&
                      (d == 64 || d == 128 || d == 256)))
       return 0;
     const int64_t bytes = t.size(2);

@@ -135,6 +135,8 @@ def release_pages(seq_lens: torch.Tensor, done: torch.Tensor, block_table: torch
 def int4_pool(n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> torch.Tensor:
     """A page pool: uint8 (n_pages, n_kv_heads, page_size * head_dim * 5 / 4),
     uninitialised (bits that no token was written to are never used)."""
+    if n_pages < 1 or n_kv_heads < 1:
+        raise ValueError("n_pages and n_kv_heads must be positive")
     _page_tokens(page_size * head_dim * 5 // 4, head_dim)
     return torch.empty((n_pages, n_kv_heads, page_size * head_dim * 5 // 4), dtype=torch.uint8, device=device)
 
@@ -151,8 +153,8 @@ def _page_tokens(nbytes: int, head_dim: int) -> int:
 def _check_pool(pages: torch.Tensor, head_dim: int) -> int:
     if not pages.is_cuda:
         L.require_cuda(pages)
-    if pages.dtype is not _U8 or pages.dim() != 3 or pages.stride(2) != 1 or not pages.size(0):
-        raise ValueError("pages must be uint8 (n_pages, n_kv_heads, bytes), contiguous in the last dim")
+    if pages.dtype is not _U8 or pages.dim() != 3 or pages.stride(2) != 1 or not pages.size(0) or not pages.size(1):
+        raise ValueError("pages must be uint8 (n_pages, n_kv_heads, bytes), not empty, contiguous in the last dim")
     return _page_tokens(pages.size(2), head_dim)
 
 

@@ -198,3 +198,20 @@ def test_attention_keys_of_the_smallest_scales(ss, steps, d, nq):
     _, wl, _, _ = R.attention(q, kr, vr, t, 128 / d, causal=False)
     odd = d // 32 if nq > 1 and steps % 2 else 0
     assert ((lse.double() - wl).abs() <= 128 / d * odd * size * 2.0 ** -24 + 1e-5 * (1 + wl.abs())).all()
+
+
+# ------------------------------------------------------------------ arguments
+
+def test_pools_without_heads_are_refused(ss):
+    pool = torch.zeros((2, 0, 1280), dtype=torch.uint8, device="cuda")
+    q = torch.zeros((1, 4, 64), dtype=torch.float16, device="cuda")
+    s = torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        ss.int4_attention(q, pool, _i32([[0]]), _i32([1]), _i32([0, 1]), 1.0, max_q=1)
+    with pytest.raises(ValueError):
+        ss.int4_fetch(s, pool, 64)
+    with pytest.raises(ValueError):
+        ss.int4_append(q[:, :0].float(), q[:, :0].float(), s, pool)
+    for bad in ((0, 2, 16, 64), (2, 0, 16, 64), (2, 2, 24, 64)):
+        with pytest.raises(ValueError):
+            ss.int4_pool(*bad)
