@@ -119,7 +119,7 @@ PyObject* plan_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!c.ok) return nullptr;
     const int64_t n = lens.size(0);
     if (!c.want(q.size(0) == n && table.size(0) == n && left.size(0) == 1 && table.stride(0) >= table.size(1) && page >= 16 &&
-                page % 16 == 0 && tokens >= 0 && tokens < (1ll << 31) && n <= 16384) || !c.here())
+                page % 16 == 0 && page < (1ll << 31) && tokens >= 0 && tokens < (1ll << 31) && n <= 16384) || !c.here())
       return nullptr;
     Tensor slots = at::empty({tokens}, lens.options().dtype(at::kLong));
     Tensor out = at::empty({2 * n + 3 + 2 * tokens}, lens.options());

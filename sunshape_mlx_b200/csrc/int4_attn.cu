@@ -841,7 +841,10 @@ int ss_int4_attention(const ss_int4_attn_args* a, void* stream) {
     p.page_inv = p.page_blocks == 1 ? 0u : (uint32_t)(((1ull << 32) + p.page_blocks - 1) / p.page_blocks);
     p.table = a->block_table; p.table_stride = a->table_stride; p.width = a->width;
     p.seq_lens = a->seq_lens; p.cu_q = a->cu_q; p.n = a->n_requests;
-    p.scale = a->scale; p.causal = a->causal; p.window = a->window;
+    // A window that no position exceeds hides nothing; without it, differences of positions and
+    // windows stay far inside 32 bits (positions go down to minus the query tokens).
+    const bool windowed = a->window > 0 && (int64_t)a->window < (int64_t)a->width * a->page_size;
+    p.scale = a->scale; p.causal = a->causal; p.window = windowed ? a->window : 0;
     p.out = a->out; p.lse = a->lse;
     p.ws = static_cast<uint8_t*>(a->workspace);
     p.tile_ws = reinterpret_cast<uint32_t*>(p.ws + attn_counter_bytes(ctas));

@@ -40,8 +40,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
         return TokenLogprobs._make(t)
     if not (logits.is_cuda and targets.is_cuda):
         L.require_cuda(logits, targets)
-    if logits.dim() != 2 or not logits.size(1):
-        raise ValueError("logits must be (rows, vocab)")
+    if logits.dim() != 2 or not 0 < logits.size(1) < 2 ** 31:
+        raise ValueError("logits must be (rows, vocab), vocab from 1 to 2^31 - 1")
     n, vocab = logits.shape
     row_stride, stride = logits.stride()
     if stride != 1 and vocab > 1:

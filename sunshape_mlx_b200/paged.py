@@ -29,6 +29,7 @@ __all__ = ["StepPlan", "plan_step", "release_pages", "int4_append", "int4_fetch"
            "int4_attention", "int4_pool", "PageTables", "Int4PagedKVCache"]
 
 _HEAD_DIMS = (64, 128, 256)
+_INT_MAX = 2 ** 31 - 1  # of the C interface's sizes
 _STATUS = {1: "the page pool has too few free pages", 2: "a request needs more pages than its table row holds",
            4: "the new tokens exceed n_tokens", 8: "more pages were released than the pool has out"}
 
@@ -72,8 +73,8 @@ def _check_tables(seq_lens, block_table, free_pages, n_free, page_size) -> int:
         raise ValueError("block_table needs a row per request, n_free one element")
     if block_table.stride(0) < block_table.size(1):
         raise ValueError("the rows of block_table must not overlap")
-    if page_size < 16 or page_size % 16:
-        raise ValueError(f"page_size must be a multiple of 16, got {page_size}")
+    if page_size < 16 or page_size % 16 or page_size > _INT_MAX:
+        raise ValueError(f"page_size must be a multiple of 16 below 2^31, got {page_size}")
     return index
 
 
@@ -262,7 +263,7 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
                            queries.stride(1), n, hq, hkv, d, pages.data_ptr(), pages.size(0),
                            pages.stride(0), pages.stride(1), page, block_table.data_ptr(),
                            block_table.stride(0), block_table.size(1), seq_lens.data_ptr(),
-                           cu_q.data_ptr(), b, max_q, scale, 1 if causal else 0, window,
+                           cu_q.data_ptr(), b, min(max_q, _INT_MAX), scale, 1 if causal else 0, min(window, _INT_MAX),
                            out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel())
         L.launch("ss_int4_attention", index, C.byref(a))
     return (out, lse) if return_lse else out
@@ -314,8 +315,8 @@ class PageTables:
     def __init__(self, n_pages: int, page_size: int, max_requests: int, max_pages: int, device="cuda"):
         if n_pages < 1 or max_requests < 1 or max_pages < 1:
             raise ValueError("n_pages, max_requests and max_pages must be positive")
-        if page_size < 16 or page_size % 16:
-            raise ValueError(f"page_size must be a multiple of 16, got {page_size}")
+        if page_size < 16 or page_size % 16 or page_size > _INT_MAX:
+            raise ValueError(f"page_size must be a multiple of 16 below 2^31, got {page_size}")
         self.n_pages, self.page_size = n_pages, page_size
         self.device = torch.device(device)
         self.block_table = torch.full((max_requests, max_pages), -1, dtype=torch.int32, device=self.device)

@@ -215,3 +215,30 @@ def test_pools_without_heads_are_refused(ss):
     for bad in ((0, 2, 16, 64), (2, 0, 16, 64), (2, 2, 24, 64)):
         with pytest.raises(ValueError):
             ss.int4_pool(*bad)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("old,new,seen", [(100, 1, 101), (0, 300, 300), (0, 300, 40), (0, 8, 3)])
+def test_attention_windows_past_every_key_hide_nothing(ss, old, new, seen, causal):
+    """Also where requests have more query rows than keys, and for numbers that no 32 bits hold."""
+    k = torch.randn((old + new, 2, 64), generator=_gen(1), device="cuda")
+    pool, row = _filled(ss, k, torch.randn_like(k))
+    q = torch.randn((new, 8, 64), generator=_gen(2), device="cuda").half()
+    args = q, pool, row[None], _i32([seen]), _i32([0, new]), 0.1
+    want = ss.int4_attention(*args, max_q=new, causal=causal)
+    ref = R.attention(q, *ss.int4_fetch(torch.arange(old + new, device="cuda"), pool, 64), seen, 0.1, causal)[0]
+    assert (want.double() - ref).abs().max() < 4e-3 * (1 + ref.abs().max())
+    for window in (seen, 10 ** 6, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5):
+        assert torch.equal(ss.int4_attention(*args, max_q=new, causal=causal, window=window), want)
+    assert torch.equal(ss.int4_attention(*args, max_q=2 ** 32 + 1, causal=causal), ss.int4_attention(*args, max_q=2 ** 31 - 1, causal=causal))
+
+
+def test_sizes_past_32_bits_are_refused(ss):
+    i = _i32([1])
+    with pytest.raises(ValueError, match="page_size"):
+        ss.plan_step(i, i, i[None], i, i, page_size=2 ** 32 + 16, n_tokens=1)
+    with pytest.raises(ValueError, match="page_size"):
+        ss.release_pages(i, i.bool(), i[None], i, i, page_size=2 ** 32 + 16)
+    x = torch.empty((1, 2 ** 31 + 8), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="vocab"):
+        ss.token_logprobs(x, torch.zeros(1, dtype=torch.int64, device="cuda"))
