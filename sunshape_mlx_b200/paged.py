@@ -56,7 +56,7 @@ _I32, _I64, _U8 = torch.int32, torch.int64, torch.uint8
 
 
 def _int32(name: str, t: torch.Tensor, dims: int, index: int) -> None:
-    if t.dtype is not _I32 or t.dim() != dims or t.get_device() != index or (t.stride(-1) != 1 and t.numel()):
+    if t.dtype is not _I32 or t.dim() != dims or t.get_device() != index or (t.size(-1) > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name} must be a contiguous {dims}-D int32 tensor on CUDA device {index}")
 
 
@@ -71,11 +71,15 @@ def _check_tables(seq_lens, block_table, free_pages, n_free, page_size) -> int:
     _int32("n_free", n_free, 1, index)
     if block_table.size(0) != seq_lens.size(0) or n_free.size(0) != 1:
         raise ValueError("block_table needs a row per request, n_free one element")
-    if block_table.stride(0) < block_table.size(1):
+    if block_table.size(0) > 1 and block_table.stride(0) < block_table.size(1):
         raise ValueError("the rows of block_table must not overlap")
     if page_size < 16 or page_size % 16 or page_size > _INT_MAX:
         raise ValueError(f"page_size must be a multiple of 16 below 2^31, got {page_size}")
     return index
+
+
+def _row_stride(table: torch.Tensor) -> int:
+    return max(table.stride(0), table.size(1))  # a single row has any stride
 
 
 def plan_step(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_table: torch.Tensor,
@@ -109,7 +113,7 @@ def plan_step(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_table: torch.T
     at_req = at_pos + 4 * n_tokens
     at_lens = at_req + 4 * n_tokens
     L.launch("ss_plan_step", index, seq_lens.data_ptr(), q_lens.data_ptr(), n, block_table.data_ptr(),
-             block_table.stride(0), block_table.size(1), free_pages.data_ptr(), free_pages.size(0),
+             _row_stride(block_table), block_table.size(1), free_pages.data_ptr(), free_pages.size(0),
              n_free.data_ptr(), page_size, n_tokens, at, at_pos, at_req, slots.data_ptr(), at_lens,
              at_lens + 4 * n, at_lens + 4 * n + 4)
     return StepPlan(cu, pos, req, slots, lens, left, status)
@@ -126,7 +130,7 @@ def release_pages(seq_lens: torch.Tensor, done: torch.Tensor, block_table: torch
         raise ValueError("done must be a contiguous bool tensor with one element per request")
     lens, left, status = torch.empty(n + 2, dtype=_I32, device=seq_lens.device).split_with_sizes((n, 1, 1))
     L.launch("ss_release_pages", index, seq_lens.data_ptr(), done.data_ptr(), n, block_table.data_ptr(),
-             block_table.stride(0), block_table.size(1), free_pages.data_ptr(), free_pages.size(0),
+             _row_stride(block_table), block_table.size(1), free_pages.data_ptr(), free_pages.size(0),
              n_free.data_ptr(), page_size, lens.data_ptr(), left.data_ptr(), status.data_ptr())
     return lens, left, status
 

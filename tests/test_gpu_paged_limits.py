@@ -242,3 +242,19 @@ def test_sizes_past_32_bits_are_refused(ss):
     x = torch.empty((1, 2 ** 31 + 8), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError, match="vocab"):
         ss.token_logprobs(x, torch.zeros(1, dtype=torch.int64, device="cuda"))
+
+
+def test_single_elements_of_any_stride(ss):
+    """A dimension of one element is contiguous whatever its stride says."""
+    wide = lambda x: torch.stack([_i32(x)] * 3, -1)[..., 0]  # noqa: E731  stride 3
+    k = torch.randn((20, 2, 64), generator=_gen(1), device="cuda")
+    pool, _ = _filled(ss, k, k)
+    q = torch.randn((1, 4, 64), generator=_gen(2), device="cuda").half()
+    want = ss.int4_attention(q, pool, _i32([[0]]), _i32([20]), _i32([0, 1]), 0.1, max_q=1)
+    table = torch.zeros((1, 3), dtype=torch.int32, device="cuda")[:, ::3]
+    assert torch.equal(ss.int4_attention(q, pool, table, wide([20]), _i32([0, 1]), 0.1, max_q=1), want)
+    p = ss.plan_step(wide([5]), wide([2]), torch.as_strided(_i32([7]), (1, 1), (0, 9)), _i32(range(8)), wide([1]), page_size=16, n_tokens=2)
+    assert p.status.item() == 0 and p.slots.tolist() == [7 * 16 + 5, 7 * 16 + 6]
+    lens, left, status = ss.release_pages(wide([5]), torch.tensor([True], device="cuda"), torch.as_strided(_i32([1]), (1, 1), (0, 9)), _i32([0, 0]), wide([1]),
+                                          page_size=16)
+    assert (lens.item(), left.item(), status.item()) == (0, 2, 0)
