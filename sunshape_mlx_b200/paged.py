@@ -231,7 +231,7 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     row that sees no key gives 0 and -inf, as does a token outside ``cu_q``.
     """
     L.poll_device_errors()
-    if queries.is_cuda and pages.is_cuda and queries.dim() == 3:
+    if queries.is_cuda and pages.is_cuda and queries.dim() == 3 and queries.size(2) in _HEAD_DIMS:
         t = (L._fast or L.fast()).attention(queries, pages, block_table, seq_lens, cu_q, scale, max_q, causal, window, return_lse,
                                             _workspace(pages, queries.size(2)))
         if t is not None:

@@ -258,3 +258,13 @@ def test_single_elements_of_any_stride(ss):
     lens, left, status = ss.release_pages(wide([5]), torch.tensor([True], device="cuda"), torch.as_strided(_i32([1]), (1, 1), (0, 9)), _i32([0, 0]), wide([1]),
                                           page_size=16)
     assert (lens.item(), left.item(), status.item()) == (0, 2, 0)
+
+
+def test_refused_head_dims_leave_no_memory_behind(ss):
+    pool = ss.int4_pool(2, 2, 16, 64)
+    q = torch.zeros((1, 4, 100_000), dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError):
+        ss.int4_attention(q, pool, _i32([[0]]), _i32([1]), _i32([0, 1]), 1.0, max_q=1)
+    assert torch.cuda.memory_allocated() - before < 1 << 20
