@@ -306,6 +306,12 @@ def launch(fn: str, index: int, *args) -> None:
         raise SunShapeCudaError(fn, rc, last_error())
 
 
+def refuse_graph(what: str, t: torch.Tensor) -> None:
+    """Raises where `t` wants a gradient that the operator `what` does not have."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or detach its input")
+
+
 def dtype_code(dt: torch.dtype) -> int:
     try:
         return _DTYPE_CODE[dt]

@@ -10,6 +10,7 @@
 // its own way, which raises the error that belongs to the case.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -35,6 +36,10 @@ struct Call {
     if (device < 0) device = t.get_device();
     want(t.get_device() == device);
     return t;
+  }
+  // An input of which a result would have to keep the graph: the wrapper refuses it.
+  void no_graph(const Tensor& t) {
+    if (ok) want(!(t.requires_grad() && at::GradMode::is_enabled()));
   }
   int64_t integer(int i) {
     if (!want(PyLong_Check(args[i]))) return 0;
@@ -179,6 +184,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const double scale = c.number(5);
     const int64_t max_q = c.integer(6), window = c.integer(8);
     const bool causal = c.truth(7), with_lse = c.truth(9);
+    c.no_graph(q);
     if (!c.ok || !c.want(q.dim() == 3 && q.size(0) > 0)) return nullptr;
     const int64_t n = q.size(0), hq = q.size(1), d = q.size(2), page = c.pool(pages, d), b = lens.size(0);
     if (!c.want(page > 0 && (q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16) && hq >= 1 && hq % pages.size(1) == 0 &&
@@ -207,6 +213,7 @@ PyObject* logprobs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return lane(args, nargs, 3, [](Call& c) -> PyObject* {
     const Tensor &x = c.tensor(0), &t = c.tensor(1);
     const int64_t k = c.integer(2);
+    c.no_graph(x);
     if (!c.ok || !c.want(x.dim() == 2 && x.size(0) > 0 && x.size(1) > 0 && x.size(1) < (1ll << 31))) return nullptr;
     const int64_t n = x.size(0), vocab = x.size(1);
     const int dt = code_of(x.scalar_type());

@@ -33,13 +33,15 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     NaN. ``top_k`` <= 32 alternatives by value, equal ones by index; -1 and
     -inf past the vocabulary. Logits of -inf are impossible tokens; a row of
     nothing else gives -inf and entropy 0. A row with NaN or +inf gives NaN
-    everywhere and ids of -1.
+    everywhere and ids of -1. There is no gradient: logits that want one are
+    refused.
     """
     t = (L._fast or L.fast()).logprobs(logits, targets, top_k)
     if t is not None:
         return TokenLogprobs._make(t)
     if not (logits.is_cuda and targets.is_cuda):
         L.require_cuda(logits, targets)
+    L.refuse_graph("token_logprobs", logits)
     if logits.dim() != 2 or not 0 < logits.size(1) < 2 ** 31:
         raise ValueError("logits must be (rows, vocab), vocab from 1 to 2^31 - 1")
     n, vocab = logits.shape

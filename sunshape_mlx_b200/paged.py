@@ -229,6 +229,7 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     (n_tokens, n_q_heads, head_dim) in the queries' dtype and, with
     ``return_lse``, the natural log-sum-exp (n_tokens, n_q_heads) in fp32. A
     row that sees no key gives 0 and -inf, as does a token outside ``cu_q``.
+    There is no gradient: queries that want one are refused.
     """
     L.poll_device_errors()
     if queries.is_cuda and pages.is_cuda and queries.dim() == 3 and queries.size(2) in _HEAD_DIMS:
@@ -238,6 +239,7 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
             return t if return_lse else t[0]
     if not queries.is_cuda:
         L.require_cuda(queries)
+    L.refuse_graph("int4_attention", queries)
     if queries.dim() != 3:
         raise ValueError("queries must be (n_tokens, n_q_heads, head_dim)")
     n, hq, d = queries.shape

@@ -268,3 +268,19 @@ def test_refused_head_dims_leave_no_memory_behind(ss):
     with pytest.raises(ValueError):
         ss.int4_attention(q, pool, _i32([[0]]), _i32([1]), _i32([0, 1]), 1.0, max_q=1)
     assert torch.cuda.memory_allocated() - before < 1 << 20
+
+
+def test_inputs_that_want_gradients_are_refused(ss):
+    k = torch.randn((20, 2, 64), generator=_gen(1), device="cuda")
+    pool, row = _filled(ss, k, k)
+    q = torch.randn((1, 4, 64), generator=_gen(2), device="cuda").half().requires_grad_()
+    args = pool, row[None], _i32([20]), _i32([0, 1]), 0.1
+    x = torch.randn((3, 50), generator=_gen(3), device="cuda").requires_grad_()
+    t = torch.zeros(3, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="gradient"):
+        ss.int4_attention(q, *args, max_q=1)
+    with pytest.raises(ValueError, match="gradient"):
+        ss.token_logprobs(x, t)
+    with torch.no_grad():
+        assert torch.equal(ss.int4_attention(q, *args, max_q=1), ss.int4_attention(q.detach(), *args, max_q=1))
+        assert torch.equal(ss.token_logprobs(x, t).logprobs, ss.token_logprobs(x.detach(), t).logprobs)
