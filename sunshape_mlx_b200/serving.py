@@ -105,8 +105,8 @@ class PagedServer:
         return forward_paged(self.model, ids, plan, self.caches, max_q=max(new.values()), rows=rows)
 
     def start(self, prompts: list[torch.Tensor]) -> tuple[list[int], list[TokenLogprobs]]:
-        """Takes prompts (1-D id tensors of at least one token) in and runs
-        them. Returns their request numbers and, per prompt, the log
+        """Takes prompts (1-D tensors of at least one id of the vocabulary) in
+        and runs them. Returns their request numbers and, per prompt, the log
         probabilities of its tokens after the first (entropy and alternatives
         are those of the position before each)."""
         dev = self.model.device
@@ -115,6 +115,9 @@ class PagedServer:
             raise RuntimeError(f"{len(prompts)} prompts for {len(free)} free rows")
         if any(p.dim() != 1 or not p.numel() for p in prompts):
             raise ValueError("prompts must be 1-D and hold a token at least")
+        vocab = self.model.cfg.vocab
+        if any(int(p.min()) < 0 or int(p.max()) >= vocab for p in prompts):  # no kernel looks at them before the embedding
+            raise ValueError(f"prompts must hold ids from 0 to {vocab - 1}")
         reqs = free[: len(prompts)]
         prompts = [p.to(dev, torch.int64) for p in prompts]
         for r in reqs:

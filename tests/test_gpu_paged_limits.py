@@ -284,3 +284,18 @@ def test_inputs_that_want_gradients_are_refused(ss):
     with torch.no_grad():
         assert torch.equal(ss.int4_attention(q, *args, max_q=1), ss.int4_attention(q.detach(), *args, max_q=1))
         assert torch.equal(ss.token_logprobs(x, t).logprobs, ss.token_logprobs(x.detach(), t).logprobs)
+
+
+def test_server_refuses_ids_outside_the_vocabulary(ss):
+    from sunshape_mlx_b200.harness import Decoder, DecoderConfig
+    from sunshape_mlx_b200.serving import PagedServer
+
+    model = Decoder(DecoderConfig(n_layers=1, hidden=128, n_heads=2, n_kv_heads=1, ffn=128, vocab=97), seed=1)
+    server = PagedServer(model, n_pages=4, page_size=16, max_requests=2, max_tokens=32)
+    fine = torch.arange(5)
+    for bad in (torch.tensor([3, 97]), torch.tensor([-1, 4]), torch.tensor([3, 97], device="cuda"), torch.tensor([2 ** 40])):
+        with pytest.raises(ValueError, match="ids from 0 to 96"):
+            server.start([fine, bad])
+        assert not server.lens and server.tables.n_free.item() == 4
+    reqs, _ = server.start([fine, torch.tensor([0, 96], device="cuda")])
+    assert reqs == [0, 1]
