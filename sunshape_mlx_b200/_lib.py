@@ -12,6 +12,7 @@ import ctypes as C
 import importlib
 import os
 import threading
+import warnings
 
 import torch
 
@@ -274,14 +275,27 @@ capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_
 _fast = None
 
 
+class _NoFast:
+    """Stands in for the native lane where it was not built: leaves every call to its wrapper."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def fast():
     """The native lane (csrc/binding.cpp): functions that do an ordinary call's
     checks, allocations and launch, and return None where the wrapper has to
-    look closer. Built beside the library."""
+    look closer. Built beside the library; without it calls take longer on the
+    host, and their results are the same."""
     global _fast
     if _fast is None:
         load()
-        _fast = importlib.import_module("._fast", __package__)
+        try:
+            _fast = importlib.import_module("._fast", __package__)
+        except ImportError as e:
+            warnings.warn(f"the native call lane is not there ({e}): calls cost more host time. "
+                          "Build it with `python -m sunshape_mlx_b200.build`.")
+            _fast = _NoFast()
     return _fast
 
 

@@ -1,5 +1,6 @@
-"""Builds libsunshape_b200.so (all CUDA sources, sm_100a) and the native lane
-of the paged wrappers (_fast, a CPython extension over it) in place.
+"""Builds libsunshape_b200.so (all CUDA sources, sm_100a) and, where torch is
+installed, the native lane of the paged wrappers (_fast, a CPython extension
+over it) in place.
 
     python -m sunshape_mlx_b200.build          # or: python sunshape_mlx_b200/build.py
 
@@ -10,6 +11,7 @@ its source or a header is newer than it; stale objects compile in parallel.
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -46,39 +48,20 @@ def _torch_flags() -> tuple[list[str], list[str]]:
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     libs = ["torch_python", "torch", "torch_cpu", "c10", "c10_cuda"]
-    return ([f"-I{p}" for p in inc] + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
+    return ([x for p in inc for x in ("-isystem", p)] + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
             ["-L" + os.path.join(root, "lib"), *[f"-l{x}" for x in libs]])
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(FAST):
-        return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(FAST))
-    deps = sources() + [FAST_SRC] + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
-    return any(os.path.getmtime(f) > t for f in deps)
+def _have_torch() -> bool:
+    return "torch" in sys.modules or importlib.util.find_spec("torch") is not None
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not _stale():
-        return LIB
-    nvcc = _nvcc()
-    objdir = os.path.join(HERE, "_build")
-    os.makedirs(objdir, exist_ok=True)
-    headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
-    objs, cmds = [], []
-    for src in sources():
-        obj = os.path.join(objdir, os.path.basename(src)[:-3] + ".o")
-        objs.append(obj)
-        fresh = os.path.exists(obj) and all(
-            os.path.getmtime(d) <= os.path.getmtime(obj) for d in [src, *headers])
-        if force or not fresh:
-            cmds.append([nvcc, *ARCH, *FLAGS, "-I", INCLUDE, "-c", src, "-o", obj])
-    inc, link = _torch_flags()
-    fast_obj = os.path.join(objdir, "binding.o")
-    if force or not (os.path.exists(fast_obj) and all(
-            os.path.getmtime(d) <= os.path.getmtime(fast_obj) for d in [FAST_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))])):
-        cmds.append(["g++", "-O2", "-std=c++17", "-fPIC", "-w", *inc, "-c", FAST_SRC, "-o", fast_obj])
-    # objects compile independently: run them side by side
+def _fresh(target: str, deps: list[str]) -> bool:
+    return os.path.exists(target) and all(os.path.getmtime(d) <= os.path.getmtime(target) for d in deps)
+
+
+def _run(cmds: list[list[str]], verbose: bool) -> None:
+    """Runs the commands side by side."""
     procs = []
     for cmd in cmds:
         if verbose:
@@ -87,17 +70,32 @@ def build(force: bool = False, verbose: bool = False) -> str:
     failed = [c for c, pr in zip(cmds, procs) if pr.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
-    tmp = LIB + ".tmp"
-    cmd = [nvcc, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB)
-    cmd = ["g++", "-shared", "-o", FAST + ".tmp", fast_obj, "-L" + HERE, "-lsunshape_b200", *link, "-Wl,-rpath,$ORIGIN"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(FAST + ".tmp", FAST)
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Builds what is out of date: the library, then, where torch is installed, the
+    extension over it. The library needs nvcc alone."""
+    headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
+    objdir = os.path.join(HERE, "_build")
+    if force or not _fresh(LIB, [*sources(), *headers]):
+        nvcc = _nvcc()
+        os.makedirs(objdir, exist_ok=True)
+        objs, cmds = [], []
+        for src in sources():
+            obj = os.path.join(objdir, os.path.basename(src)[:-3] + ".o")
+            objs.append(obj)
+            if force or not _fresh(obj, [src, *headers]):
+                cmds.append([nvcc, *ARCH, *FLAGS, "-I", INCLUDE, "-c", src, "-o", obj])
+        _run(cmds, verbose)
+        _run([[nvcc, *ARCH, "-shared", "-o", LIB + ".tmp", *objs, "-lcudart"]], verbose)
+        os.replace(LIB + ".tmp", LIB)
+    if _have_torch() and (force or not _fresh(FAST, [FAST_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))])):
+        os.makedirs(objdir, exist_ok=True)
+        inc, link = _torch_flags()
+        obj = os.path.join(objdir, "binding.o")
+        _run([["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", *inc, "-c", FAST_SRC, "-o", obj]], verbose)
+        _run([["g++", "-shared", "-o", FAST + ".tmp", obj, "-L" + HERE, "-lsunshape_b200", *link, "-Wl,-rpath,$ORIGIN"]], verbose)
+        os.replace(FAST + ".tmp", FAST)
     return LIB
 
 

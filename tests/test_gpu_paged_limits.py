@@ -299,3 +299,25 @@ def test_server_refuses_ids_outside_the_vocabulary(ss):
         assert not server.lens and server.tables.n_free.item() == 4
     reqs, _ = server.start([fine, torch.tensor([0, 96], device="cuda")])
     assert reqs == [0, 1]
+
+
+def test_the_same_results_without_the_native_lane(ss, monkeypatch):
+    from sunshape_mlx_b200 import _lib as L
+
+    k = torch.randn((200, 2, 64), generator=_gen(1), device="cuda")
+    q = torch.randn((200, 8, 64), generator=_gen(2), device="cuda").half()
+    x = torch.randn((5, 3000), generator=_gen(3), device="cuda")
+
+    def run():
+        table, free = torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), torch.arange(20, dtype=torch.int32, device="cuda")
+        p = ss.plan_step(_i32([0, 0]), _i32([130, 70]), table, free, _i32([20]), page_size=32, n_tokens=200)
+        pool = ss.int4_pool(20, 2, 32, 64).fill_(255)
+        ss.int4_append(k, k, p.slots, pool)
+        kv = ss.int4_fetch(p.slots, pool, 64)
+        o = ss.int4_attention(q, pool, table, p.seq_lens, p.cu_q, 0.1, max_q=130, return_lse=True)
+        return [*p, table, pool, *kv, *o, *ss.token_logprobs(x, torch.arange(5, device="cuda"), top_k=4)]
+
+    want = run()
+    monkeypatch.setattr(L, "_fast", L._NoFast())
+    for a, b in zip(run(), want):
+        assert torch.equal(a, b)
