@@ -321,3 +321,79 @@ def test_the_same_results_without_the_native_lane(ss, monkeypatch):
     monkeypatch.setattr(L, "_fast", L._NoFast())
     for a, b in zip(run(), want):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ what no test reached
+
+def test_append_into_a_view_of_a_larger_pool(ss):
+    g = _gen(3)
+    k, v = torch.randn((2, 9, 3, 64), generator=g, device="cuda").half()
+    wide = torch.full((2, 5, 16 * 80 + 64), 0x5A, dtype=torch.uint8, device="cuda")
+    view, slots = wide[:, 1:4, :16 * 80], torch.arange(9, device="cuda") + 12  # of both pages
+    dense = view.clone()
+    ss.int4_append(k, v, slots, view)
+    kr, vr = ss.int4_fetch(slots, view, 64)
+    assert torch.equal(kr, R.stored(k).float()) and torch.equal(vr, R.stored(v).float())
+    ss.int4_append(k, v, slots, dense)
+    assert torch.equal(view, dense)
+    assert (wide[:, [0, 4]] == 0x5A).all() and (wide[:, :, 16 * 80:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("n,page", [(1, 16), (7, 32), (700, 16), (9000, 48)])
+def test_release_pages(ss, n, page):
+    """Against the definition: pages of ended requests on the stack in the order of the requests and of their tables."""
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 5 * page, (n,), generator=g)
+    done = torch.rand(n, generator=g) < 0.4
+    held = (lens + page - 1) // page
+    pool = int(held.sum()) + 5
+    order = torch.randperm(pool, generator=g).int()
+    table = torch.full((n, 6), -1, dtype=torch.int32)
+    at = 0
+    for b in range(n):
+        table[b, :held[b]] = order[at:at + held[b]]
+        at += int(held[b])
+    free = torch.full((pool,), -7, dtype=torch.int32)
+    free[:pool - at] = order[at:]
+    gt, gf, left = table.cuda(), free.cuda(), _i32([pool - at])
+    got_lens, got_left, status = ss.release_pages(lens.int().cuda(), done.cuda(), gt, gf, left, page_size=page)
+    stack = free[:pool - at].tolist()
+    for b in range(n):
+        if done[b]:
+            stack += table[b, :held[b]].tolist()
+            table[b, :held[b]] = -1
+    assert status.item() == 0 and got_left.item() == len(stack) and gf[:len(stack)].tolist() == stack
+    assert (gf[len(stack):].cpu() == -7).all() and torch.equal(gt.cpu(), table)
+    assert torch.equal(got_lens.cpu().long(), torch.where(done, 0, lens))
+
+
+def test_release_of_more_pages_than_are_out_changes_nothing(ss):
+    table, free = _i32([[3, 4], [5, -1]]), _i32([0, 1, 2, 9, 9, 9])
+    lens, left, status = ss.release_pages(_i32([20, 9]), torch.tensor([True, True], device="cuda"), table, free, _i32([4]), page_size=16)
+    assert status.item() == 8 and left.item() == 4 and lens.tolist() == [20, 9]
+    assert table.tolist() == [[3, 4], [5, -1]] and free.tolist() == [0, 1, 2, 9, 9, 9]
+    t = ss.PageTables(n_pages=4, page_size=16, max_requests=2, max_pages=4)
+    t.seq_lens = _i32([40, 0])  # three pages that were never handed out
+    t.release(torch.tensor([True, False], device="cuda"))
+    with pytest.raises(RuntimeError, match="released"):
+        t.check()
+
+
+@pytest.mark.parametrize("d,nq", [(64, 300), (128, 300), (128, 60), (256, 700)])
+def test_attention_many_rows_of_any_stride(ss, d, nq):
+    k = torch.randn((1000 + nq, 2, d), generator=_gen(1), device="cuda")
+    pool, row = _filled(ss, k, torch.randn_like(k))
+    qkv = torch.randn((nq, 12, d), generator=_gen(2), device="cuda").half()
+    q = qkv[:, :8]
+    odd = torch.zeros(nq * 8 * d + 1, dtype=torch.float16, device="cuda")[1:].view(nq, 8, d)
+    odd.copy_(q)  # 2-byte aligned
+    args = pool, row[None], _i32([1000 + nq]), _i32([0, nq]), 0.1
+    o, lse = ss.int4_attention(q.contiguous(), *args, max_q=nq, return_lse=True)
+    for x in (q, odd, q.transpose(0, 1).contiguous().transpose(0, 1)):
+        o2, lse2 = ss.int4_attention(x, *args, max_q=nq, return_lse=True)
+        assert torch.equal(o2, o) and torch.equal(lse2, lse)
+    kr, vr = ss.int4_fetch(torch.arange(1000 + nq, device="cuda"), pool, d)
+    want, wl, pv, mag = R.attention(q, kr, vr, 1000 + nq, 0.1)
+    u = 2.0 ** -11
+    assert ((o.double() - want).abs() <= u * want.abs() + (4 * u + 2 * u * mag[..., None]) * pv + 1e-7).all()
+    assert ((lse.double() - wl).abs() <= u * mag + 1e-5 * (1 + wl.abs())).all()
