@@ -754,9 +754,8 @@ int launch_shape(AttnParams& p, cudaStream_t st) {
   static_assert(Sh::kSmem <= 227 * 1024 / Sh::kCtas, "shared memory");
   const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, MODE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   if (e != cudaSuccess) return fail(SS_ERR_CUDA, std::string("ss_int4_attention: ") + cudaGetErrorString(e));
-  p.n_slots = sm_count() * Sh::kCtas;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.n_slots);
+  cfg.gridDim = dim3(sm_count() * Sh::kCtas);
   cfg.blockDim = dim3(Sh::W * 32);
   cfg.dynamicSmemBytes = Sh::kSmem;
   cfg.stream = st;

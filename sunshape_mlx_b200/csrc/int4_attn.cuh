@@ -30,7 +30,6 @@ struct AttnParams {
   float* parts;   // and their parts: a place that does not depend on the kernel's shape
   uint32_t* tile_ws;  // the tile kernel's counters, 4 per unit
   float* tile_parts;  // and its parts, one per CTA
-  int n_slots;  // CTAs of the warp-MMA kernel
   int tiles;    // the tile kernel runs too
   int64_t tile_units;  // about how many units it has at most
   uint64_t wait_ns;   // bound of its waits

@@ -152,16 +152,18 @@ const char* ss_last_error(void) { return ss::g_last_error.c_str(); }
 int ss_device_sm_count(void) { return ss::sm_count(); }
 
 int ss_stream_capture_id(void* stream, unsigned long long* id) {
-  if (!id) return ss::fail(SS_ERR_BAD_ARG, "ss_stream_capture_id: null pointer");
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  unsigned long long now = 0;
-  const cudaError_t e = cudaStreamGetCaptureInfo(ss::as_stream(stream), &status, &now);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return ss::fail(SS_ERR_CUDA, std::string("ss_stream_capture_id: ") + cudaGetErrorString(e));
-  }
-  *id = status == cudaStreamCaptureStatusActive ? now : 0;
-  return SS_OK;
+  return ss::c_entry([&]() -> int {
+    SS_REQUIRE(id, "ss_stream_capture_id: null pointer");
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long now = 0;
+    const cudaError_t e = cudaStreamGetCaptureInfo(ss::as_stream(stream), &status, &now);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return ss::fail(SS_ERR_CUDA, std::string("ss_stream_capture_id: ") + cudaGetErrorString(e));
+    }
+    *id = status == cudaStreamCaptureStatusActive ? now : 0;
+    return SS_OK;
+  });
 }
 
 int ss_set_error_sink(int* host_word) {
