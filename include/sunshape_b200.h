@@ -384,8 +384,9 @@ int ss_decode_attn_partial(const ss_decode_args* a, float* part_out, void* strea
 
 /* Block tables and slot maps of one step, from n requests' lengths (n <= 16384).
  * Request b holds seq_lens[b] tokens and brings q_lens[b] (negative: 0). New
- * pages are popped from the stack free_pages[0 .. n_free[0]) in request order
- * and entered into block_table (rows of table_stride ints, width used). Writes
+ * pages are popped from the stack free_pages[0 .. n_free[0]) in request order;
+ * it has n_pages places, one for every page of the pool. They are entered
+ * into block_table (rows of table_stride ints, width used). Writes
  *   cu_q[n + 1]      first token of each request
  *   positions, requests, slots [n_tokens]   of each token; 0, -1, -1 past the last
  *   new_lens[n], new_free[1]                lengths and free pages after the step

@@ -9,10 +9,13 @@
 // Split. A unit is (request, kv-head, up to R query rows): the rows share its
 // keys, so a block is read once for all of them. The blocks of all units in a
 // row are cut into ranges of equal cost, one per CTA (persistent, one or two CTAs
-// on an SM); a unit cut by a range boundary leaves partial (o, m, l) rows in the
-// workspace and the last CTA to arrive joins them in the order of the ranges,
-// so results do not depend on timing. Lengths are read on the GPU: nothing
-// waits for the host.
+// on an SM). Every unit of a request counts the same keys, those that any of its
+// rows sees: right for single tokens; of a long causal prompt (256 dims come here)
+// the first units cost less than they count, and of one with a window the last
+// units read keys that only the first rows see, and mask them. A unit
+// cut by a range boundary leaves partial (o, m, l) rows in the workspace and the
+// last CTA to arrive joins them in the order of the ranges, so results do not
+// depend on timing. Lengths are read on the GPU: nothing waits for the host.
 //
 // One warp takes two 16-token blocks at a time (one for D = 256 and for 16 rows,
 // whose state fills the registers), with its own ring of cp.async copies (20 D
@@ -37,13 +40,14 @@
 // The softmax reference of a row moves only when a logit comes 5.5 (base
 // 2) above the largest so far: the usual block needs one vote and no shuffles.
 //
-// Measured (D = 128, 8 kv heads): 1 request of 524288 tokens, 64 heads, fp16 149 us
-// (4.5 TB/s); 32 requests of 500 to 16384 tokens, bf16 87 us (4.1 TB/s); 1 of 777
-// tokens 12 us. HBM would allow 103 and 55 us: a block costs about 340 warp
+// Measured (D = 128, 8 kv heads), calls on end for half a second, in brackets bursts
+// of graph replays: 1 request of 524288 tokens, 64 heads, fp16 164 us (4.1 TB/s;
+// 147 us); 32 requests of 500 to 16384 tokens, bf16 90 us (4.0 TB/s; 86 us); 1 of 777
+// tokens 14 us (12 us). HBM would allow 103 and 55 us: a block costs about 340 warp
 // instructions, 57 % of the issue slots at that rate, and what is left is
-// latency within a warp's block (the registers hold 12 warps an SM). One block at
-// a time took 163 and 123 us; keys rounded from nibbles to fp16 by conversions
-// 179 and 129 us.
+// latency within a warp's block (the registers hold 12 warps an SM). In bursts, one
+// block at a time took 163 and 123 us; keys rounded from nibbles to fp16 by
+// conversions 179 and 129 us.
 #include <algorithm>
 
 #include "int4_attn.cuh"

@@ -9,11 +9,12 @@
 //
 // A row is read once and 5 bits per value are written: HBM is the floor, but
 // quantising costs about 10 instructions a value, so a write of 16-bit rows is
-// bound by issue (70 % of the slots): two lanes a group, 16 keys and 16 values
+// bound by issue (74 % of the slots): two lanes a group, 16 keys and 16 values
 // a thread, so that what a row costs once (slot, page, addresses) is shared by
-// 32 values. 49999 tokens x 8 heads x 128: write 72 us from fp16 (3.7 TB/s), 80
-// us from fp32 (5.9 TB/s); with 8 + 8 values a thread it was 96 us. Read back
-// 55 us to fp16 (4.9 TB/s).
+// 32 values. 49999 tokens x 8 heads x 128, every 7th of them padding, calls on end:
+// write 68 us from fp16 (3.4 TB/s), 77 from bf16, 81 from fp32 (5.0 TB/s); with 8 + 8
+// values a thread it was 96 us from fp16. Read back 51 us to fp16 (5.1 TB/s); 121 us
+// to fp32 (3.8 TB/s).
 #include "int4_pages.cuh"
 
 namespace ss {

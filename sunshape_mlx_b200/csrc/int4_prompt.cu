@@ -29,13 +29,14 @@
 // and both products accumulate in fp32. O in TMEM is rescaled only when a logit
 // comes 5.5 (base 2) above the row's largest so far.
 //
-// Measured: one causal prompt of 8192 tokens, 32 query heads on 8, D = 128: bf16
-// 860 us (640 TFLOP/s of the formula's 4 D a pair; the tensor cores do half as
-// much again for lo), fp16 1013 us, D = 64 685 us. A tile of 128 keys takes
-// 1.9 us: the tensor pipe is busy 40 % of the time, issue slots 55 %, shared
+// Measured: one causal prompt of 8192 tokens, 32 query heads on 8, calls on end for
+// half a second: D = 128 bf16 938 us (586 TFLOP/s of the formula's 4 D a pair; the
+// tensor cores do half as much again for lo), fp16 1150 us, D = 64 688 us. In bursts,
+// before the power limit lowers the clocks, 870, 1035 and 690 us; the figures below
+// are such bursts. A tile of 128 keys takes 1.9 us: the tensor pipe is busy 40 % of the time, issue slots 55 %, shared
 // memory 46 %; no one of them is full, the chain decode - S - softmax - O of two
 // tiles in flight is (a third tile has no room: two stages take 205 KB, and S, P,
-// O and Q all 512 TMEM columns). A softmax thread per row instead of two: 910 us;
+// O and Q all 512 TMEM columns). When the kernel took 860 us, a softmax thread per row instead of two: 910 us;
 // tiles of 64 keys 1322; Q and P in shared memory 1598. The registers follow from
 // what a role keeps: with fewer than 120 the softmax spills O's rescale, and 28
 // warps (16 decoding) at 72 took 1421 us.

@@ -13,8 +13,9 @@
 //
 // A launch writes a few KB to a MB, so latency is all: one launch, in which every
 // CTA scans all requests' needs by itself (two ints each, read from L2) rather
-// than wait for a first kernel's sums. 64 requests 4.6 us, 1500 requests with
-// prompt chunks 7.5 us, of which an empty kernel is 2.5.
+// than wait for a first kernel's sums. 64 requests 4.0 us, 1500 requests with
+// prompt chunks 7.2 us (graph replays), of which an empty kernel is 2.5; through the
+// API 10 us either way.
 #include "common.cuh"
 
 namespace ss {

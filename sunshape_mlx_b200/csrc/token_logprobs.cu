@@ -24,9 +24,10 @@
 // Bound by HBM; an element costs about 5.5 issue slots, one of them exp2, at
 // half of what an SM can issue at full bandwidth. 256 threads and five CTAs an
 // SM, so that rows in their last phase overlap rows that stream: 2047 x 128256
-// bf16, top 8: 103.5 us (5.1 TB/s); with loads of 16 bytes, of whose sectors the
-// second reading used half, 109 us, and then 112 with 512 threads and two CTAs.
-// 333 x 50257 fp32, top 5: 16 us; one row of 128256: 9.5 us, latency.
+// bf16, top 8: calls on end 110 to 114 us (4.7 TB/s), bursts of graph replays 104 to
+// 106 us; with loads of 16 bytes, of whose sectors the second reading used half,
+// 109 us in bursts, and then 112 with 512 threads and two CTAs. 333 x 50257 fp32,
+// top 5: 16 us, and 17 to 21 with the host's calls; one row of 128256: 10 us, latency.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -91,7 +91,9 @@ def plan_step(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_table: torch.T
     New pages are popped from the stack ``free_pages[:n_free]`` and entered
     into ``block_table`` (n, width), the only argument that changes: lengths
     and the count of free pages after the step are returned, so a repeated
-    call repeats its result. ``n_tokens`` is the number of token places (a
+    call repeats its result. The stack has a place for every page of the pool
+    (its length is the pool's size: a page past it maps to slot -1).
+    ``n_tokens`` is the number of token places (a
     step of fewer tokens leaves slots of -1 at the end). If the step does not
     fit, nothing is allocated and ``status`` says why.
     """
@@ -171,7 +173,7 @@ def _check_slots(slots: torch.Tensor, n: int, index: int) -> None:
 def int4_append(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor) -> None:
     """Quantises keys and values (n, n_kv_heads, head_dim), fp32, fp16 or
     bf16, into the pages at ``slots`` (n,) int64; -1 skips a token. Slots of
-    one call must differ. Magnitudes above 2^15 saturate; a NaN makes its
+    one call must differ. No gradient reaches what is stored. Magnitudes above 2^15 saturate; a NaN makes its
     group of 32 dims read as NaN."""
     if (L._fast or L.fast()).append(keys, values, slots, pages):
         return
@@ -225,7 +227,9 @@ def int4_attention(queries: torch.Tensor, pages: torch.Tensor, block_table: torc
     ``seq_lens[b]`` tokens of row b of ``block_table`` (the new tokens
     included), and stand at its last positions. ``causal`` hides later keys;
     ``window > 0`` also hides keys at ``position - window`` and before.
-    ``max_q`` is the most query tokens of a request. Returns the output
+    ``max_q`` is the most query tokens of a request. Stored values enter as
+    fp16(code * scale + zero), probabilities as fp16 (as a sum of two where the
+    output is fp16); sums are fp32. Returns the output
     (n_tokens, n_q_heads, head_dim) in the queries' dtype and, with
     ``return_lse``, the natural log-sum-exp (n_tokens, n_q_heads) in fp32. A
     row that sees no key gives 0 and -inf, as does a token outside ``cu_q``.

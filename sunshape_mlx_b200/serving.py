@@ -9,8 +9,10 @@ step here is
   logits    of the rows that are needed
   logprobs  token_logprobs: of given tokens, with entropy and alternatives
 
-all on the GPU: prompts, parts of prompts and single tokens share a step, and
-nothing is read back but the tokens. ``PagedServer`` generates and scores;
+all on the GPU: ``forward_paged`` takes prompts, parts of prompts and single
+tokens in one step, whatever ``plan`` placed. ``PagedServer`` generates and
+scores: new prompts in parts, all of them together, then one token a step for
+every running request;
 
     python -m sunshape_mlx_b200.serving
 
@@ -72,10 +74,11 @@ class PagedServer:
     """A server's loop over at most ``max_requests`` requests at a time.
 
     ``start`` takes prompts into free rows and runs them (in parts of at most
-    ``chunk`` tokens each, together), ``step`` generates one token for every
-    running request, ``stop`` frees the pages of requests. The host keeps what
-    a scheduler knows anyway (lengths, free rows and pages); no call waits for
-    the GPU.
+    ``chunk`` tokens each, together; requests that run already wait until the
+    last part is in), ``step`` generates one token for every running request,
+    ``stop`` frees the pages of requests. The host keeps what a scheduler knows
+    anyway (lengths, free rows and pages); ``start`` waits for the GPU when it
+    copies its prompts, no other call does.
     """
 
     def __init__(self, model: Decoder, *, n_pages: int, page_size: int = 64, max_requests: int = 16,
@@ -147,7 +150,9 @@ class PagedServer:
     def step(self) -> tuple[torch.Tensor, TokenLogprobs]:
         """Feeds every running request its next token. Returns the ids that
         were fed (in the order of the request numbers) and what
-        ``token_logprobs`` says of the greedy token after each."""
+        ``token_logprobs`` says of the greedy token after each. Raises, with
+        nothing changed, while a request holds ``max_tokens`` or the pool has
+        too few pages for all: ``stop`` one first."""
         reqs = sorted(self.lens)
         if not reqs:
             raise RuntimeError("no request is running")
