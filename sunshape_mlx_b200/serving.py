@@ -94,7 +94,8 @@ class PagedServer:
         return -(-tokens // self.tables.page_size)
 
     def _run(self, new: dict[int, int], ids: torch.Tensor, rows: torch.Tensor | None):
-        """One step of `new` tokens per request, in the order of the request rows."""
+        """One step of `new` tokens per request, in the order of the request rows. One that
+        raises leaves lengths and pages as they were."""
         for r, q in new.items():
             if self.lens[r] + q > self.max_tokens:
                 raise ValueError(f"request {r} would hold more than {self.max_tokens} tokens")
@@ -103,9 +104,17 @@ class PagedServer:
         q = torch.zeros(self.tables.block_table.shape[0], dtype=torch.int32)
         for r, c in new.items():
             q[r] = c
+        t = self.tables
+        before = t.seq_lens, t.n_free
+        try:
+            plan = t.plan(q.to(self.model.device, non_blocking=True), ids.shape[0])
+            logits = forward_paged(self.model, ids, plan, self.caches, max_q=max(new.values()), rows=rows)
+        except BaseException:
+            t.seq_lens, t.n_free = before  # a plan changes nothing else but table entries past these lengths
+            raise
+        for r, c in new.items():
             self.lens[r] += c
-        plan = self.tables.plan(q.to(self.model.device, non_blocking=True), ids.shape[0])
-        return forward_paged(self.model, ids, plan, self.caches, max_q=max(new.values()), rows=rows)
+        return logits
 
     def start(self, prompts: list[torch.Tensor]) -> tuple[list[int], list[TokenLogprobs]]:
         """Takes prompts (1-D tensors of at least one id of the vocabulary) in

@@ -301,6 +301,43 @@ def test_server_refuses_ids_outside_the_vocabulary(ss):
     assert reqs == [0, 1]
 
 
+def test_server_goes_on_after_a_step_that_failed(ss, monkeypatch):
+    """A layer that raises leaves the requests where they were: the next step is the one that failed."""
+    from sunshape_mlx_b200.harness import Decoder, DecoderConfig
+    from sunshape_mlx_b200.paged import Int4PagedKVCache
+    from sunshape_mlx_b200.serving import PagedServer
+
+    model = Decoder(DecoderConfig(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, ffn=256, vocab=97), seed=1)
+    prompts = [torch.arange(15), torch.arange(32) % 7]  # the next token of either one takes a page
+
+    def serve(fail):
+        server = PagedServer(model, n_pages=8, page_size=16, max_requests=2, max_tokens=64, top_k=3)
+        server.start(prompts)
+        got = [server.step()]
+        if fail:
+            real = Int4PagedKVCache.append
+
+            def broken(self, *a):
+                if self is server.caches[1]:
+                    raise torch.cuda.OutOfMemoryError("no memory")
+                real(self, *a)
+
+            with monkeypatch.context() as m:
+                m.setattr(Int4PagedKVCache, "append", broken)
+                before = dict(server.lens), server.tables.n_free.item()
+                for _ in range(2):
+                    with pytest.raises(torch.cuda.OutOfMemoryError):
+                        server.step()
+                assert (server.lens, server.tables.n_free.item()) == before
+        got += [server.step() for _ in range(3)]
+        server.tables.check()
+        assert server.lens == {0: 19, 1: 36} and server.tables.n_free.item() == 3
+        return got
+
+    for (a, la), (b, lb) in zip(serve(True), serve(False)):
+        assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(la, lb))
+
+
 def test_the_same_results_without_the_native_lane(ss, monkeypatch):
     from sunshape_mlx_b200 import _lib as L
 
